@@ -304,6 +304,151 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
                         const int64_t b_strides[2], int64_t m, int64_t k, int64_t n, float* out,
                         void* stream);
 
+/* ---- device operators (no counterpart in the reference: a recorded plan can only unroll a
+ *      recurrence over time, holds no sine or cosine, and composes a loss from whole arrays)
+ * Operators of a decoder that lie around its matrix products, for callers that hold their own
+ * device memory.  They share these rules:
+ *  - All array pointers are DEVICE pointers on the calling thread's current device, and `stream`
+ *    is one of its streams (a cudaStream_t; NULL = the legacy default stream).  Work is enqueued on `stream` and the call
+ *    returns; nothing is allocated, no state is kept between calls, and scratch is the caller's
+ *    `workspace`, so calls on several streams or in several captured graphs do not meet as long
+ *    as their workspaces and outputs differ.  Every call may be captured.
+ *  - `element` is the storage of the large arrays: TB_ELEMENT_F32, or TB_ELEMENT_BF16 as 16-bit
+ *    values.  Arithmetic, statistics, states, sums and weights are f32 (sums of a whole sequence
+ *    or batch f64), rounded once to the storage type.  Base addresses are multiples of the
+ *    element size; strides count elements and are not negative; the last axis has stride 1.
+ *  - Results do not depend on scheduling: the same call gives the same bits.
+ *  - A malformed request answers TB_INVALID before anything is enqueued, a launch failure
+ *    TB_RUNTIME (and poisons the library).  Index values on the device (offsets, positions,
+ *    targets) are not seen by the host: the kernels keep every access in bounds whatever they
+ *    hold, and each operator says what a bad one gives.
+ *  - Outputs do not overlap inputs or each other, except where an operator allows it.
+ *  - Packed batches: `offsets` holds sequences + 1 ascending row numbers; rows
+ *    [offsets[s], offsets[s + 1]) are sequence s, which may be empty.  Rows before the first or
+ *    behind the last offset belong to none and their outputs are left as they were. */
+
+/* How the gate array of the gated scan is read. */
+enum {
+  TB_SCAN_DIRECT = 0,   /* h_t = gate_t h_{t-1} + x_t */
+  TB_SCAN_SIGMOID = 1   /* a = sigmoid(gate_t): h_t = a h_{t-1} + (1 - a) x_t */
+};
+typedef struct tb_scan_desc {
+  int64_t element, form;
+  int64_t batch, length, channels;  /* arrays [batch][length][channels] */
+  int64_t sequences;                /* packed sequences in a batch of 1, or 0: each batch row is one */
+  /* (batch, time) strides of gate, x, h, dh, dgate, dx; unused ones are ignored */
+  int64_t gate_strides[2], x_strides[2], h_strides[2], dh_strides[2], dgate_strides[2], dx_strides[2];
+  const void* gate;
+  const void* x;
+  void* h;                          /* written by the scan, read by its backward pass */
+  const int32_t* offsets;           /* sequences + 1, or NULL */
+  const float* state;               /* h before the first step, [sequences or batch][channels]; NULL = 0 */
+  float* final_state;               /* h after the last step, same shape; NULL = not wanted */
+  const void* dh;
+  const float* dfinal;              /* gradient of final_state; NULL = 0 */
+  void* dgate;
+  void* dx;
+  float* dstate;                    /* gradient of state; NULL = not wanted */
+} tb_scan_desc;
+/* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
+ * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
+ * final state is its state. */
+int tb_gated_scan(const tb_scan_desc* desc, void* stream);
+/* Its gradients from dh and dfinal: with g_t = dh_t + a_{t+1} g_{t+1}, d a_t = g_t h_{t-1},
+ * d b_t = g_t, chained through the form.  Reads the saved outputs h.  `dstate` may be `dfinal`;
+ * `dgate` and `dx` may be `dh` with its strides (one of them). */
+int tb_gated_scan_backward(const tb_scan_desc* desc, void* stream);
+
+/* Which elements of a head are turned together. */
+enum {
+  TB_ROTATE_HALVES = 0,  /* i and i + turned/2, i < turned/2 */
+  TB_ROTATE_PAIRS = 1    /* 2i and 2i + 1 */
+};
+typedef struct tb_rotate_desc {
+  int64_t element, style;
+  int64_t batch, length, q_heads, k_heads, dim;  /* q [batch][length][q_heads][dim], k likewise; dim even, <= 512 */
+  int64_t turned;                   /* leading elements of a head that are turned: even, <= dim */
+  int64_t table_rows;
+  /* (batch, token, head) strides */
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3], dq_strides[3], dk_strides[3];
+  double epsilon;                   /* >= 0 */
+  const void* q;
+  const void* k;                    /* unused when k_heads = 0; q likewise */
+  const float* table;               /* [table_rows][turned]: turned/2 cosines, then the sines */
+  const int32_t* positions;         /* [batch][length] rows of the table; NULL = 0 .. length - 1 */
+  const float* q_weight;            /* [dim]; NULL = ones */
+  const float* k_weight;
+  void* q_out;                      /* outputs; in the backward pass the gradients of q and k */
+  void* k_out;
+  const void* dq;                   /* gradients of the outputs (backward) */
+  const void* dk;
+  float* dq_weight;                 /* [dim]; NULL = not wanted */
+  float* dk_weight;
+  void* workspace;                  /* backward with a weight gradient: tb_head_rotate_workspace bytes */
+  int64_t workspace_bytes;
+} tb_rotate_desc;
+/* Root-mean-square norm of every query and key head, x / sqrt(mean(x^2) + epsilon) * weight, then
+ * the rotation by the token's position, in one pass.  A position outside the table turns its
+ * token's heads into NaN.  q_out may be q (k_out k) with the same strides. */
+int tb_head_rotate(const tb_rotate_desc* desc, void* stream);
+/* Gradients of q, k and the weights.  q_out may be dq (k_out dk), or q (k), with the same strides. */
+int tb_head_rotate_backward(const tb_rotate_desc* desc, void* stream);
+/* Bytes of workspace that the backward pass of this request needs (16-byte aligned; may be 0). */
+int64_t tb_head_rotate_workspace(const tb_rotate_desc* desc);
+
+/* log softmax(scale * logits[n])[targets[n]] of every row.  A row counts as hidden where its
+ * target is negative or its logits are all -inf: its log probability is 0.  A target of vocab or
+ * more gives NaN.  scale > 0 is the inverse temperature. */
+int tb_token_logp(int64_t element, const void* logits, int64_t row_stride, const int32_t* targets,
+                  int64_t rows, int64_t vocab, double scale, float* logp, void* stream);
+
+typedef struct tb_policy_desc {
+  int64_t element, rows, vocab;
+  int64_t logits_stride, gradient_stride;  /* elements between rows */
+  double scale;                     /* inverse temperature, > 0 */
+  double clip_low, clip_high;       /* the ratio is held within [1 - clip_low, 1 + clip_high] */
+  double kl;                        /* weight of the KL term, >= 0 */
+  const void* logits;
+  const int32_t* targets;           /* sampled tokens */
+  const float* old_logp;            /* their log probabilities when sampled */
+  const float* ref_logp;            /* under the reference model; may be NULL when kl = 0 */
+  const float* advantages;
+  const float* weights;             /* per row, the normalizer folded in; 0 hides the row */
+  float* loss;                      /* 1 */
+  float* token_loss;                /* rows; the weighted terms that loss sums */
+  float* logp;                      /* rows */
+  void* gradient;                   /* rows x vocab, of loss by logits; NULL = not wanted */
+} tb_policy_desc;
+/* Clipped policy loss with its gradient.  With logp_n as in tb_token_logp, r = exp(logp - old),
+ * d = ref - logp:  loss = sum_n weight_n (-min(r A_n, clamp(r) A_n) + kl (exp(d) - d - 1)).
+ * A hidden row (weight 0, or as in tb_token_logp) adds nothing, whatever it holds, and has a
+ * gradient of 0.  `gradient` may be `logits` with its stride. */
+int tb_policy_loss(const tb_policy_desc* desc, void* stream);
+
+typedef struct tb_preference_desc {
+  int64_t element, rows, vocab, pairs;
+  int64_t logits_stride, gradient_stride;
+  double scale;                     /* inverse temperature, > 0 */
+  double beta;                      /* > 0 */
+  double smoothing;                 /* in [0, 1): the share of pairs that are labelled the wrong way */
+  const void* logits;
+  const int32_t* targets;           /* negative: hidden (a prompt's token) */
+  const int32_t* offsets;           /* 2 * pairs + 1: the chosen answers, then the rejected ones */
+  const float* ref_logp;            /* per row */
+  const float* weights;             /* per pair; NULL = 1 / pairs */
+  float* loss;                      /* 1 */
+  float* ratios;                    /* 2 * pairs: sum of logp - ref over each answer */
+  float* logp;                      /* rows */
+  void* gradient;                   /* rows x vocab; NULL = not wanted */
+  void* workspace;                  /* tb_preference_workspace bytes */
+  int64_t workspace_bytes;
+} tb_preference_desc;
+/* Paired log-ratio loss with its gradient: m_i = beta (ratio_i - ratio_{pairs + i}),
+ * loss = sum_i weight_i (-(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)).
+ * `gradient` may be `logits` with its stride. */
+int tb_preference_loss(const tb_preference_desc* desc, void* stream);
+int64_t tb_preference_workspace(const tb_preference_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,6 +53,51 @@ class TbOptimizerDesc(C.Structure):
                 ("gradient_scale", C.c_float)]
 
 
+# Requests of the device operators: every field is 8 bytes wide, so one list of names describes a
+# struct both for ctypes and for packing it in one go.
+def _request(name, **groups):
+    fields = []
+    for kind, names in groups.items():
+        of = {"longs": C.c_int64, "doubles": C.c_double, "pointers": C.c_void_p}[kind.split("_")[0]]
+        for field in names.split():
+            field, _, count = field.partition(":")
+            fields.append((field, of * int(count) if count else of))
+    return type(name, (C.Structure,), {"_fields_": fields})
+
+
+TbScanDesc = _request(
+    "TbScanDesc",
+    longs="element form batch length channels sequences gate_strides:2 x_strides:2 h_strides:2 "
+          "dh_strides:2 dgate_strides:2 dx_strides:2",
+    pointers="gate x h offsets state final_state dh dfinal dgate dx dstate")
+TbRotateDesc = _request(
+    "TbRotateDesc",
+    longs="element style batch length q_heads k_heads dim turned table_rows q_strides:3 "
+          "k_strides:3 q_out_strides:3 k_out_strides:3 dq_strides:3 dk_strides:3",
+    doubles="epsilon",
+    pointers="q k table positions q_weight k_weight q_out k_out dq dk dq_weight dk_weight "
+             "workspace",
+    longs_last="workspace_bytes")
+TbPolicyDesc = _request(
+    "TbPolicyDesc",
+    longs="element rows vocab logits_stride gradient_stride",
+    doubles="scale clip_low clip_high kl",
+    pointers="logits targets old_logp ref_logp advantages weights loss token_loss logp gradient")
+TbPreferenceDesc = _request(
+    "TbPreferenceDesc",
+    longs="element rows vocab pairs logits_stride gradient_stride",
+    doubles="scale beta smoothing",
+    pointers="logits targets offsets ref_logp weights loss ratios logp gradient workspace",
+    longs_last="workspace_bytes")
+
+
+def request_format(desc) -> str:
+    """The `struct` format of an operator's request."""
+    code = {C.c_int64: "q", C.c_double: "d", C.c_void_p: "Q"}
+    return "<" + "".join(code[getattr(of, "_type_", of)] * getattr(of, "_length_", 1)
+                         if issubclass(of, C.Array) else code[of] for _, of in desc._fields_)
+
+
 def fptr(array: np.ndarray):
     return array.ctypes.data_as(C.POINTER(C.c_float))
 
@@ -228,6 +273,17 @@ def load_library() -> C.CDLL:
         "tb_gemm_f32_noalloc": (C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.c_void_p,
                                           C.POINTER(C.c_int64), C.c_int64, C.c_int64, C.c_int64,
                                           C.c_void_p, C.c_void_p]),
+        # the operators' requests are passed as packed bytes
+        "tb_gated_scan": (C.c_int, [C.c_char_p, P]),
+        "tb_gated_scan_backward": (C.c_int, [C.c_char_p, P]),
+        "tb_head_rotate": (C.c_int, [C.c_char_p, P]),
+        "tb_head_rotate_backward": (C.c_int, [C.c_char_p, P]),
+        "tb_head_rotate_workspace": (C.c_int64, [C.c_char_p]),
+        "tb_token_logp": (C.c_int, [C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_double,
+                                    P, P]),
+        "tb_policy_loss": (C.c_int, [C.c_char_p, P]),
+        "tb_preference_loss": (C.c_int, [C.c_char_p, P]),
+        "tb_preference_workspace": (C.c_int64, [C.c_char_p]),
     }
     for name, (restype, argtypes) in sigs.items():
         fn = getattr(lib, name)

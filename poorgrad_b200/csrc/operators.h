@@ -1,0 +1,107 @@
+// operators.h -- what the device operators (scan.cu, rotate.cu, losses.cu) share:
+// storage types and the frame of a C entry point.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <exception>
+
+#include "../../include/topos_b200.h"
+#include "kernels.h"
+#include "launch.h"
+
+namespace tb {
+
+typedef __nv_bfloat16 bf16;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
+
+// The frame of an operator's entry point: the request is checked first, then the library's
+// state, then the work is enqueued on the caller's stream.
+class OperatorCall {
+ public:
+  OperatorCall(const char* name, void* stream) : name_(name), stream_((cudaStream_t)stream) {}
+  cudaStream_t stream() const { return stream_; }
+
+  int invalid(const char* why) const {
+    char text[256];
+    snprintf(text, sizeof text, "%s: %s", name_, why);
+    set_last_error(text);
+    return TB_INVALID;
+  }
+
+  // TB_OK when work may be enqueued.
+  int ready() {
+    static std::atomic<bool> device_seen{false};
+    if (!device_seen.load(std::memory_order_relaxed)) {
+      int count = 0;
+      if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+        cudaGetLastError();
+        return fail(TB_PLATFORM_UNSUPPORTED, "no CUDA device");
+      }
+      device_seen.store(true, std::memory_order_relaxed);
+    }
+    if (poisoned()) return fail(TB_POISONED, "the backend is poisoned");
+    cudaGetLastError();  // a launch error left by earlier, unrelated work is not this call's
+    return TB_OK;
+  }
+
+  // The launches' outcome.
+  int finish(cudaError_t e) const {
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e == cudaSuccess) return TB_OK;
+    // a handle of another device or none at all: nothing ran, and the device is well
+    if (e == cudaErrorInvalidResourceHandle || e == cudaErrorContextIsDestroyed)
+      return invalid("the stream is not one of the current device");
+    char text[256];
+    snprintf(text, sizeof text, "%s: %s", name_, cudaGetErrorString(e));
+    poison_library(text);
+    return TB_RUNTIME;
+  }
+
+ private:
+  int fail(int code, const char* why) const {
+    char text[256];
+    snprintf(text, sizeof text, "%s: %s", name_, why);
+    set_last_error(text);
+    return code;
+  }
+  const char* name_;
+  cudaStream_t stream_;
+};
+
+// Runs an entry point's body; no C++ exception leaves the library.
+template <typename F>
+inline int guarded(F body) noexcept {
+  try {
+    return body();
+  } catch (const std::exception&) {
+    return TB_RUNTIME;
+  } catch (...) {
+    return TB_RUNTIME;
+  }
+}
+
+inline bool aligned_to(const void* p, int64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+// Extents a request may have: each, and their product, far below what 64-bit sizes hold.
+inline bool extents_fit(std::initializer_list<int64_t> extents) {
+  double product = 1;
+  for (int64_t e : extents) {
+    if (e < 0 || e > (int64_t(1) << 40)) return false;
+    product *= e > 0 ? (double)e : 1.0;
+  }
+  return product < (double)(int64_t(1) << 44);
+}
+
+}  // namespace tb

@@ -1,0 +1,381 @@
+"""Python face of the device operators of ``include/topos_b200.h``: what lies around the matrix
+products of a decoder's training and decode steps, on device arrays that the caller holds.
+
+- :func:`gated_scan`, :func:`gated_scan_backward` -- the gated linear recurrence over time
+- :func:`head_rotate`, :func:`head_rotate_backward` -- norms of query and key heads with the
+  position rotation; :func:`rotation_table` makes its cosines and sines
+- :func:`token_logp`, :func:`policy_loss`, :func:`preference_loss` -- losses over a vocabulary
+  with their gradients by the logits
+
+Device arrays are torch tensors (float32 or bfloat16), used as memory only: nothing here records
+gradients.  Arguments of one call live on one device; the work is enqueued on that device's current
+torch stream, and outputs that are not given are allocated by torch on that stream.  A malformed
+request raises ``ValueError`` or :class:`~poorgrad_b200.backend.BackendError`; there is no CPU
+fallback.
+"""
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple, Optional
+
+import numpy as np
+import torch
+
+from .abi import (TbPolicyDesc, TbPreferenceDesc, TbRotateDesc, TbScanDesc, load_library,
+                  request_format)
+from .backend import BackendError
+
+_ELEMENT = {torch.float32: 0, torch.bfloat16: 1}
+_FORM = {"direct": 0, "sigmoid": 1}
+_STYLE = {"halves": 0, "pairs": 1}
+_scan = struct.Struct(request_format(TbScanDesc)).pack
+_rotate = struct.Struct(request_format(TbRotateDesc)).pack
+_policy = struct.Struct(request_format(TbPolicyDesc)).pack
+_preference = struct.Struct(request_format(TbPreferenceDesc)).pack
+
+
+def _need(condition, what: str):
+    if not condition:
+        raise ValueError(what)
+
+
+def _device_of(first, name: str):
+    _need(isinstance(first, torch.Tensor) and first.is_cuda, f"{name}: a CUDA tensor is expected")
+    return first.device
+
+
+def _array(t, name: str, device, dtype, shape):
+    """Checks a large array: its type, device and shape, and that its last axis has stride 1."""
+    _need(isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype
+          and t.shape == shape,
+          f"{name}: expected {dtype} {tuple(shape)} on {device}, got "
+          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
+    _need(not shape[-1] > 1 or t.stride(-1) == 1, f"{name}: the last axis must have stride 1")
+    return t.data_ptr()
+
+
+def _words(t, name: str, device, dtype, shape):
+    """Checks a contiguous 32-bit array, or None."""
+    if t is None:
+        return 0
+    _need(isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype
+          and t.shape == shape and t.is_contiguous(),
+          f"{name}: expected contiguous {dtype} {tuple(shape)} on {device}, got "
+          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
+    return t.data_ptr()
+
+
+def _call(entry: str, device, *arguments):
+    lib = load_library()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        code = getattr(lib, entry)(*arguments, stream)
+    else:  # the default stream belongs to the current device
+        with torch.cuda.device(device):
+            code = getattr(lib, entry)(*arguments, stream)
+    if code != 0:
+        raise BackendError(code, entry)
+
+
+# ------------------------------------------------------------------ gated scan
+def _scan_extents(x, offsets, device):
+    """(batch, length, channels, sequences, rows of the states)."""
+    if offsets is None:
+        _need(x.dim() == 3, "x: expected [batch, length, channels], or packed [rows, channels] "
+                            "with offsets")
+        batch, length, channels = x.shape
+        return batch, length, channels, 0, batch
+    _need(x.dim() == 2, "x: a packed batch is [rows, channels]")
+    _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 2,
+          "offsets: expected sequences + 1 row numbers")
+    length, channels = x.shape
+    return 1, length, channels, offsets.shape[0] - 1, offsets.shape[0] - 1
+
+
+def _time_strides(t):
+    return (0, t.stride(0)) if t.dim() == 2 else (t.stride(0), t.stride(1))
+
+
+def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=None,
+               final_state=None):
+    """``h_t = a_t h_{t-1} + b_t`` over time; returns ``(h, final_state)``.
+
+    ``form="direct"``: a is ``gate`` and b is ``x``.  ``form="sigmoid"``: a is the sigmoid of
+    ``gate`` and b is ``(1 - a) x``.  ``gate`` and ``x`` are ``[batch, length, channels]``, or a
+    packed ``[rows, channels]`` whose sequences ``offsets`` (int32, sequences + 1 rising row
+    numbers) delimits; rows outside every sequence are left as they were.  ``state`` (float32,
+    ``[batch or sequences, channels]``, zeros when None) comes before the first step; the returned
+    final state may be written into ``state`` itself (``final_state=state``), as a decode loop
+    does.  ``out`` may be ``gate`` or ``x``."""
+    device = _device_of(x, "x")
+    _need(x.dtype in _ELEMENT, "x: float32 or bfloat16 is expected")
+    _need(form in _FORM, f"form: one of {sorted(_FORM)} is expected")
+    batch, length, channels, sequences, count = _scan_extents(x, offsets, device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    if final_state is None:
+        final_state = torch.empty((count, channels), dtype=torch.float32, device=device)
+    shape, dtype = x.shape, x.dtype
+    pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
+                _array(out, "out", device, dtype, shape),
+                _words(offsets, "offsets", device, torch.int32, (sequences + 1,)),
+                _words(state, "state", device, torch.float32, (count, channels)),
+                _words(final_state, "final_state", device, torch.float32, (count, channels)))
+    request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
+                    *_time_strides(gate), *_time_strides(x), *_time_strides(out),
+                    0, 0, 0, 0, 0, 0, *pointers, 0, 0, 0, 0, 0)
+    _call("tb_gated_scan", device, request)
+    return out, final_state
+
+
+def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, offsets=None,
+                        dfinal=None, dgate=None, dx=None):
+    """Gradients ``(dgate, dx, dstate)`` of :func:`gated_scan` from the gradient ``dh`` of its
+    outputs ``h`` and ``dfinal`` of its final state (zeros when None).  ``x`` is read by the
+    sigmoid form only.  One of ``dgate`` and ``dx`` may be ``dh``."""
+    device = _device_of(dh, "dh")
+    _need(dh.dtype in _ELEMENT, "dh: float32 or bfloat16 is expected")
+    _need(form in _FORM, f"form: one of {sorted(_FORM)} is expected")
+    batch, length, channels, sequences, count = _scan_extents(dh, offsets, device)
+    shape, dtype = dh.shape, dh.dtype
+    if dgate is None:
+        dgate = torch.empty(shape, dtype=dtype, device=device)
+    if dx is None:
+        dx = torch.empty(shape, dtype=dtype, device=device)
+    dstate = torch.empty((count, channels), dtype=torch.float32, device=device)
+    if form == "direct" and x is None:
+        x = gate  # not read
+    pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
+                _array(h, "h", device, dtype, shape),
+                _words(offsets, "offsets", device, torch.int32, (sequences + 1,)),
+                _words(state, "state", device, torch.float32, (count, channels)), 0,
+                _array(dh, "dh", device, dtype, shape),
+                _words(dfinal, "dfinal", device, torch.float32, (count, channels)),
+                _array(dgate, "dgate", device, dtype, shape),
+                _array(dx, "dx", device, dtype, shape), dstate.data_ptr())
+    request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
+                    *_time_strides(gate), *_time_strides(x), *_time_strides(h),
+                    *_time_strides(dh), *_time_strides(dgate), *_time_strides(dx), *pointers)
+    _call("tb_gated_scan_backward", device, request)
+    return dgate, dx, dstate
+
+
+# ----------------------------------------------------------------- head rotate
+def rotation_table(rows: int, turned: int, base: float = 10000.0, first: int = 0) -> np.ndarray:
+    """``[rows, turned]`` float32: cosines, then sines, of ``(first + row) * base^(-2i / turned)``
+    for i below turned / 2, computed in 64 bits (a far position's angle needs them)."""
+    _need(turned >= 0 and turned % 2 == 0, "turned is even and not negative")
+    half = turned // 2
+    angles = (np.arange(first, first + rows, dtype=np.float64)[:, None]
+              * base ** (-np.arange(half, dtype=np.float64) / max(half, 1))[None, :])
+    return np.concatenate([np.cos(angles), np.sin(angles)], axis=1).astype(np.float32)
+
+
+def _heads(t):
+    """A [tokens, heads, dim] array as one batch row."""
+    return t.unsqueeze(0) if t.dim() == 3 else t
+
+
+def _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon, style, q_out,
+                    k_out, dq, dk, dq_weight, dk_weight, workspace, workspace_bytes):
+    batch, length, q_heads, dim = q.shape
+    k_heads, dtype = k.shape[2], q.dtype
+    q_shape, k_shape = q.shape, (batch, length, k_heads, dim)
+    _need(isinstance(table, torch.Tensor) and table.dim() == 2,
+          "table: expected [positions, turned]")
+    _need(style in _STYLE, f"style: one of {sorted(_STYLE)} is expected")
+    pointers = (_array(q, "q", device, dtype, q_shape), _array(k, "k", device, dtype, k_shape),
+                _words(table, "table", device, torch.float32, table.shape),
+                _words(positions, "positions", device, torch.int32, (batch, length)),
+                _words(q_weight, "q_weight", device, torch.float32, (dim,)),
+                _words(k_weight, "k_weight", device, torch.float32, (dim,)),
+                _array(q_out, "q_out", device, dtype, q_shape),
+                _array(k_out, "k_out", device, dtype, k_shape))
+    if dq is None:
+        strides, more = (0,) * 6, (0, 0)
+    else:
+        more = (_array(dq, "dq", device, dtype, q_shape), _array(dk, "dk", device, dtype, k_shape))
+        strides = dq.stride()[:3] + dk.stride()[:3]
+    return _rotate(_ELEMENT[dtype], _STYLE[style], batch, length, q_heads, k_heads, dim,
+                   table.shape[1], table.shape[0], *q.stride()[:3], *k.stride()[:3],
+                   *q_out.stride()[:3], *k_out.stride()[:3], *strides, epsilon, *pointers, *more,
+                   dq_weight, dk_weight, workspace, workspace_bytes)
+
+
+def _rotate_inputs(q, k, positions):
+    device = _device_of(q, "q")
+    _need(q.dtype in _ELEMENT, "q: float32 or bfloat16 is expected")
+    _need(q.dim() in (3, 4) and isinstance(k, torch.Tensor) and k.dim() == q.dim(),
+          "q, k: expected [tokens, heads, dim] or [batch, length, heads, dim]")
+    if isinstance(positions, torch.Tensor) and positions.dim() == 1 and q.dim() == 3:
+        positions = positions.unsqueeze(0)
+    return device, positions
+
+
+def head_rotate(q, k, table, positions=None, *, q_weight=None, k_weight=None,
+                epsilon: float = 1e-5, style: str = "halves", q_out=None, k_out=None):
+    """Root-mean-square norm of every query and key head, then its rotation by the token's
+    position; returns ``(q_out, k_out)``.
+
+    ``q`` and ``k`` are ``[batch, length, heads, dim]`` or ``[tokens, heads, dim]`` with any strides
+    but 1 along ``dim`` (views of a joint projection, outputs laid out for attention).  ``table``
+    (float32 ``[positions, turned]``, :func:`rotation_table`) turns the first ``turned`` elements of
+    each head: element i with i + turned/2 (``style="halves"``) or 2i with 2i + 1 (``"pairs"``).
+    ``positions`` (int32, one per token; 0, 1, .. along the length when None) selects the rows; one
+    outside the table makes the token's heads NaN.  Weights are float32 ``[dim]``, ones when None.
+    The outputs may be the inputs."""
+    device, positions = _rotate_inputs(q, k, positions)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
+    if q.dim() == 4:
+        request = _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon,
+                                  style, q_out, k_out, None, None, 0, 0, 0, 0)
+    else:
+        request = _rotate_request(device, _heads(q), _heads(k), table, positions, q_weight,
+                                  k_weight, epsilon, style, _heads(q_out), _heads(k_out), None,
+                                  None, 0, 0, 0, 0)
+    _call("tb_head_rotate", device, request)
+    return q_out, k_out
+
+
+def head_rotate_backward(dq, dk, q, k, table, positions=None, *, q_weight=None, k_weight=None,
+                         epsilon: float = 1e-5, style: str = "halves", q_out=None, k_out=None,
+                         weights: bool = True):
+    """Gradients ``(q_grad, k_grad, q_weight_grad, k_weight_grad)`` of :func:`head_rotate` from the
+    gradients ``dq`` and ``dk`` of its outputs; the last two are float32 ``[dim]``, or None with
+    ``weights=False``.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
+    device, positions = _rotate_inputs(q, k, positions)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
+    dq_weight = dk_weight = workspace = None
+    p = [0, 0, 0, 0]
+    if weights:
+        dim = q.shape[-1]
+        both = torch.empty((2, dim), dtype=torch.float32, device=device)
+        dq_weight, dk_weight = both[0], both[1]
+        size = load_library().tb_head_rotate_workspace
+        draft = _rotate(0, 0, q.shape[0], 1, q.shape[-2], k.shape[-2], dim, *(0,) * 20, 0.0,
+                        *(0,) * 10, dq_weight.data_ptr(), dk_weight.data_ptr(), 0, 0)
+        workspace = torch.empty((size(draft),), dtype=torch.uint8, device=device)
+        p = [dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), workspace.numel()]
+    request = _rotate_request(device, _heads(q), _heads(k), table, positions, q_weight, k_weight,
+                              epsilon, style, _heads(q_out), _heads(k_out), _heads(dq), _heads(dk),
+                              *p)
+    _call("tb_head_rotate_backward", device, request)
+    return q_out, k_out, dq_weight, dk_weight
+
+
+# ---------------------------------------------------------------------- losses
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                  # scalar
+    token_loss: torch.Tensor            # [rows], the weighted terms that loss sums
+    logp: torch.Tensor                  # [rows]
+    gradient: Optional[torch.Tensor]    # [rows, vocab]
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor                  # scalar
+    ratios: torch.Tensor                # [2 pairs], sum of logp - ref over each answer
+    logp: torch.Tensor                  # [rows]
+    gradient: Optional[torch.Tensor]    # [rows, vocab]
+
+
+def _logits(logits):
+    device = _device_of(logits, "logits")
+    _need(logits.dtype in _ELEMENT and logits.dim() == 2,
+          "logits: float32 or bfloat16 [rows, vocab] is expected")
+    return device, _array(logits, "logits", device, logits.dtype, logits.shape)
+
+
+def _gradient_of(logits, gradient, device):
+    """(tensor, pointer, row stride) of a gradient that is wanted (True), given, or neither."""
+    if gradient is None or gradient is False:
+        return None, 0, 0
+    if gradient is True:
+        gradient = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    return gradient, _array(gradient, "gradient", device, logits.dtype,
+                            logits.shape), gradient.stride(0)
+
+
+def token_logp(logits, targets, *, scale: float = 1.0):
+    """Float32 log probabilities of ``targets`` (int32 ``[rows]``) under ``softmax(scale * logits)``
+    of each row.  A hidden row -- a negative target, or no logit above -inf -- gives 0, a target
+    beyond the vocabulary NaN."""
+    device, pointer = _logits(logits)
+    rows, vocab = logits.shape
+    _need(targets is not None, "targets: missing")
+    logp = torch.empty((rows,), dtype=torch.float32, device=device)
+    _call("tb_token_logp", device, _ELEMENT[logits.dtype], pointer, logits.stride(0),
+          _words(targets, "targets", device, torch.int32, (rows,)), rows, vocab, scale,
+          logp.data_ptr())
+    return logp
+
+
+def policy_loss(logits, targets, old_logp, advantages, weights, *, ref_logp=None,
+                clip_low: float = 0.2, clip_high: float = 0.2, kl: float = 0.0,
+                scale: float = 1.0, gradient=True) -> PolicyLoss:
+    """Clipped policy loss over sampled tokens, with its gradient by the logits.
+
+    With ``r = exp(logp - old_logp)`` and ``d = ref_logp - logp``, the loss is the sum over rows of
+    ``weight * (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1))``; the
+    weights hold the normalizer (1 / tokens, say) and hide a row where they are 0.  A hidden row,
+    also one as in :func:`token_logp`, adds nothing whatever it holds and has a gradient of 0.
+    ``gradient`` is True, False, or the array to write, which may be ``logits`` itself."""
+    device, pointer = _logits(logits)
+    rows, vocab = logits.shape
+    _need(targets is not None and old_logp is not None and advantages is not None
+          and weights is not None and (kl == 0 or ref_logp is not None),
+          "targets, old_logp, advantages and weights are needed, and ref_logp where kl is not 0")
+    gradient, to, stride = _gradient_of(logits, gradient, device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    token_loss = torch.empty((rows,), dtype=torch.float32, device=device)
+    logp = torch.empty((rows,), dtype=torch.float32, device=device)
+    f32, shape = torch.float32, (rows,)
+    request = _policy(_ELEMENT[logits.dtype], rows, vocab, logits.stride(0), stride, scale, clip_low,
+                      clip_high, kl, pointer,
+                      _words(targets, "targets", device, torch.int32, shape),
+                      _words(old_logp, "old_logp", device, f32, shape),
+                      _words(ref_logp, "ref_logp", device, f32, shape),
+                      _words(advantages, "advantages", device, f32, shape),
+                      _words(weights, "weights", device, f32, shape),
+                      loss.data_ptr(), token_loss.data_ptr(), logp.data_ptr(), to)
+    _call("tb_policy_loss", device, request)
+    return PolicyLoss(loss, token_loss, logp, gradient)
+
+
+def preference_loss(logits, targets, offsets, ref_logp, *, beta: float = 0.1,
+                    smoothing: float = 0.0, weights=None, scale: float = 1.0,
+                    gradient=True) -> PreferenceLoss:
+    """Paired log-ratio loss over packed answers, with its gradient by the logits.
+
+    ``offsets`` (int32, 2 pairs + 1 rising row numbers) delimits the chosen answers, then the
+    rejected ones in the same order; ``targets`` is negative at rows that are not scored (prompts);
+    ``ref_logp`` holds the reference model's log probability of each row.  With
+    ``m = beta (ratio_chosen - ratio_rejected)`` the loss is the weighted sum (``weights`` float32
+    per pair, 1 / pairs when None) of ``-(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m)``.
+    Rows outside every answer are left as they were.  ``gradient`` as in :func:`policy_loss`."""
+    device, pointer = _logits(logits)
+    rows, vocab = logits.shape
+    _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 3
+          and offsets.shape[0] % 2 == 1, "offsets: expected 2 pairs + 1 row numbers")
+    _need(targets is not None and ref_logp is not None, "targets and ref_logp are needed")
+    pairs = offsets.shape[0] // 2
+    gradient, to, stride = _gradient_of(logits, gradient, device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    ratios = torch.empty((2 * pairs,), dtype=torch.float32, device=device)
+    logp = torch.empty((rows,), dtype=torch.float32, device=device)
+    f32 = torch.float32
+    head = (_ELEMENT[logits.dtype], rows, vocab, pairs, logits.stride(0), stride, scale, beta,
+            smoothing, pointer, _words(targets, "targets", device, torch.int32, (rows,)),
+            _words(offsets, "offsets", device, torch.int32, (2 * pairs + 1,)),
+            _words(ref_logp, "ref_logp", device, f32, (rows,)),
+            _words(weights, "weights", device, f32, (pairs,)),
+            loss.data_ptr(), ratios.data_ptr(), logp.data_ptr(), to)
+    size = load_library().tb_preference_workspace(_preference(*head, 0, 0))
+    workspace = torch.empty((size,), dtype=torch.uint8, device=device)
+    _call("tb_preference_loss", device, _preference(*head, workspace.data_ptr(), size))
+    return PreferenceLoss(loss, ratios, logp, gradient)
