@@ -393,8 +393,8 @@ typedef struct tb_rotate_desc {
 int tb_head_rotate(const tb_rotate_desc* desc, void* stream);
 /* Gradients of q, k and the weights.  q_out may be dq (k_out dk), or q (k), with the same strides. */
 int tb_head_rotate_backward(const tb_rotate_desc* desc, void* stream);
-/* Bytes of workspace that the backward pass of this request needs (16-byte aligned; may be 0). */
-int64_t tb_head_rotate_workspace(const tb_rotate_desc* desc);
+/* Bytes of 16-byte aligned workspace for the weight gradients of heads of `dim` elements. */
+int64_t tb_head_rotate_workspace(int64_t dim);
 
 /* log softmax(scale * logits[n])[targets[n]] of every row.  A row counts as hidden where its
  * target is negative or its logits are all -inf: its log probability is 0.  A target of vocab or
@@ -447,7 +447,8 @@ typedef struct tb_preference_desc {
  * loss = sum_i weight_i (-(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)).
  * `gradient` may be `logits` with its stride. */
 int tb_preference_loss(const tb_preference_desc* desc, void* stream);
-int64_t tb_preference_workspace(const tb_preference_desc* desc);
+/* Bytes of 16-byte aligned workspace for a preference loss over `rows`. */
+int64_t tb_preference_workspace(int64_t rows);
 
 #ifdef __cplusplus
 }

@@ -278,12 +278,12 @@ def load_library() -> C.CDLL:
         "tb_gated_scan_backward": (C.c_int, [C.c_char_p, P]),
         "tb_head_rotate": (C.c_int, [C.c_char_p, P]),
         "tb_head_rotate_backward": (C.c_int, [C.c_char_p, P]),
-        "tb_head_rotate_workspace": (C.c_int64, [C.c_char_p]),
+        "tb_head_rotate_workspace": (C.c_int64, [C.c_int64]),
         "tb_token_logp": (C.c_int, [C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_double,
                                     P, P]),
         "tb_policy_loss": (C.c_int, [C.c_char_p, P]),
         "tb_preference_loss": (C.c_int, [C.c_char_p, P]),
-        "tb_preference_workspace": (C.c_int64, [C.c_char_p]),
+        "tb_preference_workspace": (C.c_int64, [C.c_int64]),
     }
     for name, (restype, argtypes) in sigs.items():
         fn = getattr(lib, name)

@@ -283,8 +283,6 @@ int policy_loss(const tb_policy_desc* desc, void* stream) {
   return call.finish(e);
 }
 
-int64_t preference_workspace(const tb_preference_desc& d) { return d.rows * 12; }
-
 int preference_loss(const tb_preference_desc* desc, void* stream) {
   OperatorCall call("tb_preference_loss", stream);
   if (!desc) return call.invalid("no request");
@@ -299,8 +297,8 @@ int preference_loss(const tb_preference_desc* desc, void* stream) {
   if (!words_ok({d.loss, d.ratios, d.offsets}) || !aligned_to(d.weights, 4) ||
       (d.rows > 0 && !words_ok({d.targets, d.ref_logp, d.logp})))
     return call.invalid("a row array is NULL or unaligned");
-  if (preference_workspace(d) > 0) {
-    if (!d.workspace || d.workspace_bytes < preference_workspace(d))
+  if (tb_preference_workspace(d.rows) > 0) {
+    if (!d.workspace || d.workspace_bytes < tb_preference_workspace(d.rows))
       return call.invalid("the workspace is too small");
     if (!aligned_to(d.workspace, 16)) return call.invalid("the workspace is not 16-byte aligned");
   }
@@ -334,6 +332,4 @@ extern "C" int tb_policy_loss(const tb_policy_desc* desc, void* stream) {
 extern "C" int tb_preference_loss(const tb_preference_desc* desc, void* stream) {
   return tb::guarded([&] { return tb::preference_loss(desc, stream); });
 }
-extern "C" int64_t tb_preference_workspace(const tb_preference_desc* desc) {
-  return desc && desc->rows > 0 ? tb::preference_workspace(*desc) : 0;
-}
+extern "C" int64_t tb_preference_workspace(int64_t rows) { return rows > 0 ? rows * 12 : 0; }

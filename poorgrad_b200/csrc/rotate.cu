@@ -81,7 +81,7 @@ __global__ void k_rotate(tb_rotate_desc d, int64_t rows) {
   }
 }
 
-constexpr int kBackwardBlocks = 296;  // rows of weight-gradient partials
+constexpr int64_t kBackwardBlocks = 296;  // rows of weight-gradient partials
 
 template <typename T>
 __global__ void k_rotate_backward(tb_rotate_desc d, int64_t rows) {
@@ -161,7 +161,7 @@ __global__ void k_rotate_weights(tb_rotate_desc d) {
 }
 
 int64_t workspace_bytes(const tb_rotate_desc& d) {
-  return d.dq_weight || d.dk_weight ? (int64_t)kBackwardBlocks * 2 * d.dim * 4 : 0;
+  return d.dq_weight || d.dk_weight ? tb_head_rotate_workspace(d.dim) : 0;
 }
 
 bool strides_ok(const tb_rotate_desc& d, const int64_t s[3], int64_t heads, bool written) {
@@ -245,6 +245,6 @@ extern "C" int tb_head_rotate(const tb_rotate_desc* desc, void* stream) {
 extern "C" int tb_head_rotate_backward(const tb_rotate_desc* desc, void* stream) {
   return tb::guarded([&] { return tb::rotate_call("tb_head_rotate_backward", desc, stream, true); });
 }
-extern "C" int64_t tb_head_rotate_workspace(const tb_rotate_desc* desc) {
-  return desc && desc->dim > 0 && desc->dim <= 512 ? tb::workspace_bytes(*desc) : 0;
+extern "C" int64_t tb_head_rotate_workspace(int64_t dim) {
+  return dim > 0 && dim <= 512 ? tb::kBackwardBlocks * 2 * dim * 4 : 0;
 }

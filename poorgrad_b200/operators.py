@@ -39,42 +39,66 @@ def _need(condition, what: str):
         raise ValueError(what)
 
 
+# The checks below build their messages only when they fail: a small call costs a few microseconds
+# of host time, and its checks are most of them.
+def _unfit(t, name: str, device, dtype, shape, more: str):
+    got = (t.dtype, tuple(t.shape), t.stride(), t.device) if isinstance(t, torch.Tensor) else type(t)
+    raise ValueError(f"{name}: expected {dtype} {tuple(shape)} on {device}, {more}; got {got}")
+
+
 def _device_of(first, name: str):
-    _need(isinstance(first, torch.Tensor) and first.is_cuda, f"{name}: a CUDA tensor is expected")
+    if not (isinstance(first, torch.Tensor) and first.is_cuda and first.dtype in _ELEMENT):
+        raise ValueError(f"{name}: a float32 or bfloat16 CUDA tensor is expected")
     return first.device
 
 
 def _array(t, name: str, device, dtype, shape):
-    """Checks a large array: its type, device and shape, and that its last axis has stride 1."""
-    _need(isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype
-          and t.shape == shape,
-          f"{name}: expected {dtype} {tuple(shape)} on {device}, got "
-          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
-    _need(not shape[-1] > 1 or t.stride(-1) == 1, f"{name}: the last axis must have stride 1")
+    """Address of a large array of this type, device and shape whose last axis has stride 1."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
+            and t.device == device and (t.stride(-1) == 1 or shape[-1] <= 1)):
+        _unfit(t, name, device, dtype, shape, "stride 1 along the last axis")
     return t.data_ptr()
 
 
 def _words(t, name: str, device, dtype, shape):
-    """Checks a contiguous 32-bit array, or None."""
+    """Address of a contiguous 32-bit array, or 0 for None."""
     if t is None:
         return 0
-    _need(isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype
-          and t.shape == shape and t.is_contiguous(),
-          f"{name}: expected contiguous {dtype} {tuple(shape)} on {device}, got "
-          f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
+            and t.device == device and t.is_contiguous()):
+        _unfit(t, name, device, dtype, shape, "contiguous")
     return t.data_ptr()
 
 
-def _call(entry: str, device, *arguments):
-    lib = load_library()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        code = getattr(lib, entry)(*arguments, stream)
-    else:  # the default stream belongs to the current device
+def _like(t):
+    """A new dense array in the order of t's axes, the last one innermost."""
+    made = torch.empty_like(t)
+    return made if made.stride(-1) == 1 or t.shape[-1] <= 1 else t.new_empty(t.shape)
+
+
+_entries: dict = {}
+# the stream's handle without a Stream object around it, where this torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _entry(name: str):
+    found = _entries.get(name)
+    if found is None:
+        found = _entries[name] = getattr(load_library(), name)
+    return found
+
+
+def _call(name: str, device, *arguments):
+    entry = _entries.get(name) or _entry(name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = entry(*arguments, _raw_stream(index))
+    else:  # the entry points launch on the current device
         with torch.cuda.device(device):
-            code = getattr(lib, entry)(*arguments, stream)
+            code = entry(*arguments, _raw_stream(index))
     if code != 0:
-        raise BackendError(code, entry)
+        raise BackendError(code, name)
 
 
 # ------------------------------------------------------------------ gated scan
@@ -90,6 +114,13 @@ def _scan_extents(x, offsets, device):
           "offsets: expected sequences + 1 row numbers")
     length, channels = x.shape
     return 1, length, channels, offsets.shape[0] - 1, offsets.shape[0] - 1
+
+
+def _states(like, x, count, channels):
+    """A new [count, channels] float32 array (a copy of `like`'s form is the quicker to make)."""
+    if like is not None and like.shape == (count, channels) and like.dtype is torch.float32:
+        return torch.empty_like(like)
+    return x.new_empty((count, channels), dtype=torch.float32)
 
 
 def _time_strides(t):
@@ -108,13 +139,12 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
     final state may be written into ``state`` itself (``final_state=state``), as a decode loop
     does.  ``out`` may be ``gate`` or ``x``."""
     device = _device_of(x, "x")
-    _need(x.dtype in _ELEMENT, "x: float32 or bfloat16 is expected")
-    _need(form in _FORM, f"form: one of {sorted(_FORM)} is expected")
+    _need(form in _FORM, "form: 'direct' or 'sigmoid' is expected")
     batch, length, channels, sequences, count = _scan_extents(x, offsets, device)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        out = _like(x)
     if final_state is None:
-        final_state = torch.empty((count, channels), dtype=torch.float32, device=device)
+        final_state = _states(state, x, count, channels)
     shape, dtype = x.shape, x.dtype
     pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
                 _array(out, "out", device, dtype, shape),
@@ -134,15 +164,14 @@ def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, of
     outputs ``h`` and ``dfinal`` of its final state (zeros when None).  ``x`` is read by the
     sigmoid form only.  One of ``dgate`` and ``dx`` may be ``dh``."""
     device = _device_of(dh, "dh")
-    _need(dh.dtype in _ELEMENT, "dh: float32 or bfloat16 is expected")
-    _need(form in _FORM, f"form: one of {sorted(_FORM)} is expected")
+    _need(form in _FORM, "form: 'direct' or 'sigmoid' is expected")
     batch, length, channels, sequences, count = _scan_extents(dh, offsets, device)
     shape, dtype = dh.shape, dh.dtype
     if dgate is None:
-        dgate = torch.empty(shape, dtype=dtype, device=device)
+        dgate = _like(dh)
     if dx is None:
-        dx = torch.empty(shape, dtype=dtype, device=device)
-    dstate = torch.empty((count, channels), dtype=torch.float32, device=device)
+        dx = _like(dh)
+    dstate = _states(state, dh, count, channels)
     if form == "direct" and x is None:
         x = gate  # not read
     pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
@@ -183,7 +212,7 @@ def _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon,
     q_shape, k_shape = q.shape, (batch, length, k_heads, dim)
     _need(isinstance(table, torch.Tensor) and table.dim() == 2,
           "table: expected [positions, turned]")
-    _need(style in _STYLE, f"style: one of {sorted(_STYLE)} is expected")
+    _need(style in _STYLE, "style: 'halves' or 'pairs' is expected")
     pointers = (_array(q, "q", device, dtype, q_shape), _array(k, "k", device, dtype, k_shape),
                 _words(table, "table", device, torch.float32, table.shape),
                 _words(positions, "positions", device, torch.int32, (batch, length)),
@@ -204,7 +233,6 @@ def _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon,
 
 def _rotate_inputs(q, k, positions):
     device = _device_of(q, "q")
-    _need(q.dtype in _ELEMENT, "q: float32 or bfloat16 is expected")
     _need(q.dim() in (3, 4) and isinstance(k, torch.Tensor) and k.dim() == q.dim(),
           "q, k: expected [tokens, heads, dim] or [batch, length, heads, dim]")
     if isinstance(positions, torch.Tensor) and positions.dim() == 1 and q.dim() == 3:
@@ -226,9 +254,9 @@ def head_rotate(q, k, table, positions=None, *, q_weight=None, k_weight=None,
     The outputs may be the inputs."""
     device, positions = _rotate_inputs(q, k, positions)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        q_out = _like(q)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
+        k_out = _like(k)
     if q.dim() == 4:
         request = _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon,
                                   style, q_out, k_out, None, None, 0, 0, 0, 0)
@@ -248,19 +276,16 @@ def head_rotate_backward(dq, dk, q, k, table, positions=None, *, q_weight=None, 
     ``weights=False``.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
     device, positions = _rotate_inputs(q, k, positions)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        q_out = _like(q)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=q.dtype, device=device)
+        k_out = _like(k)
     dq_weight = dk_weight = workspace = None
     p = [0, 0, 0, 0]
     if weights:
         dim = q.shape[-1]
-        both = torch.empty((2, dim), dtype=torch.float32, device=device)
-        dq_weight, dk_weight = both[0], both[1]
-        size = load_library().tb_head_rotate_workspace
-        draft = _rotate(0, 0, q.shape[0], 1, q.shape[-2], k.shape[-2], dim, *(0,) * 20, 0.0,
-                        *(0,) * 10, dq_weight.data_ptr(), dk_weight.data_ptr(), 0, 0)
-        workspace = torch.empty((size(draft),), dtype=torch.uint8, device=device)
+        dq_weight = q.new_empty((dim,), dtype=torch.float32)
+        dk_weight = torch.empty_like(dq_weight)
+        workspace = q.new_empty((_entry("tb_head_rotate_workspace")(dim),), dtype=torch.uint8)
         p = [dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), workspace.numel()]
     request = _rotate_request(device, _heads(q), _heads(k), table, positions, q_weight, k_weight,
                               epsilon, style, _heads(q_out), _heads(k_out), _heads(dq), _heads(dk),
@@ -286,8 +311,7 @@ class PreferenceLoss(NamedTuple):
 
 def _logits(logits):
     device = _device_of(logits, "logits")
-    _need(logits.dtype in _ELEMENT and logits.dim() == 2,
-          "logits: float32 or bfloat16 [rows, vocab] is expected")
+    _need(logits.dim() == 2, "logits: expected [rows, vocab]")
     return device, _array(logits, "logits", device, logits.dtype, logits.shape)
 
 
@@ -296,7 +320,7 @@ def _gradient_of(logits, gradient, device):
     if gradient is None or gradient is False:
         return None, 0, 0
     if gradient is True:
-        gradient = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        gradient = _like(logits)
     return gradient, _array(gradient, "gradient", device, logits.dtype,
                             logits.shape), gradient.stride(0)
 
@@ -308,7 +332,7 @@ def token_logp(logits, targets, *, scale: float = 1.0):
     device, pointer = _logits(logits)
     rows, vocab = logits.shape
     _need(targets is not None, "targets: missing")
-    logp = torch.empty((rows,), dtype=torch.float32, device=device)
+    logp = logits.new_empty((rows,), dtype=torch.float32)
     _call("tb_token_logp", device, _ELEMENT[logits.dtype], pointer, logits.stride(0),
           _words(targets, "targets", device, torch.int32, (rows,)), rows, vocab, scale,
           logp.data_ptr())
@@ -331,14 +355,14 @@ def policy_loss(logits, targets, old_logp, advantages, weights, *, ref_logp=None
           and weights is not None and (kl == 0 or ref_logp is not None),
           "targets, old_logp, advantages and weights are needed, and ref_logp where kl is not 0")
     gradient, to, stride = _gradient_of(logits, gradient, device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    token_loss = torch.empty((rows,), dtype=torch.float32, device=device)
-    logp = torch.empty((rows,), dtype=torch.float32, device=device)
     f32, shape = torch.float32, (rows,)
+    old = _words(old_logp, "old_logp", device, f32, shape)
+    loss, token_loss, logp = (old_logp.new_empty(()), torch.empty_like(old_logp),
+                              torch.empty_like(old_logp))
     request = _policy(_ELEMENT[logits.dtype], rows, vocab, logits.stride(0), stride, scale, clip_low,
                       clip_high, kl, pointer,
                       _words(targets, "targets", device, torch.int32, shape),
-                      _words(old_logp, "old_logp", device, f32, shape),
+                      old,
                       _words(ref_logp, "ref_logp", device, f32, shape),
                       _words(advantages, "advantages", device, f32, shape),
                       _words(weights, "weights", device, f32, shape),
@@ -365,17 +389,16 @@ def preference_loss(logits, targets, offsets, ref_logp, *, beta: float = 0.1,
     _need(targets is not None and ref_logp is not None, "targets and ref_logp are needed")
     pairs = offsets.shape[0] // 2
     gradient, to, stride = _gradient_of(logits, gradient, device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    ratios = torch.empty((2 * pairs,), dtype=torch.float32, device=device)
-    logp = torch.empty((rows,), dtype=torch.float32, device=device)
     f32 = torch.float32
-    head = (_ELEMENT[logits.dtype], rows, vocab, pairs, logits.stride(0), stride, scale, beta,
+    ref = _words(ref_logp, "ref_logp", device, f32, (rows,))
+    loss, ratios, logp = (ref_logp.new_empty(()), ref_logp.new_empty((2 * pairs,)),
+                          torch.empty_like(ref_logp))
+    size = _entry("tb_preference_workspace")(rows)
+    workspace = logits.new_empty((size,), dtype=torch.uint8)
+    request = (_ELEMENT[logits.dtype], rows, vocab, pairs, logits.stride(0), stride, scale, beta,
             smoothing, pointer, _words(targets, "targets", device, torch.int32, (rows,)),
-            _words(offsets, "offsets", device, torch.int32, (2 * pairs + 1,)),
-            _words(ref_logp, "ref_logp", device, f32, (rows,)),
+            _words(offsets, "offsets", device, torch.int32, (2 * pairs + 1,)), ref,
             _words(weights, "weights", device, f32, (pairs,)),
-            loss.data_ptr(), ratios.data_ptr(), logp.data_ptr(), to)
-    size = load_library().tb_preference_workspace(_preference(*head, 0, 0))
-    workspace = torch.empty((size,), dtype=torch.uint8, device=device)
-    _call("tb_preference_loss", device, _preference(*head, workspace.data_ptr(), size))
+            loss.data_ptr(), ratios.data_ptr(), logp.data_ptr(), to, workspace.data_ptr(), size)
+    _call("tb_preference_loss", device, _preference(*request))
     return PreferenceLoss(loss, ratios, logp, gradient)
