@@ -349,6 +349,8 @@ typedef struct tb_scan_desc {
   void* dgate;
   void* dx;
   float* dstate;                    /* gradient of state; NULL = not wanted */
+  void* workspace;                  /* tb_gated_scan_workspace bytes, or NULL */
+  int64_t workspace_bytes;
 } tb_scan_desc;
 /* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
  * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
@@ -358,6 +360,9 @@ int tb_gated_scan(const tb_scan_desc* desc, void* stream);
  * d b_t = g_t, chained through the form.  Reads the saved outputs h.  `dstate` may be `dfinal`;
  * `dgate` and `dx` may be `dh` with its strides (one of them). */
 int tb_gated_scan_backward(const tb_scan_desc* desc, void* stream);
+/* Bytes of 16-byte aligned workspace with which long sequences of few channels are cut along time
+ * (0: such a call needs none).  Without it the call is served all the same, more slowly. */
+int64_t tb_gated_scan_workspace(int64_t batch, int64_t length, int64_t channels);
 
 /* Which elements of a head are turned together. */
 enum {

@@ -69,7 +69,8 @@ TbScanDesc = _request(
     "TbScanDesc",
     longs="element form batch length channels sequences gate_strides:2 x_strides:2 h_strides:2 "
           "dh_strides:2 dgate_strides:2 dx_strides:2",
-    pointers="gate x h offsets state final_state dh dfinal dgate dx dstate")
+    pointers="gate x h offsets state final_state dh dfinal dgate dx dstate workspace",
+    longs_last="workspace_bytes")
 TbRotateDesc = _request(
     "TbRotateDesc",
     longs="element style batch length q_heads k_heads dim turned table_rows q_strides:3 "
@@ -276,6 +277,7 @@ def load_library() -> C.CDLL:
         # the operators' requests are passed as packed bytes
         "tb_gated_scan": (C.c_int, [C.c_char_p, P]),
         "tb_gated_scan_backward": (C.c_int, [C.c_char_p, P]),
+        "tb_gated_scan_workspace": (C.c_int64, [C.c_int64] * 3),
         "tb_head_rotate": (C.c_int, [C.c_char_p, P]),
         "tb_head_rotate_backward": (C.c_int, [C.c_char_p, P]),
         "tb_head_rotate_workspace": (C.c_int64, [C.c_int64]),

@@ -123,6 +123,15 @@ def _states(like, x, count, channels):
     return x.new_empty((count, channels), dtype=torch.float32)
 
 
+def _scan_workspace(x, batch, length, channels):
+    """(tensor, address, bytes) of the scratch that a long call is cut along time with."""
+    size = _entry("tb_gated_scan_workspace")(batch, length, channels) if length >= 512 else 0
+    if not size:
+        return None, 0, 0
+    workspace = x.new_empty((size,), dtype=torch.uint8)
+    return workspace, workspace.data_ptr(), size
+
+
 def _time_strides(t):
     return (0, t.stride(0)) if t.dim() == 2 else (t.stride(0), t.stride(1))
 
@@ -151,9 +160,10 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
                 _words(offsets, "offsets", device, torch.int32, (sequences + 1,)),
                 _words(state, "state", device, torch.float32, (count, channels)),
                 _words(final_state, "final_state", device, torch.float32, (count, channels)))
+    workspace, scratch, size = _scan_workspace(x, batch, length, channels)
     request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
                     *_time_strides(gate), *_time_strides(x), *_time_strides(out),
-                    0, 0, 0, 0, 0, 0, *pointers, 0, 0, 0, 0, 0)
+                    0, 0, 0, 0, 0, 0, *pointers, 0, 0, 0, 0, 0, scratch, size)
     _call("tb_gated_scan", device, request)
     return out, final_state
 
@@ -182,9 +192,11 @@ def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, of
                 _words(dfinal, "dfinal", device, torch.float32, (count, channels)),
                 _array(dgate, "dgate", device, dtype, shape),
                 _array(dx, "dx", device, dtype, shape), dstate.data_ptr())
+    workspace, scratch, size = _scan_workspace(dh, batch, length, channels)
     request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
                     *_time_strides(gate), *_time_strides(x), *_time_strides(h),
-                    *_time_strides(dh), *_time_strides(dgate), *_time_strides(dx), *pointers)
+                    *_time_strides(dh), *_time_strides(dgate), *_time_strides(dx), *pointers,
+                    scratch, size)
     _call("tb_gated_scan_backward", device, request)
     return dgate, dx, dstate
 
