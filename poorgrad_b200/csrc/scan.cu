@@ -11,22 +11,123 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-struct Gate {
-  float a, b;  // sigmoid and 1 - sigmoid
+// One lane's V channels of a row as f32, V = 1 or 2.  Pairs use the packed f32x2 instructions: the
+// scan issues some 15 to 25 instructions an element, and that, not memory, bounds it otherwise.
+template <int V>
+struct Vec;
+template <>
+struct Vec<1> {
+  float x;
+  __device__ __forceinline__ float get(int) const { return x; }
+  __device__ __forceinline__ void set(int, float v) { x = v; }
 };
-// Both from one exponential of -|g|, so neither loses bits where it is small.
-__device__ __forceinline__ Gate sigmoid_pair(float g) {
-  const float e = __expf(-fabsf(g));
-  const float r = __fdividef(1.0f, 1.0f + e);
-  const float s = e * r;
-  return g >= 0 ? Gate{r, s} : Gate{s, r};
+template <>
+struct Vec<2> {
+  float2 x;
+  __device__ __forceinline__ float get(int i) const { return i ? x.y : x.x; }
+  __device__ __forceinline__ void set(int i, float v) { (i ? x.y : x.x) = v; }
+};
+template <int V>
+__device__ __forceinline__ Vec<V> splat(float v) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, v);
+  return r;
+}
+__device__ __forceinline__ unsigned long long packed(Vec<2> v) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x.x), "f"(v.x.y));
+  return r;
+}
+__device__ __forceinline__ Vec<2> unpacked(unsigned long long r) {
+  Vec<2> v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x.x), "=f"(v.x.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.x * b.x}; }
+__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.x + b.x}; }
+__device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.x, b.x, c.x)}; }
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
+  return unpacked(r);
+}
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
+  return unpacked(r);
+}
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)), "l"(packed(c)));
+  return unpacked(r);
+}
+template <int V>
+__device__ __forceinline__ Vec<V> select(bool p, Vec<V> a, Vec<V> b) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, p ? a.get(i) : b.get(i));
+  return r;
 }
 
-// V consecutive channels of one row, as loaded.
+// V channels of one row as stored.
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Lane {
-  T v[V];
+struct Raw;
+template <>
+struct Raw<float, 1> {
+  typedef float type;
+  static __device__ __forceinline__ Vec<1> read(float r) { return {r}; }
+  static __device__ __forceinline__ float made(Vec<1> v) { return v.x; }
 };
+template <>
+struct Raw<float, 2> {
+  typedef float2 type;
+  static __device__ __forceinline__ Vec<2> read(float2 r) { return {r}; }
+  static __device__ __forceinline__ float2 made(Vec<2> v) { return v.x; }
+};
+template <>
+struct Raw<bf16, 1> {
+  typedef unsigned short type;
+  static __device__ __forceinline__ Vec<1> read(unsigned short r) {
+    return {__uint_as_float((unsigned)r << 16)};
+  }
+  static __device__ __forceinline__ unsigned short made(Vec<1> v) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(v.x));
+  }
+};
+template <>
+struct Raw<bf16, 2> {
+  typedef unsigned type;
+  static __device__ __forceinline__ Vec<2> read(unsigned r) {
+    return {{__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)}};
+  }
+  static __device__ __forceinline__ unsigned made(Vec<2> v) {
+    unsigned r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.x.y), "f"(v.x.x));
+    return r;
+  }
+};
+
+template <int V>
+struct Gate {
+  Vec<V> a, b;  // sigmoid and 1 - sigmoid
+};
+// With e = exp(-g): 1 / (1 + e) and e / (1 + e), so that neither loses bits where it is small.  g is
+// held above -87, where e still has a reciprocal (and sigmoid(g) < 2^-125); a NaN stays one.
+template <int V>
+__device__ __forceinline__ Gate<V> sigmoid_pair(Vec<V> g) {
+  Vec<V> e, r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float h;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(h) : "f"(g.get(i)), "f"(-87.0f));
+    e.set(i, __expf(-h));
+  }
+  const Vec<V> sum = e + splat<V>(1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, __fdividef(1.0f, sum.get(i)));
+  return {r, e * r};
+}
 
 __device__ __forceinline__ int64_t clamped_offset(const tb_scan_desc& d, int64_t s) {
   // offsets are data: whatever they hold, rows stay within the array
@@ -39,46 +140,72 @@ struct Marks {
   unsigned enters, leaves, inside;
   int sequence;
 };
+// How many of the first `sequences` offsets are at or below t (32 are looked at a time).
+__device__ __forceinline__ int64_t begun_by(const tb_scan_desc& d, int64_t t) {
+  const int lane = threadIdx.x % 32;
+  int64_t lo = 0, n = d.sequences;  // the answer lies in [lo, lo + n]
+  while (n > 0) {
+    const int64_t stride = (n + 31) / 32, i = lo + (lane + 1) * stride - 1;
+    const bool below = i < lo + n && d.offsets[i] <= t;
+    const int64_t k = __popc(__ballot_sync(~0u, below));
+    lo += k * stride;
+    n = min(n - k * stride, stride - 1);
+  }
+  return lo;
+}
 template <int L, bool BACK>
 __device__ __forceinline__ Marks marks_of(const tb_scan_desc& d, int64_t b, int64_t first) {
   const int lane = threadIdx.x % 32;
-  const int64_t step = first + lane, t = BACK ? d.length - 1 - step : step;
-  const bool here = lane < L && step < d.length;
-  bool starts, ends, inside = here;
-  int sequence = (int)b;
-  if (d.sequences == 0) {
-    starts = t == 0;
-    ends = t == d.length - 1;
-  } else {
-    // the last sequence that starts at or before t
-    int64_t lo = 0, hi = d.sequences;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (here && d.offsets[mid] <= t) lo = mid; else hi = mid;
-    }
-    const int64_t from = d.offsets[lo], to = d.offsets[lo + 1];
-    sequence = (int)lo;
-    inside = here && from <= t && t < to;
-    starts = t == from || t == 0;
-    ends = t == to - 1 || t == d.length - 1;
-  }
+  constexpr unsigned kAll = L == 32 ? ~0u : (1u << L) - 1;
+  const int64_t left = d.length - first;
+  const unsigned here = left >= L ? kAll : left <= 0 ? 0u : (1u << (int)left) - 1;
   Marks m;
-  m.sequence = sequence;
+  if (d.sequences == 0) {
+    m.sequence = (int)b;
+    m.inside = here;
+    m.enters = first == 0 ? here & 1 : 0u;
+    m.leaves = left > 0 && left <= L ? 1u << (int)(left - 1) : 0u;
+    return m;
+  }
+  const int64_t low = BACK ? d.length - first - L : first, high = low + L - 1;  // rows
+  const int64_t begun = begun_by(d, low), s = max(begun - 1, (int64_t)0);
+  const int64_t from = d.offsets[s], to = d.offsets[s + 1];
+  if (here == kAll && begun > 0 && from < low && high < to - 1 && low > 0 && high < d.length - 1) {
+    m.sequence = (int)s;  // the run lies within one sequence
+    m.inside = kAll;
+    m.enters = m.leaves = 0;
+    return m;
+  }
+  const int64_t step = first + lane, t = BACK ? d.length - 1 - step : step;
+  const bool mine = here >> lane & 1;
+  // the last sequence that starts at or before t
+  int64_t lo = s, hi = d.sequences;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) / 2;
+    if (mine && d.offsets[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int64_t mine_from = d.offsets[lo], mine_to = d.offsets[lo + 1];
+  const bool inside = mine && mine_from <= t && t < mine_to;
+  const bool starts = t == mine_from || t == 0, ends = t == mine_to - 1 || t == d.length - 1;
+  m.sequence = (int)lo;
   m.inside = __ballot_sync(~0u, inside);
   m.enters = __ballot_sync(~0u, inside && (BACK ? ends : starts));
   m.leaves = __ballot_sync(~0u, inside && (BACK ? starts : ends));
   return m;
 }
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kMaxRanks = 8;
 
 // What a run of steps does to the value v carried into it: v -> A v + H, or H alone where a
 // sequence begins inside the run (then v belongs to another sequence and may be anything).
+template <int V>
 struct Affine {
-  float A, H;
+  Vec<V> A, H;
 };
-__device__ __forceinline__ float apply(Affine f, bool begins, float v) {
-  return begins ? f.H : fmaf(f.A, v, f.H);
+template <int V>
+__device__ __forceinline__ Vec<V> apply(Affine<V> f, bool begins, Vec<V> v) {
+  return select(begins, f.H, fma(f.A, v, f.H));
 }
 
 // How a call is cut: `ranks` blocks of a cluster take consecutive spans of kWarps * L steps, over
@@ -88,7 +215,7 @@ __device__ __forceinline__ float apply(Affine f, bool begins, float v) {
 struct Cut {
   int ranks, tiles, parts;
   int64_t part_steps;
-  Affine* maps;  // [batch][parts][channels], parts > 1
+  float2* maps;  // (A, H), [batch][parts][channels], parts > 1
   int* begins;   // [batch][parts]
 };
 
@@ -104,22 +231,21 @@ enum { kWhole = 0, kMaps = 1, kFromMaps = 2 };
 // and walks them again to write the outputs.
 template <typename T, int V, int L, int FORM, bool BACK, int PASS>
 struct Scan {
-  typedef Lane<T, V> Row;
-  static constexpr bool kReadsX = FORM == TB_SCAN_SIGMOID || !BACK;
+  typedef Raw<T, V> R;
+  typedef typename R::type Row;
+  static constexpr bool kReadsX = FORM == TB_SCAN_SIGMOID;
   const tb_scan_desc& d;
-  const int lane, warp;
   const int64_t b, c;
   const bool in;  // this lane's channels exist
   const float* entry_state;
   float* exit_state;
   Row g[L], u[L], before[L], xs[L];  // u: x, or dh backwards
-  float a[L][V], add[L][V];
+  Vec<V> a[L], add[L];
 
   __device__ Scan(const tb_scan_desc& d, int64_t b, int64_t c)
-      : d(d), lane(threadIdx.x % 32), warp(threadIdx.x / 32), b(b), c(c), in(c < d.channels),
-        entry_state(BACK ? d.dfinal : d.state), exit_state(BACK ? d.dstate : d.final_state) {}
+      : d(d), b(b), c(c), in(c < d.channels), entry_state(BACK ? d.dfinal : d.state),
+        exit_state(BACK ? d.dstate : d.final_state) {}
 
-  // A row pointer walks with the steps.
   template <typename P>
   __device__ __forceinline__ P* at(P* base, const int64_t s[2], int64_t t) const {
     return base + b * s[0] + t * s[1] + c;
@@ -138,58 +264,65 @@ struct Scan {
     const int64_t left = d.length - first;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const bool here = ALL || (in && i < left);
       if (!ALL) g[i] = u[i] = before[i] = xs[i] = Row{};
-      if (here) {
-        g[i] = *(const Row*)(pg + i * sg);
-        u[i] = *(const Row*)(pu + i * su);
+      if (ALL || (in && i < left)) {
+        g[i] = *(const Row*)pg;
+        u[i] = *(const Row*)pu;
         if (BACK && PASS != kMaps) {
           // the row before the first is the state's
-          if (ALL ? i < L - 1 || t0 >= L : t0 - i > 0) before[i] = *(const Row*)(ph + i * sh);
-          else before[i] = Row{};
-          if (kReadsX) xs[i] = *(const Row*)(px + i * sx);
+          if (ALL && i < L - 1) before[i] = *(const Row*)ph;
+          else before[i] = t0 - i > 0 ? *(const Row*)ph : Row{};
+          if (kReadsX) xs[i] = *(const Row*)px;
         }
       }
+      pg += sg;
+      pu += su;
+      ph += sh;
+      px += sx;
     }
   }
 
-  // a and the added term of each step (kept where the outputs do not work them out again), and
-  // the steps' map.  A step that enters a sequence holds the entry state's part in its term, so
-  // that state is read before any other state is written.  What rows outside every sequence hold
-  // goes nowhere: the next row inside one enters it.
-  template <bool MARKED>
-  __device__ __forceinline__ void reduce(const Marks& m, Affine map[V]) {
+  __device__ __forceinline__ Vec<V> state_at(const float* states, int64_t at) const {
+    Vec<V> r = splat<V>(0.0f);
+    if (states && in)
 #pragma unroll
-    for (int v = 0; v < V; ++v) map[v] = {1.0f, 0.0f};
+      for (int v = 0; v < V; ++v) r.set(v, states[at + v]);
+    return r;
+  }
+
+  // The added term of each step (and a, where the outputs do not work it out again), and the
+  // steps' map.  A step that enters a sequence holds the entry state's part in its term, so that
+  // state is read before any other state is written.  What rows outside every sequence hold goes
+  // nowhere: the next row inside one enters it.
+  template <bool MARKED>
+  __device__ __forceinline__ Affine<V> reduce(const Marks& m) {
+    Affine<V> map{splat<V>(1.0f), splat<V>(0.0f)};
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const bool enters = MARKED && (m.enters >> i & 1);
-      const int64_t state = enters ? (int64_t)__shfl_sync(~0u, m.sequence, i) * d.channels + c : 0;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float av = to_f32(g[i].v[v]), bv = to_f32(u[i].v[v]);
-        if (FORM == TB_SCAN_SIGMOID) {
-          const Gate p = sigmoid_pair(av);
-          av = p.a;
-          if (!BACK) bv *= p.b;
-        }
-        if (enters) {
-          const float e = entry_state && in ? entry_state[state + v] : 0.0f;
-          bv = BACK ? bv + e : fmaf(av, e, bv);
-          map[v].H = BACK ? av * bv : bv;
-        } else {
-          map[v].H = BACK ? av * (map[v].H + bv) : fmaf(av, map[v].H, bv);
-        }
-        map[v].A *= av;
-        if (!BACK) a[i][v] = av;
-        add[i][v] = bv;
+      Vec<V> av = R::read(g[i]), bv = R::read(u[i]);
+      if (FORM == TB_SCAN_SIGMOID) {
+        const Gate<V> p = sigmoid_pair(av);
+        av = p.a;
+        if (!BACK) bv = bv * p.b;
       }
+      if (MARKED && (m.enters >> i & 1)) {
+        const Vec<V> e =
+            state_at(entry_state, (int64_t)__shfl_sync(~0u, m.sequence, i) * d.channels + c);
+        bv = BACK ? bv + e : fma(av, e, bv);
+        map.H = BACK ? av * bv : bv;
+      } else {
+        map.H = BACK ? av * (map.H + bv) : fma(av, map.H, bv);
+      }
+      map.A = map.A * av;
+      if (!BACK) a[i] = av;
+      add[i] = bv;
     }
+    return map;
   }
 
   // ALL as in load(); MARKED: some step enters or leaves a sequence or lies outside all of them.
   template <bool ALL, bool MARKED>
-  __device__ __forceinline__ void write(const Marks& m, int64_t first, float value[V]) {
+  __device__ __forceinline__ void write(const Marks& m, int64_t first, Vec<V> value) {
     const int64_t t0 = BACK ? d.length - 1 - first : first, way = BACK ? -1 : 1;
     T* p1 = BACK ? at((T*)d.dgate, d.dgate_strides, t0) : at((T*)d.h, d.h_strides, t0);
     T* p2 = at((T*)d.dx, d.dx_strides, t0);
@@ -198,52 +331,50 @@ struct Scan {
     for (int i = 0; i < L; ++i) {
       const bool enters = MARKED && (m.enters >> i & 1), leaves = MARKED && (m.leaves >> i & 1);
       const int64_t state = leaves ? (int64_t)__shfl_sync(~0u, m.sequence, i) * d.channels + c : 0;
-      Row out, out2;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (BACK) {
-          const float gt = enters ? add[i][v] : add[i][v] + value[v];
-          float prior = to_f32(before[i].v[v]);
-          if (leaves) prior = d.state && in ? d.state[state + v] : 0.0f;
-          float av = to_f32(g[i].v[v]);
-          if (FORM == TB_SCAN_SIGMOID) {
-            const Gate p = sigmoid_pair(av);
-            av = p.a;
-            const float gb = gt * p.b;
-            out.v[v] = from_f32<T>(gb * p.a * (prior - to_f32(xs[i].v[v])));
-            out2.v[v] = from_f32<T>(gb);
-          } else {
-            out.v[v] = from_f32<T>(gt * prior);
-            out2.v[v] = from_f32<T>(gt);
-          }
-          value[v] = av * gt;
+      Vec<V> out, out2;
+      if (BACK) {
+        const Vec<V> gt = MARKED ? select(enters, add[i], add[i] + value) : add[i] + value;
+        Vec<V> prior = R::read(before[i]), av = R::read(g[i]);
+        if (leaves) prior = state_at(d.state, state);
+        if (FORM == TB_SCAN_SIGMOID) {
+          const Gate<V> p = sigmoid_pair(av);
+          av = p.a;
+          out2 = gt * p.b;
+          out = out2 * p.a * fma(R::read(xs[i]), splat<V>(-1.0f), prior);
         } else {
-          value[v] = enters ? add[i][v] : fmaf(a[i][v], value[v], add[i][v]);
-          out.v[v] = from_f32<T>(value[v]);
+          out2 = gt;
+          out = gt * prior;
         }
+        value = av * gt;
+      } else {
+        value = MARKED ? select(enters, add[i], fma(a[i], value, add[i])) : fma(a[i], value, add[i]);
+        out = value;
       }
       if ((ALL || in) && (!MARKED || (m.inside >> i & 1))) {
-        *(Row*)(p1 + i * s1) = out;
-        if (BACK) *(Row*)(p2 + i * s2) = out2;
+        *(Row*)p1 = R::made(out);
+        if (BACK) *(Row*)p2 = R::made(out2);
       }
       if (leaves && in && exit_state)
 #pragma unroll
-        for (int v = 0; v < V; ++v) exit_state[state + v] = value[v];
+        for (int v = 0; v < V; ++v) exit_state[state + v] = value.get(v);
+      p1 += s1;
+      p2 += s2;
     }
   }
 };
 
 template <typename T, int V, int L, int FORM, bool BACK, int PASS>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_scan(tb_scan_desc d, Cut cut) {
+__global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut) {
   pdl_entry();
-  __shared__ Affine maps[2][kWarps][V][32];
+  __shared__ Affine<V> maps[2][kWarps][32];
   __shared__ int begins[2][kWarps];
-  __shared__ Affine rank_maps[2][8][V][32];
-  __shared__ int rank_begins[2][8];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, ranks = cut.ranks;
+  __shared__ Affine<V> rank_maps[2][kMaxRanks][32];
+  __shared__ int rank_begins[2][kMaxRanks];
+  const int lane = threadIdx.x % 32, warp = __shfl_sync(~0u, threadIdx.x / 32, 0);
+  const int ranks = cut.ranks;
   const int rank = blockIdx.x % ranks, tile = blockIdx.x / ranks % cut.tiles;
-  const int64_t part = (int64_t)blockIdx.x / ranks / cut.tiles % cut.parts;
-  const int64_t b = (int64_t)blockIdx.x / ranks / cut.tiles / cut.parts;
+  const int part = blockIdx.x / ranks / cut.tiles % cut.parts;
+  const int64_t b = blockIdx.x / ranks / cut.tiles / cut.parts;
   Scan<T, V, L, FORM, BACK, PASS> s(d, b, (int64_t)(tile * 32 + lane) * V);
 
   // sequences without a step hand their entry state on
@@ -252,106 +383,88 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_scan(tb_scan_desc d, Cut cut
     for (int64_t i = warp; i < count; i += kWarps) {
       if (d.sequences && clamped_offset(d, i + 1) > clamped_offset(d, i)) continue;
       const int64_t at = (d.sequences ? i : b) * d.channels + s.c;
+      const Vec<V> e = s.state_at(s.entry_state, at);
       if (s.in)
-        for (int v = 0; v < V; ++v) s.exit_state[at + v] = s.entry_state ? s.entry_state[at + v] : 0.0f;
+        for (int v = 0; v < V; ++v) s.exit_state[at + v] = e.get(v);
     }
   }
 
-  float carry[V] = {};
+  Vec<V> carry = splat<V>(0.0f);
   if (PASS == kFromMaps && s.in)
-    for (int64_t p = 0; p < part; ++p) {
-      const Affine* f = cut.maps + (b * cut.parts + p) * d.channels + s.c;
-      const bool begun = cut.begins[b * cut.parts + p];
+    for (int p = 0; p < part; ++p) {
+      const float2* from = cut.maps + (b * cut.parts + p) * d.channels + s.c;
+      Affine<V> f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) carry[v] = apply(f[v], begun, carry[v]);
+      for (int v = 0; v < V; ++v) {
+        f.A.set(v, from[v].x);
+        f.H.set(v, from[v].y);
+      }
+      carry = apply(f, cut.begins[b * cut.parts + p], carry);
     }
-  Affine whole[V];  // the part's map so far
-#pragma unroll
-  for (int v = 0; v < V; ++v) whole[v] = {1.0f, 0.0f};
+  Affine<V> whole{splat<V>(1.0f), splat<V>(0.0f)};  // the part's map so far
   bool whole_begins = false;
 
   int parity = 0;
   const int64_t from = part * cut.part_steps, to = min(from + cut.part_steps, d.length);
   for (int64_t base = from; base < to; base += (int64_t)ranks * kWarps * L, parity ^= 1) {
-    const int64_t first = base + (int64_t)(rank * kWarps + warp) * L;
+    const int64_t first = base + (rank * kWarps + warp) * L;
     // a part is a whole number of spans, so that no step belongs to two
-    const bool all = s.in && first + L <= d.length;
-    const bool uniform = __all_sync(~0u, all);
-    if (uniform) s.template load<true>(first); else s.template load<false>(first);
+    const bool all = __all_sync(~0u, s.in) && first + L <= d.length;
+    if (all) s.template load<true>(first); else s.template load<false>(first);
     const Marks m = marks_of<L, BACK>(d, b, first);
     const bool marked = m.enters | m.leaves | (m.inside != (1u << L) - 1);
-    Affine map[V];
-    if (m.enters) s.template reduce<true>(m, map); else s.template reduce<false>(m, map);
-#pragma unroll
-    for (int v = 0; v < V; ++v) maps[parity][warp][v][lane] = map[v];
+    const Affine<V> map = m.enters ? s.template reduce<true>(m) : s.template reduce<false>(m);
+    maps[parity][warp][lane] = map;
     if (lane == 0) begins[parity][warp] = m.enters != 0;
     __syncthreads();
     if (ranks > 1 || PASS == kMaps) {
       // this block's map
-      Affine block[V];
+      Affine<V> block{splat<V>(1.0f), splat<V>(0.0f)};
       bool any = false;
-#pragma unroll
-      for (int v = 0; v < V; ++v) block[v] = {1.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const bool begun = begins[parity][w];
+        const Affine<V> f = maps[parity][w][lane];
         any |= begun;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Affine f = maps[parity][w][v][lane];
-          block[v] = {block[v].A * f.A, apply(f, begun, block[v].H)};
-        }
+        block = {block.A * f.A, apply(f, begun, block.H)};
       }
       if (PASS == kMaps) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          whole[v] = {whole[v].A * block[v].A, apply(block[v], any, whole[v].H)};
+        whole = {whole.A * block.A, apply(block, any, whole.H)};
         whole_begins |= any;
         continue;
       }
       cg::cluster_group cluster = cg::this_cluster();
-      if (warp < ranks) {  // to every block of the cluster
-        Affine* there = cluster.map_shared_rank(&rank_maps[parity][rank][0][0], warp);
-#pragma unroll
-        for (int v = 0; v < V; ++v) there[v * 32 + lane] = block[v];
-        if (lane == 0) *cluster.map_shared_rank(&rank_begins[parity][rank], warp) = any;
+      for (int r = warp; r < ranks; r += kWarps) {  // to every block of the cluster
+        cluster.map_shared_rank(&rank_maps[parity][rank][0], r)[lane] = block;
+        if (lane == 0) *cluster.map_shared_rank(&rank_begins[parity][rank], r) = any;
       }
       cluster.sync();
     }
     // the value carried into this warp's steps, and past all blocks' steps
-    float value[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) value[v] = carry[v];
-    if (ranks > 1)
+    Vec<V> value = carry;
+    if (ranks > 1) {
       for (int r = 0; r < ranks; ++r) {
-        const bool begun = rank_begins[parity][r];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (r == rank) value[v] = carry[v];
-          carry[v] = apply(rank_maps[parity][r][v][lane], begun, carry[v]);
-        }
+        if (r == rank) value = carry;
+        carry = apply(rank_maps[parity][r][lane], rank_begins[parity][r], carry);
       }
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const bool begun = begins[parity][w];
+      for (int w = 0; w < kWarps - 1; ++w)
+        if (w < warp) value = apply(maps[parity][w][lane], begins[parity][w], value);
+    } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (ranks == 1) {
-          if (w == warp) value[v] = carry[v];
-          carry[v] = apply(maps[parity][w][v][lane], begun, carry[v]);
-        } else if (w < warp) {
-          value[v] = apply(maps[parity][w][v][lane], begun, value[v]);
-        }
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) value = carry;
+        carry = apply(maps[parity][w][lane], begins[parity][w], carry);
       }
     }
-    if (uniform && !marked) s.template write<true, false>(m, first, value);
+    if (all && !marked) s.template write<true, false>(m, first, value);
     else s.template write<false, true>(m, first, value);
   }
   if (PASS == kMaps && warp == 0) {
     if (s.in)
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        cut.maps[(b * cut.parts + part) * d.channels + s.c + v] = whole[v];
+        cut.maps[(b * cut.parts + part) * d.channels + s.c + v] = {whole.A.get(v), whole.H.get(v)};
     if (lane == 0 && tile == 0) cut.begins[b * cut.parts + part] = whole_begins;
   }
 }
@@ -453,22 +566,21 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
   if (cut.parts > 1) {
     cut.part_steps = (spans + cut.parts - 1) / cut.parts * span;
     cut.parts = (int)((d.length + cut.part_steps - 1) / cut.part_steps);
-    cut.maps = (Affine*)d.workspace;
+    cut.maps = (float2*)d.workspace;
     cut.begins = (int*)(cut.maps + d.batch * cut.parts * d.channels);
     const cudaError_t e = launch<T, V, L, FORM, BACK, kMaps>(d, cut, stream);
     return e != cudaSuccess ? e : launch<T, V, L, FORM, BACK, kFromMaps>(d, cut, stream);
   }
-  while (cut.ranks < 8 && columns * cut.ranks < 2 * 148 && cut.ranks < spans) cut.ranks *= 2;
+  while (cut.ranks < kMaxRanks && columns * cut.ranks < 2 * 148 && cut.ranks < spans) cut.ranks *= 2;
   return launch<T, V, L, FORM, BACK, kWhole>(d, cut, stream);
 }
 
 template <typename T, int FORM, bool BACK>
 cudaError_t enqueue_form(const tb_scan_desc& d, cudaStream_t stream) {
-  constexpr int64_t kPair = 4 / sizeof(T);  // channels in 4 bytes
-  if (kPair == 1 || lanes_fit(d, BACK, sizeof(T), 4))
-    // the backward pass of the sigmoid form holds four arrays: 16 pairs of each would spill
-    return enqueue<T, kPair, BACK && FORM == TB_SCAN_SIGMOID && kPair == 2 ? 8 : 16, FORM, BACK>(d, stream);
-  return enqueue<T, 1, 16, FORM, BACK>(d, stream);
+  // the backward pass holds up to four arrays: 16 steps of each would spill
+  constexpr int kSteps = BACK && (sizeof(T) == 4 || FORM == TB_SCAN_SIGMOID) ? 8 : 16;
+  return lanes_fit(d, BACK, sizeof(T), 2 * sizeof(T)) ? enqueue<T, 2, kSteps, FORM, BACK>(d, stream)
+                                                      : enqueue<T, 1, 16, FORM, BACK>(d, stream);
 }
 
 template <typename T>
@@ -499,7 +611,7 @@ int64_t scan_workspace(int64_t batch, int64_t length, int64_t channels) {
   if (!extents_fit({batch, length, channels}) || batch * length * channels == 0) return 0;
   // the widest blocks make the fewest columns, the shortest spans the most parts
   const int64_t parts = parts_of(batch * ((channels + 63) / 64), (length + kWarps * 8 - 1) / (kWarps * 8));
-  return parts > 1 ? (batch * parts * (channels * (int64_t)sizeof(Affine) + 4) + 15) / 16 * 16 : 0;
+  return parts > 1 ? (batch * parts * (channels * (int64_t)sizeof(float2) + 4) + 15) / 16 * 16 : 0;
 }
 }  // namespace tb
 
