@@ -108,6 +108,19 @@ struct Raw<bf16, 2> {
   }
 };
 
+// The bare instructions: the intrinsics around them also serve denormals, which do not matter here
+// and cost half of the instructions of a sigmoid.
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <int V>
 struct Gate {
   Vec<V> a, b;  // sigmoid and 1 - sigmoid
@@ -121,11 +134,14 @@ __device__ __forceinline__ Gate<V> sigmoid_pair(Vec<V> g) {
   for (int i = 0; i < V; ++i) {
     float h;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(h) : "f"(g.get(i)), "f"(-87.0f));
-    e.set(i, __expf(-h));
+    e.set(i, h);
   }
+  e = e * splat<V>(-1.4426950408889634f);  // exp(-g) = 2^(-g log2(e))
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.set(i, ex2_approx(e.get(i)));
   const Vec<V> sum = e + splat<V>(1.0f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.set(i, __fdividef(1.0f, sum.get(i)));
+  for (int i = 0; i < V; ++i) r.set(i, rcp_approx(sum.get(i)));
   return {r, e * r};
 }
 
@@ -239,7 +255,9 @@ struct Scan {
   const bool in;  // this lane's channels exist
   const float* entry_state;
   float* exit_state;
-  Row g[L], u[L], before[L], xs[L];  // u: x, or dh backwards
+  struct Rows {
+    Row g[L], u[L], before[L], xs[L];  // u: x, or dh backwards
+  };
   Vec<V> a[L], add[L];
 
   __device__ Scan(const tb_scan_desc& d, int64_t b, int64_t c)
@@ -253,7 +271,7 @@ struct Scan {
 
   // ALL: every step lies within the array and its channels exist.
   template <bool ALL>
-  __device__ __forceinline__ void load(int64_t first) {
+  __device__ __forceinline__ void load(Rows& r, int64_t first) const {
     const int64_t t0 = BACK ? d.length - 1 - first : first, way = BACK ? -1 : 1;
     const T* pg = at((const T*)d.gate, d.gate_strides, t0);
     const T* pu = BACK ? at((const T*)d.dh, d.dh_strides, t0) : at((const T*)d.x, d.x_strides, t0);
@@ -264,15 +282,15 @@ struct Scan {
     const int64_t left = d.length - first;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      if (!ALL) g[i] = u[i] = before[i] = xs[i] = Row{};
+      if (!ALL) r.g[i] = r.u[i] = r.before[i] = r.xs[i] = Row{};
       if (ALL || (in && i < left)) {
-        g[i] = *(const Row*)pg;
-        u[i] = *(const Row*)pu;
+        r.g[i] = *(const Row*)pg;
+        r.u[i] = *(const Row*)pu;
         if (BACK && PASS != kMaps) {
           // the row before the first is the state's
-          if (ALL && i < L - 1) before[i] = *(const Row*)ph;
-          else before[i] = t0 - i > 0 ? *(const Row*)ph : Row{};
-          if (kReadsX) xs[i] = *(const Row*)px;
+          if (ALL && i < L - 1) r.before[i] = *(const Row*)ph;
+          else r.before[i] = t0 - i > 0 ? *(const Row*)ph : Row{};
+          if (kReadsX) r.xs[i] = *(const Row*)px;
         }
       }
       pg += sg;
@@ -295,11 +313,11 @@ struct Scan {
   // state is read before any other state is written.  What rows outside every sequence hold goes
   // nowhere: the next row inside one enters it.
   template <bool MARKED>
-  __device__ __forceinline__ Affine<V> reduce(const Marks& m) {
+  __device__ __forceinline__ Affine<V> reduce(const Rows& r, const Marks& m) {
     Affine<V> map{splat<V>(1.0f), splat<V>(0.0f)};
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      Vec<V> av = R::read(g[i]), bv = R::read(u[i]);
+      Vec<V> av = R::read(r.g[i]), bv = R::read(r.u[i]);
       if (FORM == TB_SCAN_SIGMOID) {
         const Gate<V> p = sigmoid_pair(av);
         av = p.a;
@@ -322,7 +340,7 @@ struct Scan {
 
   // ALL as in load(); MARKED: some step enters or leaves a sequence or lies outside all of them.
   template <bool ALL, bool MARKED>
-  __device__ __forceinline__ void write(const Marks& m, int64_t first, Vec<V> value) {
+  __device__ __forceinline__ void write(const Rows& r, const Marks& m, int64_t first, Vec<V> value) {
     const int64_t t0 = BACK ? d.length - 1 - first : first, way = BACK ? -1 : 1;
     T* p1 = BACK ? at((T*)d.dgate, d.dgate_strides, t0) : at((T*)d.h, d.h_strides, t0);
     T* p2 = at((T*)d.dx, d.dx_strides, t0);
@@ -334,13 +352,13 @@ struct Scan {
       Vec<V> out, out2;
       if (BACK) {
         const Vec<V> gt = MARKED ? select(enters, add[i], add[i] + value) : add[i] + value;
-        Vec<V> prior = R::read(before[i]), av = R::read(g[i]);
+        Vec<V> prior = R::read(r.before[i]), av = R::read(r.g[i]);
         if (leaves) prior = state_at(d.state, state);
         if (FORM == TB_SCAN_SIGMOID) {
           const Gate<V> p = sigmoid_pair(av);
           av = p.a;
           out2 = gt * p.b;
-          out = out2 * p.a * fma(R::read(xs[i]), splat<V>(-1.0f), prior);
+          out = out2 * p.a * fma(R::read(r.xs[i]), splat<V>(-1.0f), prior);
         } else {
           out2 = gt;
           out = gt * prior;
@@ -406,14 +424,25 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
 
   int parity = 0;
   const int64_t from = part * cut.part_steps, to = min(from + cut.part_steps, d.length);
-  for (int64_t base = from; base < to; base += (int64_t)ranks * kWarps * L, parity ^= 1) {
-    const int64_t first = base + (rank * kWarps + warp) * L;
-    // a part is a whole number of spans, so that no step belongs to two
-    const bool all = __all_sync(~0u, s.in) && first + L <= d.length;
-    if (all) s.template load<true>(first); else s.template load<false>(first);
-    const Marks m = marks_of<L, BACK>(d, b, first);
+  const int64_t span = (int64_t)ranks * kWarps * L;
+  // a part is a whole number of spans, so that no step belongs to two
+  const bool whole_warp = __all_sync(~0u, s.in);
+  typename Scan<T, V, L, FORM, BACK, PASS>::Rows rows, next;
+  int64_t first = from + (rank * kWarps + warp) * L;
+  bool all = whole_warp && first + L <= d.length;
+  if (all) s.template load<true>(rows, first); else s.template load<false>(rows, first);
+  Marks m = marks_of<L, BACK>(d, b, first), next_m = m;
+  for (int64_t base = from; base < to; base += span, parity ^= 1) {
     const bool marked = m.enters | m.leaves | (m.inside != (1u << L) - 1);
-    const Affine<V> map = m.enters ? s.template reduce<true>(m) : s.template reduce<false>(m);
+    const Affine<V> map = m.enters ? s.template reduce<true>(rows, m) : s.template reduce<false>(rows, m);
+    // the next steps are on their way while these are finished
+    const int64_t next_first = first + span;
+    const bool next_all = whole_warp && next_first + L <= d.length;
+    if (base + span < to) {
+      if (next_all) s.template load<true>(next, next_first);
+      else s.template load<false>(next, next_first);
+      next_m = marks_of<L, BACK>(d, b, next_first);
+    }
     maps[parity][warp][lane] = map;
     if (lane == 0) begins[parity][warp] = m.enters != 0;
     __syncthreads();
@@ -431,6 +460,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       if (PASS == kMaps) {
         whole = {whole.A * block.A, apply(block, any, whole.H)};
         whole_begins |= any;
+        rows = next, m = next_m, first = next_first, all = next_all;
         continue;
       }
       cg::cluster_group cluster = cg::this_cluster();
@@ -457,8 +487,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
         carry = apply(maps[parity][w][lane], begins[parity][w], carry);
       }
     }
-    if (all && !marked) s.template write<true, false>(m, first, value);
-    else s.template write<false, true>(m, first, value);
+    if (all && !marked) s.template write<true, false>(rows, m, first, value);
+    else s.template write<false, true>(rows, m, first, value);
+    rows = next, m = next_m, first = next_first, all = next_all;
   }
   if (PASS == kMaps && warp == 0) {
     if (s.in)
@@ -469,11 +500,20 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   }
 }
 
-// Into how many parts the time axis of a call is cut, each part two launches' work: one map of it,
-// then its outputs.  1 where the columns alone, or a cluster over each, fill the GPU.
+// Blocks a cluster: as many as bring two blocks to every SM.
+int ranks_of(int64_t columns, int64_t spans) {
+  int ranks = 1;
+  while (ranks < kMaxRanks && columns * ranks < 2 * 148 && ranks < spans) ranks *= 2;
+  return ranks;
+}
+// Into how many parts the time axis is cut, each part two launches' work: its map, then its
+// outputs.  1 where one launch fills the GPU and its clusters do not walk long: measured, 256
+// columns of 64 spans take 101 us in one launch and 146 cut, 96 of 16 spans 16 and 21; but 96
+// columns of 65 spans 46 and 38, 16 of 63 spans 25 and 13, 12 of 2048 spans 728 and 217.
 constexpr int64_t kMaxParts = 64;
 int parts_of(int64_t columns, int64_t spans) {
-  if (columns >= 2 * 148 || (columns * 8 >= 2 * 148 && spans <= 16)) return 1;
+  const int ranks = ranks_of(columns, spans);
+  if (columns >= 148 || spans <= 2 * ranks || (columns * ranks >= 148 && spans <= 8 * ranks)) return 1;
   return (int)std::max<int64_t>(1, std::min({kMaxParts, (spans + 1) / 2, 8 * 148 / columns}));
 }
 
@@ -571,16 +611,17 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
     const cudaError_t e = launch<T, V, L, FORM, BACK, kMaps>(d, cut, stream);
     return e != cudaSuccess ? e : launch<T, V, L, FORM, BACK, kFromMaps>(d, cut, stream);
   }
-  while (cut.ranks < kMaxRanks && columns * cut.ranks < 2 * 148 && cut.ranks < spans) cut.ranks *= 2;
+  cut.ranks = ranks_of(columns, spans);
   return launch<T, V, L, FORM, BACK, kWhole>(d, cut, stream);
 }
 
 template <typename T, int FORM, bool BACK>
 cudaError_t enqueue_form(const tb_scan_desc& d, cudaStream_t stream) {
-  // the backward pass holds up to four arrays: 16 steps of each would spill
-  constexpr int kSteps = BACK && (sizeof(T) == 4 || FORM == TB_SCAN_SIGMOID) ? 8 : 16;
-  return lanes_fit(d, BACK, sizeof(T), 2 * sizeof(T)) ? enqueue<T, 2, kSteps, FORM, BACK>(d, stream)
-                                                      : enqueue<T, 1, 16, FORM, BACK>(d, stream);
+  // as many steps a warp as 128 registers hold, with the next ones on their way
+  constexpr int kPairs = sizeof(T) == 2 ? (BACK ? 8 : 16) : !BACK || FORM == TB_SCAN_DIRECT ? 8 : 4;
+  return lanes_fit(d, BACK, sizeof(T), 2 * sizeof(T))
+             ? enqueue<T, 2, kPairs, FORM, BACK>(d, stream)
+             : enqueue<T, 1, BACK ? 8 : 16, FORM, BACK>(d, stream);
 }
 
 template <typename T>
@@ -609,8 +650,12 @@ int scan_call(const char* name, const tb_scan_desc* desc, void* stream, bool bac
 
 int64_t scan_workspace(int64_t batch, int64_t length, int64_t channels) {
   if (!extents_fit({batch, length, channels}) || batch * length * channels == 0) return 0;
-  // the widest blocks make the fewest columns, the shortest spans the most parts
-  const int64_t parts = parts_of(batch * ((channels + 63) / 64), (length + kWarps * 8 - 1) / (kWarps * 8));
+  // whichever block the call takes: columns of 32 or 64 channels, spans of 4, 8 or 16 steps a warp
+  int64_t parts = 1;
+  for (int64_t width : {32, 64})
+    for (int64_t steps : {4, 8, 16})
+      parts = std::max<int64_t>(parts, parts_of(batch * ((channels + width - 1) / width),
+                                                (length + kWarps * steps - 1) / (kWarps * steps)));
   return parts > 1 ? (batch * parts * (channels * (int64_t)sizeof(float2) + 4) + 15) / 16 * 16 : 0;
 }
 }  // namespace tb
