@@ -1,5 +1,7 @@
 // rotate.cu -- the root-mean-square norm of every query and key head with the rotation by the
 // token's position, and its backward pass.
+#include <algorithm>
+
 #include "operators.h"
 
 namespace tb {
@@ -81,7 +83,339 @@ __global__ void k_rotate(tb_rotate_desc d, int64_t rows) {
   }
 }
 
-constexpr int64_t kBackwardBlocks = 296;  // rows of weight-gradient partials
+// ---- heads whose rows, halves and rests are whole 16- or 8-byte vectors
+//
+// G lanes take a head, each VEC pairs of its elements: a vector of first and a vector of second
+// elements (or, turned as adjacent pairs, two vectors in a row).  A warp takes 32 / G heads of one
+// token at a time, and kUnroll such sets, with one reading of the token's cosines and sines.
+template <typename T, int VEC>
+struct Chunk;
+template <>
+struct Chunk<float, 4> {
+  typedef float4 type;
+  static __device__ __forceinline__ void read(float4 r, float (&v)[4]) {
+    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  }
+  static __device__ __forceinline__ float4 made(const float (&v)[4]) { return {v[0], v[1], v[2], v[3]}; }
+};
+__device__ __forceinline__ void unpack(unsigned r, float& lo, float& hi) {
+  lo = __uint_as_float(r << 16);
+  hi = __uint_as_float(r & 0xffff0000u);
+}
+__device__ __forceinline__ unsigned pack(float lo, float hi) {
+  unsigned r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+struct Chunk<bf16, 4> {
+  typedef uint2 type;
+  static __device__ __forceinline__ void read(uint2 r, float (&v)[4]) {
+    unpack(r.x, v[0], v[1]);
+    unpack(r.y, v[2], v[3]);
+  }
+  static __device__ __forceinline__ uint2 made(const float (&v)[4]) {
+    return {pack(v[0], v[1]), pack(v[2], v[3])};
+  }
+};
+template <>
+struct Chunk<bf16, 8> {
+  typedef uint4 type;
+  static __device__ __forceinline__ void read(uint4 r, float (&v)[8]) {
+    unpack(r.x, v[0], v[1]);
+    unpack(r.y, v[2], v[3]);
+    unpack(r.z, v[4], v[5]);
+    unpack(r.w, v[6], v[7]);
+  }
+  static __device__ __forceinline__ uint4 made(const float (&v)[8]) {
+    return {pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
+  }
+};
+
+// A lane's part of a head: where its two vectors lie, and what is common to heads of its side.
+template <typename T, int VEC, bool ADJACENT>
+struct Part {
+  typedef Chunk<T, VEC> C;
+  typedef typename C::type Raw;
+  int first, second;  // element offsets
+  bool in, turns;
+  __device__ Part(const tb_rotate_desc& d, int chunk) {
+    const int half = (int)d.turned / 2, p = chunk * VEC;
+    in = p < (int)d.dim / 2;
+    turns = in && p < half;
+    if (ADJACENT) {
+      first = 2 * p;
+      second = first + VEC;
+    } else {
+      const Pair e = pair_of(p, (int)d.dim, (int)d.turned, TB_ROTATE_HALVES);
+      first = e.u;
+      second = e.v;
+    }
+  }
+  // Two vectors as first and second elements of the pairs, and back.
+  __device__ __forceinline__ void read(Raw r1, Raw r2, float (&u)[VEC], float (&v)[VEC]) const {
+    C::read(r1, u);
+    C::read(r2, v);
+    if (ADJACENT) swap(u, v, true);
+  }
+  __device__ __forceinline__ void made(float (&u)[VEC], float (&v)[VEC], Raw& r1, Raw& r2) const {
+    if (ADJACENT) swap(u, v, false);
+    r1 = C::made(u);
+    r2 = C::made(v);
+  }
+  // Pairs laid out one after the other in u, v <-> first elements in u, second in v.
+  static __device__ __forceinline__ void swap(float (&u)[VEC], float (&v)[VEC], bool apart) {
+    float w[2 * VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      w[j] = u[j];
+      w[VEC + j] = v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      if (apart) {  // 0 1 2 3 | 4 5 6 7 -> 0 2 4 6 | 1 3 5 7
+        u[j] = w[2 * j];
+        v[j] = w[2 * j + 1];
+      } else {
+        const int a = j, b = VEC + j;
+        u[j] = a % 2 ? w[VEC + a / 2] : w[a / 2];
+        v[j] = b % 2 ? w[VEC + b / 2] : w[b / 2];
+      }
+    }
+  }
+  __device__ __forceinline__ void angles(const tb_rotate_desc& d, int64_t position, int chunk,
+                                         float (&cosine)[VEC], float (&sine)[VEC]) const {
+    const bool known = position >= 0 && position < d.table_rows;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      cosine[j] = known ? 1.0f : NAN;
+      sine[j] = known ? 0.0f : NAN;
+    }
+    if (!turns || !known) return;
+    const float* row = d.table + position * d.turned + chunk * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {
+      const float4 c = *(const float4*)(row + j), s = *(const float4*)(row + d.turned / 2 + j);
+      cosine[j] = c.x, cosine[j + 1] = c.y, cosine[j + 2] = c.z, cosine[j + 3] = c.w;
+      sine[j] = s.x, sine[j + 1] = s.y, sine[j + 2] = s.z, sine[j + 3] = s.w;
+    }
+  }
+  __device__ __forceinline__ void weights(const float* w, float (&u)[VEC], float (&v)[VEC]) const {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) u[j] = v[j] = 1.0f;
+    if (!w || !in) return;
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {
+      const float4 a = *(const float4*)(w + first + j), b = *(const float4*)(w + second + j);
+      u[j] = a.x, u[j + 1] = a.y, u[j + 2] = a.z, u[j + 3] = a.w;
+      v[j] = b.x, v[j + 1] = b.y, v[j + 2] = b.z, v[j + 3] = b.w;
+    }
+    if (ADJACENT) swap(u, v, true);
+  }
+};
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// One side (queries or keys) of a call.
+struct Side {
+  const void *in, *grad;
+  void* out;
+  const float* weight;
+  int64_t in_s[3], grad_s[3], out_s[3];
+  int heads, blocks;  // blocks: sets of heads that a warp takes of one token
+};
+struct Sides {
+  Side q, k;
+  int64_t tokens;
+};
+
+constexpr int kUnroll = 2;
+
+template <typename T, int VEC, int G, bool ADJACENT>
+__global__ void __launch_bounds__(256) k_rotate_vectors(tb_rotate_desc d, Sides sides) {
+  pdl_entry();
+  typedef Part<T, VEC, ADJACENT> P;
+  typedef typename P::Raw Raw;
+  constexpr int kRows = 32 / G;
+  const int lane = threadIdx.x % 32, chunk = lane % G;
+  const int64_t item = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int blocks = sides.q.blocks + sides.k.blocks;
+  const int64_t token = item / blocks;
+  if (token >= sides.tokens) return;
+  int block = (int)(item - token * blocks);
+  const bool key = block >= sides.q.blocks;
+  const Side& side = key ? sides.k : sides.q;
+  if (key) block -= sides.q.blocks;
+  const int64_t b = token / d.length, t = token - b * d.length;
+  const P part(d, chunk);
+  const int head0 = block * kRows * kUnroll + lane / G;
+  const T* x = (const T*)side.in + b * side.in_s[0] + t * side.in_s[1] + head0 * side.in_s[2];
+  T* y = (T*)side.out + b * side.out_s[0] + t * side.out_s[1] + head0 * side.out_s[2];
+  Raw r1[kUnroll], r2[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    r1[i] = r2[i] = Raw{};
+    if (part.in && head0 + i * kRows < side.heads) {
+      r1[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.first);
+      r2[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.second);
+    }
+  }
+  float cosine[VEC], sine[VEC], wu[VEC], wv[VEC];
+  part.angles(d, d.positions ? d.positions[token] : t, chunk, cosine, sine);
+  part.weights(side.weight, wu, wv);
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+    float u[VEC], v[VEC], squares = 0;
+    part.read(r1[i], r2[i], u, v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) squares += u[j] * u[j] + v[j] * v[j];
+    const float scale = rsqrtf(group_sum<G>(squares) / (float)d.dim + (float)d.epsilon);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float p = u[j] * scale * wu[j], q = v[j] * scale * wv[j];
+      u[j] = p * cosine[j] - q * sine[j];
+      v[j] = q * cosine[j] + p * sine[j];
+    }
+    if (part.in && head0 + i * kRows < side.heads) {
+      Raw o1, o2;
+      part.made(u, v, o1, o2);
+      *(Raw*)(y + i * kRows * side.out_s[2] + part.first) = o1;
+      *(Raw*)(y + i * kRows * side.out_s[2] + part.second) = o2;
+    }
+  }
+}
+
+constexpr int64_t kBackwardBlocks = 2 * 148;  // of each side, at most: rows of partials
+
+// Blocks [0, q_blocks) take the query heads, the others the key heads, so that a lane holds one
+// side's part of the weight gradient in registers over all its tokens.
+template <typename T, int VEC, int G, bool ADJACENT>
+__global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_desc d, Sides sides,
+                                                                    int q_blocks) {
+  pdl_entry();
+  typedef Part<T, VEC, ADJACENT> P;
+  typedef typename P::Raw Raw;
+  constexpr int kRows = 32 / G, kWarps = 8;
+  __shared__ float sums[kWarps][2 * VEC][G];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, chunk = lane % G;
+  const bool key = (int)blockIdx.x >= q_blocks;
+  const Side& side = key ? sides.k : sides.q;
+  const int of = key ? gridDim.x - q_blocks : q_blocks, mine = key ? blockIdx.x - q_blocks : blockIdx.x;
+  const P part(d, chunk);
+  float wu[VEC], wv[VEC], du[VEC] = {}, dv[VEC] = {};
+  part.weights(side.weight, wu, wv);
+  for (int64_t item = (int64_t)mine * kWarps + warp; item < sides.tokens * side.blocks;
+       item += (int64_t)of * kWarps) {
+    const int64_t token = item / side.blocks;
+    const int head0 = (int)(item - token * side.blocks) * kRows * kUnroll + lane / G;
+    const int64_t b = token / d.length, t = token - b * d.length;
+    const T* x = (const T*)side.in + b * side.in_s[0] + t * side.in_s[1] + head0 * side.in_s[2];
+    const T* dy = (const T*)side.grad + b * side.grad_s[0] + t * side.grad_s[1] + head0 * side.grad_s[2];
+    T* dx = (T*)side.out + b * side.out_s[0] + t * side.out_s[1] + head0 * side.out_s[2];
+    Raw r1[kUnroll], r2[kUnroll], g1[kUnroll], g2[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      r1[i] = r2[i] = g1[i] = g2[i] = Raw{};
+      if (part.in && head0 + i * kRows < side.heads) {
+        r1[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.first);
+        r2[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.second);
+        g1[i] = *(const Raw*)(dy + i * kRows * side.grad_s[2] + part.first);
+        g2[i] = *(const Raw*)(dy + i * kRows * side.grad_s[2] + part.second);
+      }
+    }
+    float cosine[VEC], sine[VEC];
+    part.angles(d, d.positions ? d.positions[token] : t, chunk, cosine, sine);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const bool here = part.in && head0 + i * kRows < side.heads;
+      float u[VEC], v[VEC], gu[VEC], gv[VEC], squares = 0;
+      part.read(r1[i], r2[i], u, v);
+      part.read(g1[i], g2[i], gu, gv);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) squares += u[j] * u[j] + v[j] * v[j];
+      const float scale = rsqrtf(group_sum<G>(squares) / (float)d.dim + (float)d.epsilon);
+      float inner = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float p = gu[j] * cosine[j] + gv[j] * sine[j], q = gv[j] * cosine[j] - gu[j] * sine[j];
+        u[j] *= scale;
+        v[j] *= scale;
+        if (here) {
+          du[j] += p * u[j];
+          dv[j] += q * v[j];
+        }
+        gu[j] = p * wu[j];
+        gv[j] = q * wv[j];
+        inner += gu[j] * u[j] + gv[j] * v[j];
+      }
+      inner = group_sum<G>(part.in ? inner : 0.0f) / (float)d.dim;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        u[j] = scale * (gu[j] - u[j] * inner);
+        v[j] = scale * (gv[j] - v[j] * inner);
+      }
+      if (here) {
+        Raw o1, o2;
+        part.made(u, v, o1, o2);
+        *(Raw*)(dx + i * kRows * side.out_s[2] + part.first) = o1;
+        *(Raw*)(dx + i * kRows * side.out_s[2] + part.second) = o2;
+      }
+    }
+  }
+  if (!d.workspace) return;
+  // lanes of one chunk, then the warps, in a fixed order; the elements in their places
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+#pragma unroll
+    for (int o = 16; o >= G; o >>= 1) {
+      du[j] += __shfl_xor_sync(~0u, du[j], o);
+      dv[j] += __shfl_xor_sync(~0u, dv[j], o);
+    }
+  }
+  if (ADJACENT) P::swap(du, dv, false);
+  if (lane < G)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      sums[warp][j][chunk] = du[j];
+      sums[warp][VEC + j][chunk] = dv[j];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * VEC * G; i += 256) {
+    const int j = i / G, c = i % G;
+    const P at(d, c);
+    if (!at.in) continue;
+    float s = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += sums[w][j][c];
+    ((float*)d.workspace)[(int64_t)blockIdx.x * d.dim + (j < VEC ? at.first + j : at.second + j - VEC)] = s;
+  }
+}
+
+// Weight gradients: the blocks' partials in their order, 8 threads an element.
+__global__ void __launch_bounds__(256) k_rotate_weights(tb_rotate_desc d, int q_blocks, int blocks) {
+  pdl_entry();
+  __shared__ float sums[8][32];
+  const int dim = (int)d.dim, per_side = (dim + 31) / 32;
+  const bool key = (int)blockIdx.x >= per_side;
+  const int j = (blockIdx.x - (key ? per_side : 0)) * 32 + threadIdx.x % 32, row = threadIdx.x / 32;
+  const int from = key ? q_blocks : 0, to = key ? blocks : q_blocks;
+  float s = 0;
+  if (j < dim)
+    for (int b = from + row; b < to; b += 8) s += ((const float*)d.workspace)[(int64_t)b * dim + j];
+  sums[row][threadIdx.x % 32] = s;
+  __syncthreads();
+  float* out = key ? d.dk_weight : d.dq_weight;
+  if (row == 0 && j < dim && out) {
+    for (int r = 1; r < 8; ++r) s += sums[r][threadIdx.x];
+    out[j] = s;
+  }
+}
+
+// ---- any other head
 
 template <typename T>
 __global__ void k_rotate_backward(tb_rotate_desc d, int64_t rows) {
@@ -143,21 +477,10 @@ __global__ void k_rotate_backward(tb_rotate_desc d, int64_t rows) {
   for (int j = threadIdx.x; j < 2 * dim; j += blockDim.x) {
     float s = 0;
     for (int w = 0; w < warps; ++w) s += sums[w * 2 * dim + j];
-    ((float*)d.workspace)[(int64_t)blockIdx.x * 2 * dim + j] = s;
+    // all query rows of partials, then all key rows
+    const int64_t row = blockIdx.x + (j < dim ? 0 : gridDim.x);
+    ((float*)d.workspace)[row * dim + (j < dim ? j : j - dim)] = s;
   }
-}
-
-// Weight gradients: the partials in block order, 32 threads an element.
-__global__ void k_rotate_weights(tb_rotate_desc d) {
-  pdl_entry();
-  const int lane = threadIdx.x % 32, dim = (int)d.dim;
-  const int j = (int)((blockIdx.x * blockDim.x + threadIdx.x) / 32);
-  if (j >= 2 * dim) return;
-  float s = 0;
-  for (int b = lane; b < kBackwardBlocks; b += 32) s += ((const float*)d.workspace)[b * 2 * dim + j];
-  s = warp_sum(s);
-  float* out = j < dim ? d.dq_weight : d.dk_weight;
-  if (lane == 0 && out) out[j < dim ? j : j - dim] = s;
 }
 
 int64_t workspace_bytes(const tb_rotate_desc& d) {
@@ -208,22 +531,100 @@ const char* check(const tb_rotate_desc& d, bool backward) {
   return nullptr;
 }
 
+// Whether a side's heads are made of whole vectors of VEC elements.
+template <typename T, int VEC>
+bool vectors_fit(const tb_rotate_desc& d, const Side& side, bool backward) {
+  const auto fits = [&](const void* p, const int64_t s[3]) {
+    return aligned_to(p, VEC * sizeof(T)) && (d.batch <= 1 || s[0] % VEC == 0) &&
+           (d.length <= 1 || s[1] % VEC == 0) && (side.heads <= 1 || s[2] % VEC == 0);
+  };
+  return side.heads == 0 || (fits(side.in, side.in_s) && fits(side.out, side.out_s) &&
+                             (!backward || fits(side.grad, side.grad_s)) && aligned_to(side.weight, 16));
+}
+template <typename T, int VEC>
+bool vectors_fit(const tb_rotate_desc& d, const Sides& sides, bool backward) {
+  return d.turned / 2 % VEC == 0 && (d.dim - d.turned) / 2 % VEC == 0 && d.dim / 2 / VEC <= 32 &&
+         aligned_to(d.table, 16) && vectors_fit<T, VEC>(d, sides.q, backward) &&
+         vectors_fit<T, VEC>(d, sides.k, backward);
+}
+
+cudaError_t enqueue_weights(const tb_rotate_desc& d, int64_t q_blocks, int64_t blocks, cudaStream_t stream) {
+  return launch_pdl(k_rotate_weights, dim3((unsigned)(2 * ((d.dim + 31) / 32))), dim3(256), 0, stream,
+                    d, (int)q_blocks, (int)blocks);
+}
+
+template <typename T, int VEC, int G, bool ADJACENT>
+cudaError_t enqueue_vectors(const tb_rotate_desc& d, Sides sides, bool backward, cudaStream_t stream) {
+  constexpr int kHeads = 32 / G * kUnroll;
+  sides.q.blocks = (sides.q.heads + kHeads - 1) / kHeads;
+  sides.k.blocks = (sides.k.heads + kHeads - 1) / kHeads;
+  const int64_t q_items = sides.tokens * sides.q.blocks, k_items = sides.tokens * sides.k.blocks;
+  if (!backward) {
+    const int64_t blocks = (q_items + k_items + 7) / 8;
+    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    return launch_pdl(k_rotate_vectors<T, VEC, G, ADJACENT>, dim3((unsigned)blocks), dim3(256), 0,
+                      stream, d, sides);
+  }
+  // two blocks a SM, shared out by the sides' work
+  const int64_t most = 2 * 148;
+  int64_t q_blocks = q_items ? std::max<int64_t>(1, most * q_items / (q_items + k_items)) : 0;
+  int64_t k_blocks = k_items ? std::max<int64_t>(1, most - q_blocks) : 0;
+  q_blocks = std::min(q_blocks, (q_items + 7) / 8);
+  k_blocks = std::min(k_blocks, (k_items + 7) / 8);
+  cudaError_t e = launch_pdl(k_rotate_vectors_backward<T, VEC, G, ADJACENT>,
+                             dim3((unsigned)(q_blocks + k_blocks)), dim3(256), 0, stream, d, sides,
+                             (int)q_blocks);
+  return e == cudaSuccess && d.workspace ? enqueue_weights(d, q_blocks, q_blocks + k_blocks, stream) : e;
+}
+
+template <typename T, int VEC>
+cudaError_t enqueue_vectors(const tb_rotate_desc& d, const Sides& sides, bool backward, cudaStream_t stream) {
+  const int64_t chunks = d.dim / 2 / VEC;
+  const bool adjacent = d.style == TB_ROTATE_PAIRS;
+#define TB_ROTATE_GROUP(G)                                                                   \
+  if (chunks <= G)                                                                           \
+    return adjacent ? enqueue_vectors<T, VEC, G, true>(d, sides, backward, stream)           \
+                    : enqueue_vectors<T, VEC, G, false>(d, sides, backward, stream);
+  TB_ROTATE_GROUP(4)
+  TB_ROTATE_GROUP(8)
+  TB_ROTATE_GROUP(16)
+  TB_ROTATE_GROUP(32)
+#undef TB_ROTATE_GROUP
+  return cudaErrorInvalidValue;
+}
+
 template <typename T>
 cudaError_t enqueue(tb_rotate_desc d, bool backward, cudaStream_t stream) {
-  const int64_t rows = d.batch * d.length * (d.q_heads + d.k_heads);
+  const int64_t tokens = d.batch * d.length, rows = tokens * (d.q_heads + d.k_heads);
+  if (!backward || !workspace_bytes(d)) d.workspace = nullptr;
+  if (rows == 0) return d.workspace ? enqueue_weights(d, 0, 0, stream) : cudaSuccess;
+  Sides sides = {};
+  sides.tokens = tokens;
+  const auto side = [](Side& s, const void* in, const void* grad, void* out, const float* weight,
+                       const int64_t* in_s, const int64_t* grad_s, const int64_t* out_s, int64_t heads) {
+    s.in = in;
+    s.grad = grad;
+    s.out = out;
+    s.weight = weight;
+    std::copy(in_s, in_s + 3, s.in_s);
+    std::copy(grad_s, grad_s + 3, s.grad_s);
+    std::copy(out_s, out_s + 3, s.out_s);
+    s.heads = (int)heads;
+  };
+  side(sides.q, d.q, d.dq, d.q_out, d.q_weight, d.q_strides, d.dq_strides, d.q_out_strides, d.q_heads);
+  side(sides.k, d.k, d.dk, d.k_out, d.k_weight, d.k_strides, d.dk_strides, d.k_out_strides, d.k_heads);
+  constexpr int kVec = 16 / sizeof(T);
+  if (vectors_fit<T, kVec>(d, sides, backward)) return enqueue_vectors<T, kVec>(d, sides, backward, stream);
+  if constexpr (kVec == 8)
+    if (vectors_fit<T, 4>(d, sides, backward)) return enqueue_vectors<T, 4>(d, sides, backward, stream);
   if (!backward) {
     const int64_t blocks = (rows + 7) / 8;
     if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-    return blocks ? launch_pdl(k_rotate<T>, dim3((unsigned)blocks), dim3(256), 0, stream, d, rows)
-                  : cudaSuccess;
+    return launch_pdl(k_rotate<T>, dim3((unsigned)blocks), dim3(256), 0, stream, d, rows);
   }
-  if (!workspace_bytes(d)) d.workspace = nullptr;
-  if (!rows && !d.workspace) return cudaSuccess;
-  cudaError_t e = launch_pdl(k_rotate_backward<T>, dim3(kBackwardBlocks), dim3(256),
-                             (size_t)8 * 2 * d.dim * 4, stream, d, rows);
-  if (e == cudaSuccess && d.workspace)
-    e = launch_pdl(k_rotate_weights, dim3((unsigned)((2 * d.dim + 7) / 8)), dim3(256), 0, stream, d);
-  return e;
+  const cudaError_t e = launch_pdl(k_rotate_backward<T>, dim3(kBackwardBlocks), dim3(256),
+                                   (size_t)8 * 2 * d.dim * 4, stream, d, rows);
+  return e == cudaSuccess && d.workspace ? enqueue_weights(d, kBackwardBlocks, 2 * kBackwardBlocks, stream) : e;
 }
 
 int rotate_call(const char* name, const tb_rotate_desc* desc, void* stream, bool backward) {
