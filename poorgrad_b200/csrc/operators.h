@@ -27,6 +27,44 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two f32 operations in one instruction (sm_100's packed f32x2 forms, each rounded as its scalar).
+__device__ __forceinline__ unsigned long long packed(float2 v) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpacked(unsigned long long r) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+  return v;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
+  return unpacked(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
+  return unpacked(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)), "l"(packed(c)));
+  return unpacked(r);
+}
+__device__ __forceinline__ float2 both(float v) { return {v, v}; }
+
+// Two bf16 values of one word, the lower first, and back.
+__device__ __forceinline__ float2 unpack_bf16(unsigned r) {
+  return {__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)};
+}
+__device__ __forceinline__ unsigned pack_bf16(float2 v) {
+  unsigned r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+
 // The frame of an operator's entry point: the request is checked first, then the library's
 // state, then the work is enqueued on the caller's stream.
 class OperatorCall {

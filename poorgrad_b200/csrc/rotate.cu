@@ -83,53 +83,56 @@ __global__ void k_rotate(tb_rotate_desc d, int64_t rows) {
   }
 }
 
-// ---- heads whose rows, halves and rests are whole 16- or 8-byte vectors
+// ---- heads of up to 64 elements, or whose rows, halves and rests are whole 16- or 8-byte vectors
 //
 // G lanes take a head, each VEC pairs of its elements: a vector of first and a vector of second
 // elements (or, turned as adjacent pairs, two vectors in a row).  A warp takes 32 / G heads of one
-// token at a time, and kUnroll such sets, with one reading of the token's cosines and sines.
+// token at a time, and UNROLL such sets, with one reading of the token's cosines and sines.
+// VEC elements as VEC / 2 pairs of f32, for the packed instructions.
 template <typename T, int VEC>
 struct Chunk;
 template <>
 struct Chunk<float, 4> {
   typedef float4 type;
-  static __device__ __forceinline__ void read(float4 r, float (&v)[4]) {
-    v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
+  static __device__ __forceinline__ void read(float4 r, float2 (&v)[2]) {
+    v[0] = {r.x, r.y};
+    v[1] = {r.z, r.w};
   }
-  static __device__ __forceinline__ float4 made(const float (&v)[4]) { return {v[0], v[1], v[2], v[3]}; }
+  static __device__ __forceinline__ float4 made(const float2 (&v)[2]) {
+    return {v[0].x, v[0].y, v[1].x, v[1].y};
+  }
 };
-__device__ __forceinline__ void unpack(unsigned r, float& lo, float& hi) {
-  lo = __uint_as_float(r << 16);
-  hi = __uint_as_float(r & 0xffff0000u);
-}
-__device__ __forceinline__ unsigned pack(float lo, float hi) {
-  unsigned r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 template <>
 struct Chunk<bf16, 4> {
   typedef uint2 type;
-  static __device__ __forceinline__ void read(uint2 r, float (&v)[4]) {
-    unpack(r.x, v[0], v[1]);
-    unpack(r.y, v[2], v[3]);
+  static __device__ __forceinline__ void read(uint2 r, float2 (&v)[2]) {
+    v[0] = unpack_bf16(r.x);
+    v[1] = unpack_bf16(r.y);
   }
-  static __device__ __forceinline__ uint2 made(const float (&v)[4]) {
-    return {pack(v[0], v[1]), pack(v[2], v[3])};
+  static __device__ __forceinline__ uint2 made(const float2 (&v)[2]) {
+    return {pack_bf16(v[0]), pack_bf16(v[1])};
   }
 };
 template <>
 struct Chunk<bf16, 8> {
   typedef uint4 type;
-  static __device__ __forceinline__ void read(uint4 r, float (&v)[8]) {
-    unpack(r.x, v[0], v[1]);
-    unpack(r.y, v[2], v[3]);
-    unpack(r.z, v[4], v[5]);
-    unpack(r.w, v[6], v[7]);
+  static __device__ __forceinline__ void read(uint4 r, float2 (&v)[4]) {
+    v[0] = unpack_bf16(r.x);
+    v[1] = unpack_bf16(r.y);
+    v[2] = unpack_bf16(r.z);
+    v[3] = unpack_bf16(r.w);
   }
-  static __device__ __forceinline__ uint4 made(const float (&v)[8]) {
-    return {pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])};
+  static __device__ __forceinline__ uint4 made(const float2 (&v)[4]) {
+    return {pack_bf16(v[0]), pack_bf16(v[1]), pack_bf16(v[2]), pack_bf16(v[3])};
   }
+};
+
+// Single elements, for heads whose rows are not aligned: the second of each pair of f32 is unused.
+template <typename T>
+struct Chunk<T, 1> {
+  typedef T type;
+  static __device__ __forceinline__ void read(T r, float2 (&v)[1]) { v[0] = {to_f32(r), 0.0f}; }
+  static __device__ __forceinline__ T made(const float2 (&v)[1]) { return from_f32<T>(v[0].x); }
 };
 
 // A lane's part of a head: where its two vectors lie, and what is common to heads of its side.
@@ -137,6 +140,7 @@ template <typename T, int VEC, bool ADJACENT>
 struct Part {
   typedef Chunk<T, VEC> C;
   typedef typename C::type Raw;
+  static constexpr int N = (VEC + 1) / 2;
   int first, second;  // element offsets
   bool in, turns;
   __device__ Part(const tb_rotate_desc& d, int chunk) {
@@ -153,66 +157,84 @@ struct Part {
     }
   }
   // Two vectors as first and second elements of the pairs, and back.
-  __device__ __forceinline__ void read(Raw r1, Raw r2, float (&u)[VEC], float (&v)[VEC]) const {
+  __device__ __forceinline__ void read(Raw r1, Raw r2, float2 (&u)[N], float2 (&v)[N]) const {
     C::read(r1, u);
     C::read(r2, v);
-    if (ADJACENT) swap(u, v, true);
+    if (ADJACENT) apart(u, v);
   }
-  __device__ __forceinline__ void made(float (&u)[VEC], float (&v)[VEC], Raw& r1, Raw& r2) const {
-    if (ADJACENT) swap(u, v, false);
+  __device__ __forceinline__ void made(float2 (&u)[N], float2 (&v)[N], Raw& r1, Raw& r2) const {
+    if (ADJACENT) joined(u, v);
     r1 = C::made(u);
     r2 = C::made(v);
   }
-  // Pairs laid out one after the other in u, v <-> first elements in u, second in v.
-  static __device__ __forceinline__ void swap(float (&u)[VEC], float (&v)[VEC], bool apart) {
-    float w[2 * VEC];
+  // 0 1 2 3 | 4 5 6 7 -> 0 2 4 6 | 1 3 5 7, and back.
+  static __device__ __forceinline__ void apart(float2 (&u)[N], float2 (&v)[N]) {
+    if constexpr (VEC > 1) {
+      float2 w[2 * N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[j] = u[j];
-      w[VEC + j] = v[j];
-    }
+      for (int j = 0; j < N; ++j) w[j] = u[j], w[N + j] = v[j];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (apart) {  // 0 1 2 3 | 4 5 6 7 -> 0 2 4 6 | 1 3 5 7
-        u[j] = w[2 * j];
-        v[j] = w[2 * j + 1];
-      } else {
-        const int a = j, b = VEC + j;
-        u[j] = a % 2 ? w[VEC + a / 2] : w[a / 2];
-        v[j] = b % 2 ? w[VEC + b / 2] : w[b / 2];
+      for (int j = 0; j < N; ++j) {
+        u[j] = {w[2 * j].x, w[2 * j + 1].x};
+        v[j] = {w[2 * j].y, w[2 * j + 1].y};
       }
     }
   }
-  __device__ __forceinline__ void angles(const tb_rotate_desc& d, int64_t position, int chunk,
-                                         float (&cosine)[VEC], float (&sine)[VEC]) const {
+  static __device__ __forceinline__ void joined(float2 (&u)[N], float2 (&v)[N]) {
+    if constexpr (VEC > 1) {
+      float2 w[2 * N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        w[2 * j] = {u[j].x, v[j].x};
+        w[2 * j + 1] = {u[j].y, v[j].y};
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[j] = w[j], v[j] = w[N + j];
+    }
+  }
+  static __device__ __forceinline__ void load(const float* from, float2 (&v)[N]) {
+    if constexpr (VEC == 1) {
+      v[0] = {from[0], 0.0f};
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        [[maybe_unused]] const float4 a = *(const float4*)(from + 2 * j);
+        v[j] = {a.x, a.y};
+        v[j + 1] = {a.z, a.w};
+      }
+    }
+  }
+  __device__ __forceinline__ void angles(const tb_rotate_desc& d, int position, int chunk,
+                                         float2 (&cosine)[N], float2 (&sine)[N]) const {
     const bool known = position >= 0 && position < d.table_rows;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      cosine[j] = known ? 1.0f : NAN;
-      sine[j] = known ? 0.0f : NAN;
+    for (int j = 0; j < N; ++j) {
+      cosine[j] = both(known ? 1.0f : NAN);
+      sine[j] = both(known ? 0.0f : NAN);
     }
     if (!turns || !known) return;
     const float* row = d.table + position * d.turned + chunk * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const float4 c = *(const float4*)(row + j), s = *(const float4*)(row + d.turned / 2 + j);
-      cosine[j] = c.x, cosine[j + 1] = c.y, cosine[j + 2] = c.z, cosine[j + 3] = c.w;
-      sine[j] = s.x, sine[j + 1] = s.y, sine[j + 2] = s.z, sine[j + 3] = s.w;
-    }
+    load(row, cosine);
+    load(row + d.turned / 2, sine);
   }
-  __device__ __forceinline__ void weights(const float* w, float (&u)[VEC], float (&v)[VEC]) const {
+  __device__ __forceinline__ void weights(const float* w, float2 (&u)[N], float2 (&v)[N]) const {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) u[j] = v[j] = 1.0f;
+    for (int j = 0; j < N; ++j) u[j] = v[j] = both(1.0f);
     if (!w || !in) return;
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4) {
-      const float4 a = *(const float4*)(w + first + j), b = *(const float4*)(w + second + j);
-      u[j] = a.x, u[j + 1] = a.y, u[j + 2] = a.z, u[j + 3] = a.w;
-      v[j] = b.x, v[j + 1] = b.y, v[j + 2] = b.z, v[j + 3] = b.w;
-    }
-    if (ADJACENT) swap(u, v, true);
+    load(w + first, u);
+    load(w + second, v);
+    if (ADJACENT) apart(u, v);
   }
 };
+template <int N>
+__device__ __forceinline__ float squares_of(const float2 (&u)[N], const float2 (&v)[N]) {
+  float2 s = mul2(u[0], u[0]);
+#pragma unroll
+  for (int j = 1; j < N; ++j) s = fma2(u[j], u[j], s);
+#pragma unroll
+  for (int j = 0; j < N; ++j) s = fma2(v[j], v[j], s);
+  return s.x + s.y;
+}
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -233,165 +255,198 @@ struct Sides {
   int64_t tokens;
 };
 
-constexpr int kUnroll = 2;
+// The set of heads that a warp takes in one go: item / blocks is the token, the rest the set.
+struct Item {
+  unsigned token, b, t;
+  int from;  // first head of the set
+  __device__ Item(const tb_rotate_desc& d, const Side& side, unsigned item, int heads) {
+    token = item / (unsigned)side.blocks;
+    from = (int)(item - token * side.blocks) * heads;
+    b = token / (unsigned)d.length;
+    t = token - b * (unsigned)d.length;
+  }
+  __device__ __forceinline__ int64_t offset(const int64_t s[3], int head) const {
+    return b * s[0] + t * s[1] + head * s[2];
+  }
+  __device__ __forceinline__ int position(const tb_rotate_desc& d) const {
+    return d.positions ? d.positions[token] : (int)t;
+  }
+};
 
-template <typename T, int VEC, int G, bool ADJACENT>
-__global__ void __launch_bounds__(256) k_rotate_vectors(tb_rotate_desc d, Sides sides) {
+// Blocks [0, q_blocks) take the query heads, the others the key heads, each warp one item after
+// the other: the weights stay in registers, and the next item's position is read an item ahead,
+// for the angles wait for it.
+template <typename T, int VEC, int G, bool ADJACENT, int UNROLL>
+__global__ void __launch_bounds__(256, 3) k_rotate_vectors(tb_rotate_desc d, Sides sides, int q_blocks) {
   pdl_entry();
   typedef Part<T, VEC, ADJACENT> P;
   typedef typename P::Raw Raw;
-  constexpr int kRows = 32 / G;
-  const int lane = threadIdx.x % 32, chunk = lane % G;
-  const int64_t item = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int blocks = sides.q.blocks + sides.k.blocks;
-  const int64_t token = item / blocks;
-  if (token >= sides.tokens) return;
-  int block = (int)(item - token * blocks);
-  const bool key = block >= sides.q.blocks;
+  constexpr int kRows = 32 / G, kWarps = 8, N = (VEC + 1) / 2;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, chunk = lane % G;
+  const bool key = (int)blockIdx.x >= q_blocks;
   const Side& side = key ? sides.k : sides.q;
-  if (key) block -= sides.q.blocks;
-  const int64_t b = token / d.length, t = token - b * d.length;
+  const int of = key ? gridDim.x - q_blocks : q_blocks, mine = key ? blockIdx.x - q_blocks : blockIdx.x;
   const P part(d, chunk);
-  const int head0 = block * kRows * kUnroll + lane / G;
-  const T* x = (const T*)side.in + b * side.in_s[0] + t * side.in_s[1] + head0 * side.in_s[2];
-  T* y = (T*)side.out + b * side.out_s[0] + t * side.out_s[1] + head0 * side.out_s[2];
-  Raw r1[kUnroll], r2[kUnroll];
-#pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    r1[i] = r2[i] = Raw{};
-    if (part.in && head0 + i * kRows < side.heads) {
-      r1[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.first);
-      r2[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.second);
-    }
-  }
-  float cosine[VEC], sine[VEC], wu[VEC], wv[VEC];
-  part.angles(d, d.positions ? d.positions[token] : t, chunk, cosine, sine);
+  const float share = 1.0f / (float)d.dim, epsilon = (float)d.epsilon;
+  const unsigned items = (unsigned)sides.tokens * side.blocks;
+  unsigned i = mine * kWarps + warp;
+  if (i >= items) return;
+  int position = Item(d, side, i, kRows * UNROLL).position(d);
+  float2 wu[N], wv[N];
   part.weights(side.weight, wu, wv);
+  for (; i < items; i += of * kWarps) {
+    const Item item(d, side, i, kRows * UNROLL);
+    const int head0 = item.from + lane / G;
+    const T* x = (const T*)side.in + item.offset(side.in_s, head0);
+    T* y = (T*)side.out + item.offset(side.out_s, head0);
+    Raw r1[UNROLL], r2[UNROLL];
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    float u[VEC], v[VEC], squares = 0;
-    part.read(r1[i], r2[i], u, v);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) squares += u[j] * u[j] + v[j] * v[j];
-    const float scale = rsqrtf(group_sum<G>(squares) / (float)d.dim + (float)d.epsilon);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float p = u[j] * scale * wu[j], q = v[j] * scale * wv[j];
-      u[j] = p * cosine[j] - q * sine[j];
-      v[j] = q * cosine[j] + p * sine[j];
+    for (int h = 0; h < UNROLL; ++h) {
+      r1[h] = r2[h] = Raw{};
+      if (part.in && head0 + h * kRows < side.heads) {
+        const T* row = x + h * kRows * side.in_s[2];
+        r1[h] = *(const Raw*)(row + part.first);
+        r2[h] = *(const Raw*)(row + part.second);
+      }
     }
-    if (part.in && head0 + i * kRows < side.heads) {
-      Raw o1, o2;
-      part.made(u, v, o1, o2);
-      *(Raw*)(y + i * kRows * side.out_s[2] + part.first) = o1;
-      *(Raw*)(y + i * kRows * side.out_s[2] + part.second) = o2;
+    float2 cosine[N], sine[N];
+    part.angles(d, position, chunk, cosine, sine);
+    if (i + of * kWarps < items) position = Item(d, side, i + of * kWarps, kRows * UNROLL).position(d);
+#pragma unroll
+    for (int h = 0; h < UNROLL; ++h) {
+      if (item.from + h * kRows >= side.heads) break;
+      float2 u[N], v[N];
+      part.read(r1[h], r2[h], u, v);
+      const float scale = rsqrtf(group_sum<G>(squares_of(u, v)) * share + epsilon);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float2 p = mul2(mul2(u[j], both(scale)), wu[j]), q = mul2(mul2(v[j], both(scale)), wv[j]);
+        u[j] = fma2(p, cosine[j], mul2(mul2(q, both(-1.0f)), sine[j]));
+        v[j] = fma2(q, cosine[j], mul2(p, sine[j]));
+      }
+      if (part.in && head0 + h * kRows < side.heads) {
+        Raw o1, o2;
+        part.made(u, v, o1, o2);
+        T* row = y + h * kRows * side.out_s[2];
+        *(Raw*)(row + part.first) = o1;
+        *(Raw*)(row + part.second) = o2;
+      }
     }
   }
 }
 
 constexpr int64_t kBackwardBlocks = 2 * 148;  // of each side, at most: rows of partials
 
-// Blocks [0, q_blocks) take the query heads, the others the key heads, so that a lane holds one
-// side's part of the weight gradient in registers over all its tokens.
-template <typename T, int VEC, int G, bool ADJACENT>
+// The same division of work; a lane holds its part of the weight gradient in registers.
+template <typename T, int VEC, int G, bool ADJACENT, int UNROLL>
 __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_desc d, Sides sides,
                                                                     int q_blocks) {
   pdl_entry();
   typedef Part<T, VEC, ADJACENT> P;
   typedef typename P::Raw Raw;
-  constexpr int kRows = 32 / G, kWarps = 8;
-  __shared__ float sums[kWarps][2 * VEC][G];
+  constexpr int kRows = 32 / G, kWarps = 8, N = (VEC + 1) / 2;
+  __shared__ float2 sums[kWarps][2 * N][G];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, chunk = lane % G;
   const bool key = (int)blockIdx.x >= q_blocks;
   const Side& side = key ? sides.k : sides.q;
   const int of = key ? gridDim.x - q_blocks : q_blocks, mine = key ? blockIdx.x - q_blocks : blockIdx.x;
   const P part(d, chunk);
-  float wu[VEC], wv[VEC], du[VEC] = {}, dv[VEC] = {};
+  const float share = 1.0f / (float)d.dim, epsilon = (float)d.epsilon;
+  float2 wu[N], wv[N], du[N], dv[N];
   part.weights(side.weight, wu, wv);
-  for (int64_t item = (int64_t)mine * kWarps + warp; item < sides.tokens * side.blocks;
-       item += (int64_t)of * kWarps) {
-    const int64_t token = item / side.blocks;
-    const int head0 = (int)(item - token * side.blocks) * kRows * kUnroll + lane / G;
-    const int64_t b = token / d.length, t = token - b * d.length;
-    const T* x = (const T*)side.in + b * side.in_s[0] + t * side.in_s[1] + head0 * side.in_s[2];
-    const T* dy = (const T*)side.grad + b * side.grad_s[0] + t * side.grad_s[1] + head0 * side.grad_s[2];
-    T* dx = (T*)side.out + b * side.out_s[0] + t * side.out_s[1] + head0 * side.out_s[2];
-    Raw r1[kUnroll], r2[kUnroll], g1[kUnroll], g2[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      r1[i] = r2[i] = g1[i] = g2[i] = Raw{};
-      if (part.in && head0 + i * kRows < side.heads) {
-        r1[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.first);
-        r2[i] = *(const Raw*)(x + i * kRows * side.in_s[2] + part.second);
-        g1[i] = *(const Raw*)(dy + i * kRows * side.grad_s[2] + part.first);
-        g2[i] = *(const Raw*)(dy + i * kRows * side.grad_s[2] + part.second);
+  for (int j = 0; j < N; ++j) du[j] = dv[j] = both(0.0f);
+  const unsigned items = (unsigned)sides.tokens * side.blocks;
+  unsigned i = mine * kWarps + warp;
+  int position = i < items ? Item(d, side, i, kRows * UNROLL).position(d) : 0;
+  for (; i < items; i += of * kWarps) {
+    const Item item(d, side, i, kRows * UNROLL);
+    const int from = item.from, head0 = from + lane / G;
+    const T* x = (const T*)side.in + item.offset(side.in_s, head0);
+    const T* dy = (const T*)side.grad + item.offset(side.grad_s, head0);
+    T* dx = (T*)side.out + item.offset(side.out_s, head0);
+    Raw r1[UNROLL], r2[UNROLL], g1[UNROLL], g2[UNROLL];
+#pragma unroll
+    for (int h = 0; h < UNROLL; ++h) {
+      r1[h] = r2[h] = g1[h] = g2[h] = Raw{};
+      if (part.in && head0 + h * kRows < side.heads) {
+        const T *row = x + h * kRows * side.in_s[2], *grad = dy + h * kRows * side.grad_s[2];
+        r1[h] = *(const Raw*)(row + part.first);
+        r2[h] = *(const Raw*)(row + part.second);
+        g1[h] = *(const Raw*)(grad + part.first);
+        g2[h] = *(const Raw*)(grad + part.second);
       }
     }
-    float cosine[VEC], sine[VEC];
-    part.angles(d, d.positions ? d.positions[token] : t, chunk, cosine, sine);
+    float2 cosine[N], sine[N];
+    part.angles(d, position, chunk, cosine, sine);
+    if (i + of * kWarps < items) position = Item(d, side, i + of * kWarps, kRows * UNROLL).position(d);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const bool here = part.in && head0 + i * kRows < side.heads;
-      float u[VEC], v[VEC], gu[VEC], gv[VEC], squares = 0;
-      part.read(r1[i], r2[i], u, v);
-      part.read(g1[i], g2[i], gu, gv);
+    for (int h = 0; h < UNROLL; ++h) {
+      if (from + h * kRows >= side.heads) break;
+      const bool here = part.in && head0 + h * kRows < side.heads;
+      float2 u[N], v[N], gu[N], gv[N];
+      part.read(r1[h], r2[h], u, v);
+      part.read(g1[h], g2[h], gu, gv);
+      const float scale = rsqrtf(group_sum<G>(squares_of(u, v)) * share + epsilon);
+      float2 inner = both(0.0f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) squares += u[j] * u[j] + v[j] * v[j];
-      const float scale = rsqrtf(group_sum<G>(squares) / (float)d.dim + (float)d.epsilon);
-      float inner = 0;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float p = gu[j] * cosine[j] + gv[j] * sine[j], q = gv[j] * cosine[j] - gu[j] * sine[j];
-        u[j] *= scale;
-        v[j] *= scale;
+      for (int j = 0; j < N; ++j) {
+        const float2 p = fma2(gu[j], cosine[j], mul2(gv[j], sine[j]));
+        const float2 q = fma2(gv[j], cosine[j], mul2(mul2(gu[j], both(-1.0f)), sine[j]));
+        u[j] = mul2(u[j], both(scale));
+        v[j] = mul2(v[j], both(scale));
         if (here) {
-          du[j] += p * u[j];
-          dv[j] += q * v[j];
+          du[j] = fma2(p, u[j], du[j]);
+          dv[j] = fma2(q, v[j], dv[j]);
         }
-        gu[j] = p * wu[j];
-        gv[j] = q * wv[j];
-        inner += gu[j] * u[j] + gv[j] * v[j];
+        gu[j] = mul2(p, wu[j]);
+        gv[j] = mul2(q, wv[j]);
+        inner = fma2(gu[j], u[j], fma2(gv[j], v[j], inner));
       }
-      inner = group_sum<G>(part.in ? inner : 0.0f) / (float)d.dim;
+      const float mean = group_sum<G>(part.in ? inner.x + inner.y : 0.0f) * share;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        u[j] = scale * (gu[j] - u[j] * inner);
-        v[j] = scale * (gv[j] - v[j] * inner);
+      for (int j = 0; j < N; ++j) {
+        u[j] = mul2(both(scale), fma2(u[j], both(-mean), gu[j]));
+        v[j] = mul2(both(scale), fma2(v[j], both(-mean), gv[j]));
       }
       if (here) {
         Raw o1, o2;
         part.made(u, v, o1, o2);
-        *(Raw*)(dx + i * kRows * side.out_s[2] + part.first) = o1;
-        *(Raw*)(dx + i * kRows * side.out_s[2] + part.second) = o2;
+        T* row = dx + h * kRows * side.out_s[2];
+        *(Raw*)(row + part.first) = o1;
+        *(Raw*)(row + part.second) = o2;
       }
     }
   }
   if (!d.workspace) return;
   // lanes of one chunk, then the warps, in a fixed order; the elements in their places
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
+  for (int j = 0; j < N; ++j) {
 #pragma unroll
     for (int o = 16; o >= G; o >>= 1) {
-      du[j] += __shfl_xor_sync(~0u, du[j], o);
-      dv[j] += __shfl_xor_sync(~0u, dv[j], o);
+      du[j] = add2(du[j], {__shfl_xor_sync(~0u, du[j].x, o), __shfl_xor_sync(~0u, du[j].y, o)});
+      dv[j] = add2(dv[j], {__shfl_xor_sync(~0u, dv[j].x, o), __shfl_xor_sync(~0u, dv[j].y, o)});
     }
   }
-  if (ADJACENT) P::swap(du, dv, false);
+  if (ADJACENT) P::joined(du, dv);
   if (lane < G)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
+    for (int j = 0; j < N; ++j) {
       sums[warp][j][chunk] = du[j];
-      sums[warp][VEC + j][chunk] = dv[j];
+      sums[warp][N + j][chunk] = dv[j];
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * VEC * G; i += 256) {
+  for (int i = threadIdx.x; i < 2 * N * G; i += 256) {
     const int j = i / G, c = i % G;
     const P at(d, c);
     if (!at.in) continue;
-    float s = 0;
+    float2 s = sums[0][j][c];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += sums[w][j][c];
-    ((float*)d.workspace)[(int64_t)blockIdx.x * d.dim + (j < VEC ? at.first + j : at.second + j - VEC)] = s;
+    for (int w = 1; w < kWarps; ++w) s = add2(s, sums[w][j][c]);
+    float* to = (float*)d.workspace + (int64_t)blockIdx.x * d.dim;
+    to += j < N ? at.first + 2 * j : at.second + 2 * (j - N);
+    if constexpr (VEC == 1) *to = s.x;
+    else *(float2*)to = s;
   }
 }
 
@@ -415,7 +470,7 @@ __global__ void __launch_bounds__(256) k_rotate_weights(tb_rotate_desc d, int q_
   }
 }
 
-// ---- any other head
+// ---- any other head: a warp each
 
 template <typename T>
 __global__ void k_rotate_backward(tb_rotate_desc d, int64_t rows) {
@@ -499,7 +554,7 @@ const char* check(const tb_rotate_desc& d, bool backward) {
   if (d.style != TB_ROTATE_HALVES && d.style != TB_ROTATE_PAIRS) return "unknown style";
   if (!extents_fit({d.batch, d.length, d.q_heads, d.dim}) || d.length > INT32_MAX ||
       !extents_fit({d.batch, d.length, d.k_heads, d.dim}) || !extents_fit({d.table_rows, d.turned}) ||
-      d.q_heads > INT32_MAX / 2 || d.k_heads > INT32_MAX / 2)
+      d.batch * d.length * (d.q_heads + d.k_heads) > INT32_MAX)
     return "extents out of range";
   if (d.dim < 2 || d.dim > 512 || d.dim % 2) return "dim is even and at most 512";
   if (d.turned < 0 || d.turned > d.dim || d.turned % 2) return "turned is even and at most dim";
@@ -539,12 +594,13 @@ bool vectors_fit(const tb_rotate_desc& d, const Side& side, bool backward) {
            (d.length <= 1 || s[1] % VEC == 0) && (side.heads <= 1 || s[2] % VEC == 0);
   };
   return side.heads == 0 || (fits(side.in, side.in_s) && fits(side.out, side.out_s) &&
-                             (!backward || fits(side.grad, side.grad_s)) && aligned_to(side.weight, 16));
+                             (!backward || fits(side.grad, side.grad_s)) &&
+                              aligned_to(side.weight, VEC == 1 ? 4 : 16));
 }
 template <typename T, int VEC>
 bool vectors_fit(const tb_rotate_desc& d, const Sides& sides, bool backward) {
   return d.turned / 2 % VEC == 0 && (d.dim - d.turned) / 2 % VEC == 0 && d.dim / 2 / VEC <= 32 &&
-         aligned_to(d.table, 16) && vectors_fit<T, VEC>(d, sides.q, backward) &&
+         aligned_to(d.table, VEC == 1 ? 4 : 16) && vectors_fit<T, VEC>(d, sides.q, backward) &&
          vectors_fit<T, VEC>(d, sides.k, backward);
 }
 
@@ -555,23 +611,22 @@ cudaError_t enqueue_weights(const tb_rotate_desc& d, int64_t q_blocks, int64_t b
 
 template <typename T, int VEC, int G, bool ADJACENT>
 cudaError_t enqueue_vectors(const tb_rotate_desc& d, Sides sides, bool backward, cudaStream_t stream) {
-  constexpr int kHeads = 32 / G * kUnroll;
+  // sets of heads a warp takes in one go: as many loads as its registers hold
+  constexpr int kUnroll = VEC == 8 ? 2 : 4;
+  const int kHeads = 32 / G * kUnroll;
   sides.q.blocks = (sides.q.heads + kHeads - 1) / kHeads;
   sides.k.blocks = (sides.k.heads + kHeads - 1) / kHeads;
   const int64_t q_items = sides.tokens * sides.q.blocks, k_items = sides.tokens * sides.k.blocks;
-  if (!backward) {
-    const int64_t blocks = (q_items + k_items + 7) / 8;
-    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-    return launch_pdl(k_rotate_vectors<T, VEC, G, ADJACENT>, dim3((unsigned)blocks), dim3(256), 0,
-                      stream, d, sides);
-  }
-  // two blocks a SM, shared out by the sides' work
-  const int64_t most = 2 * 148;
+  // as many blocks as run at once, shared out by the sides' work
+  const int64_t most = (backward ? 2 : 3) * 148;
   int64_t q_blocks = q_items ? std::max<int64_t>(1, most * q_items / (q_items + k_items)) : 0;
   int64_t k_blocks = k_items ? std::max<int64_t>(1, most - q_blocks) : 0;
   q_blocks = std::min(q_blocks, (q_items + 7) / 8);
   k_blocks = std::min(k_blocks, (k_items + 7) / 8);
-  cudaError_t e = launch_pdl(k_rotate_vectors_backward<T, VEC, G, ADJACENT>,
+  if (!backward)
+    return launch_pdl(k_rotate_vectors<T, VEC, G, ADJACENT, kUnroll>,
+                      dim3((unsigned)(q_blocks + k_blocks)), dim3(256), 0, stream, d, sides, (int)q_blocks);
+  cudaError_t e = launch_pdl(k_rotate_vectors_backward<T, VEC, G, ADJACENT, kUnroll>,
                              dim3((unsigned)(q_blocks + k_blocks)), dim3(256), 0, stream, d, sides,
                              (int)q_blocks);
   return e == cudaSuccess && d.workspace ? enqueue_weights(d, q_blocks, q_blocks + k_blocks, stream) : e;
@@ -617,9 +672,9 @@ cudaError_t enqueue(tb_rotate_desc d, bool backward, cudaStream_t stream) {
   if (vectors_fit<T, kVec>(d, sides, backward)) return enqueue_vectors<T, kVec>(d, sides, backward, stream);
   if constexpr (kVec == 8)
     if (vectors_fit<T, 4>(d, sides, backward)) return enqueue_vectors<T, 4>(d, sides, backward, stream);
+  if (vectors_fit<T, 1>(d, sides, backward)) return enqueue_vectors<T, 1>(d, sides, backward, stream);
   if (!backward) {
     const int64_t blocks = (rows + 7) / 8;
-    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
     return launch_pdl(k_rotate<T>, dim3((unsigned)blocks), dim3(256), 0, stream, d, rows);
   }
   const cudaError_t e = launch_pdl(k_rotate_backward<T>, dim3(kBackwardBlocks), dim3(256),

@@ -34,34 +34,12 @@ __device__ __forceinline__ Vec<V> splat(float v) {
   for (int i = 0; i < V; ++i) r.set(i, v);
   return r;
 }
-__device__ __forceinline__ unsigned long long packed(Vec<2> v) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x.x), "f"(v.x.y));
-  return r;
-}
-__device__ __forceinline__ Vec<2> unpacked(unsigned long long r) {
-  Vec<2> v;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x.x), "=f"(v.x.y) : "l"(r));
-  return v;
-}
 __device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.x * b.x}; }
 __device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.x + b.x}; }
 __device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.x, b.x, c.x)}; }
-__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
-  return unpacked(r);
-}
-__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)));
-  return unpacked(r);
-}
-__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)), "l"(packed(c)));
-  return unpacked(r);
-}
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) { return {mul2(a.x, b.x)}; }
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) { return {add2(a.x, b.x)}; }
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) { return {fma2(a.x, b.x, c.x)}; }
 template <int V>
 __device__ __forceinline__ Vec<V> select(bool p, Vec<V> a, Vec<V> b) {
   Vec<V> r;
@@ -98,14 +76,8 @@ struct Raw<bf16, 1> {
 template <>
 struct Raw<bf16, 2> {
   typedef unsigned type;
-  static __device__ __forceinline__ Vec<2> read(unsigned r) {
-    return {{__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u)}};
-  }
-  static __device__ __forceinline__ unsigned made(Vec<2> v) {
-    unsigned r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.x.y), "f"(v.x.x));
-    return r;
-  }
+  static __device__ __forceinline__ Vec<2> read(unsigned r) { return {unpack_bf16(r)}; }
+  static __device__ __forceinline__ unsigned made(Vec<2> v) { return pack_bf16(v.x); }
 };
 
 // The bare instructions: the intrinsics around them also serve denormals, which do not matter here
