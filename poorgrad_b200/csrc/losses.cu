@@ -5,71 +5,250 @@
 // alone: dz_v = c scale (1[v = t] - p_v) with c = d loss / d L of the row.  Maxima are taken of
 // the raw logits and scale multiplies differences from them, so masks of the type's lowest
 // value do not overflow.
+#include <cooperative_groups.h>
+
 #include "operators.h"
 
 namespace tb {
 namespace {
 
-constexpr int kThreads = 512;
+namespace cg = cooperative_groups;
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// max z, and the sum of exp(scale (z - top)); k = scale log2(e).  A sum of 0: no logit above -inf.
 struct RowStats {
-  float top, sum;  // max z, sum exp(scale (z - top)); sum = 0 where no logit is above -inf
+  float top, sum;
 };
-// Differences from the top are never taken from -inf, and exp(0) = 1 exactly; a NaN or +inf
-// logit makes the sum NaN (fmaxf passes a NaN over, the exponential does not).
-__device__ __forceinline__ RowStats merge(RowStats p, RowStats q, float scale) {
-  const float top = fmaxf(p.top, q.top);
-  if (top == -INFINITY) return {top, p.sum + q.sum};
-  return {top, p.sum * __expf(scale * (p.top - top)) + q.sum * __expf(scale * (q.top - top))};
-}
-__device__ __forceinline__ RowStats add(RowStats s, float z, float scale) {
-  const float top = fmaxf(s.top, z);
-  if (top == -INFINITY) return {top, z != z ? z : s.sum};
-  return {top, s.sum * __expf(scale * (s.top - top)) + __expf(scale * (z - top))};
+// What differences are taken from: -inf would make NaN of -inf logits, and any finite number does.
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }
+// A NaN logit makes the sum NaN (the maximum passes it over, the exponential does not), and so does
+// +inf, by inf - inf.
+__device__ __forceinline__ RowStats merge(RowStats p, RowStats q, float k) {
+  const float top = fmaxf(p.top, q.top), base = base_of(top);
+  return {top, p.sum * ex2(k * (p.top - base)) + q.sum * ex2(k * (q.top - base))};
 }
 
-// Block-wide statistics of a row; every thread gets them.
+// 16 bytes of a row.
 template <typename T>
-__device__ RowStats row_stats(const T* z, int64_t vocab, float scale) {
-  __shared__ RowStats part[kThreads / 32];
-  RowStats s{-INFINITY, 0.0f};
-  for (int64_t v = threadIdx.x; v < vocab; v += kThreads) s = add(s, to_f32(z[v]), scale);
+struct Vector;
+template <>
+struct Vector<float> {
+  static constexpr int kPairs = 2;
+  static __device__ __forceinline__ void read(uint4 r, float2 (&v)[2]) {
+    v[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
+    v[1] = {__uint_as_float(r.z), __uint_as_float(r.w)};
+  }
+  static __device__ __forceinline__ uint4 made(const float2 (&v)[2]) {
+    return {__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+            __float_as_uint(v[1].y)};
+  }
+};
+template <>
+struct Vector<bf16> {
+  static constexpr int kPairs = 4;
+  static __device__ __forceinline__ void read(uint4 r, float2 (&v)[4]) {
+    v[0] = unpack_bf16(r.x);
+    v[1] = unpack_bf16(r.y);
+    v[2] = unpack_bf16(r.z);
+    v[3] = unpack_bf16(r.w);
+  }
+  static __device__ __forceinline__ uint4 made(const float2 (&v)[4]) {
+    return {pack_bf16(v[0]), pack_bf16(v[1]), pack_bf16(v[2]), pack_bf16(v[3])};
+  }
+};
+
+// Adds N pairs to a thread's statistics: one rescaling for all of them.
+template <int N>
+__device__ __forceinline__ void add(RowStats& s, const float2 (&v)[N], float k) {
+  float top = fmaxf(v[0].x, v[0].y);
+#pragma unroll
+  for (int j = 1; j < N; ++j) top = fmaxf(top, fmaxf(v[j].x, v[j].y));
+  if (top > s.top) {
+    s.sum *= ex2(k * (s.top - top));
+    s.top = top;
+  }
+  const float2 minus = both(-base_of(s.top));
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float2 x = mul2(add2(v[j], minus), both(k));
+    s.sum += ex2(x.x) + ex2(x.y);
+  }
+}
+__device__ __forceinline__ void add(RowStats& s, float z, float k) {
+  if (z > s.top) {
+    s.sum *= ex2(k * (s.top - z));
+    s.top = z;
+  }
+  s.sum += ex2(k * (z - base_of(s.top)));
+}
+
+// A row as single elements up to a 16-byte boundary, vectors, and single elements again; the
+// vectors and single elements of one block of `ranks` that share the row.
+template <typename T>
+struct RowShare {
+  static constexpr int kVec = 16 / sizeof(T);
+  int64_t first, count;  // this block's vectors, counted from the boundary
+  int64_t head;          // elements before the boundary
+  int64_t single;        // this thread's single element, or -1
+  __device__ RowShare(const T* z, int64_t vocab, int rank, int ranks, int64_t per) {
+    head = min((int64_t)((16 - ((uintptr_t)z & 15)) & 15) / (int64_t)sizeof(T), vocab);
+    const int64_t vectors = (vocab - head) / kVec, tail = head + vectors * kVec;
+    first = min(rank * per, vectors);
+    count = min(per, vectors - first);
+    // threads 0 .. 7 of the first block take the head's elements, 8 .. 15 of the last the tail's
+    single = -1;
+    if (rank == 0 && threadIdx.x < 8 && threadIdx.x < head) single = threadIdx.x;
+    if (rank == ranks - 1 && threadIdx.x >= 8 && threadIdx.x < 16 && tail + threadIdx.x - 8 < vocab)
+      single = tail + threadIdx.x - 8;
+  }
+  __device__ __forceinline__ int64_t element(int64_t vector) const { return head + (first + vector) * kVec; }
+};
+
+// The statistics of all threads, in a fixed order; every thread gets them.
+template <int THREADS>
+__device__ __forceinline__ RowStats block_stats(RowStats s, float k) {
+  __shared__ RowStats part[THREADS / 32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, scale);
-  __syncthreads();
+    s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, k);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
   __syncthreads();
-  s = part[0];
-  for (int w = 1; w < kThreads / 32; ++w) s = merge(s, part[w], scale);
+  s = part[threadIdx.x % (THREADS / 32)];
+#pragma unroll
+  for (int o = THREADS / 64; o > 0; o >>= 1)
+    s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, k);
   return s;
 }
 
-// Writes c scale (1[v = t] - p_v) over a row; zeros for c = 0 rows marked hidden.
-template <typename T>
-__device__ void row_gradient(const T* z, T* out, int64_t vocab, float scale, RowStats s, int64_t t,
-                             float c, bool hidden) {
-  const float step = c * scale, share = step / s.sum;
-  for (int64_t v = threadIdx.x; v < vocab; v += kThreads) {
-    float d = 0.0f;
-    if (!hidden) d = (v == t ? step : 0.0f) - share * __expf(scale * (to_f32(z[v]) - s.top));
-    out[v] = from_f32<T>(d);
+// Statistics of a row straight from memory.
+template <typename T, int THREADS>
+__device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k) {
+  typedef Vector<T> Vec;
+  constexpr int N = Vec::kPairs, kAtOnce = 4;
+  const RowShare<T> row(z, vocab, 0, 1, INT64_MAX / 2);
+  const uint4* from = (const uint4*)(z + row.head);
+  RowStats s{-INFINITY, 0.0f};
+  if (row.single >= 0) add(s, to_f32(z[row.single]), k);
+  int64_t i = threadIdx.x;
+  for (; i + (kAtOnce - 1) * THREADS < row.count; i += kAtOnce * THREADS) {
+    uint4 r[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) r[j] = from[i + j * THREADS];
+    float2 v[kAtOnce * N];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) Vec::read(r[j], *(float2(*)[N])&v[j * N]);
+    add(s, v, k);
   }
+  for (; i < row.count; i += THREADS) {
+    float2 v[N];
+    Vec::read(from[i], v);
+    add(s, v, k);
+  }
+  return block_stats<THREADS>(s, k);
+}
+
+// c scale (1[v = t] - p_v) of one vector, whose first element is `at`.
+template <int N>
+__device__ __forceinline__ void differentiate(float2 (&v)[N], RowStats s, float k, float share, float step,
+                                              int64_t target, int64_t at) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float2 x = mul2(add2(v[j], both(-s.top)), both(k));
+    v[j] = mul2({ex2(x.x), ex2(x.y)}, both(-share));
+  }
+  if (target >= at && target < at + 2 * N) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (target == at + 2 * j) v[j].x += step;
+      if (target == at + 2 * j + 1) v[j].y += step;
+    }
+  }
+}
+
+// A row's gradient: where it goes, and what it is made of.  Rows of zeros have step = share = 0 and
+// read nothing.
+template <typename T>
+struct RowGradient {
+  typedef Vector<T> Vec;
+  T* out;
+  RowStats s;
+  float k, step, share;
+  int64_t target;
+  bool whole;  // the output's rows start where the input's do, counted in 16 bytes
+
+  __device__ RowGradient(T* out, const T* z, RowStats s, float scale, float slope, int64_t target)
+      : out(out), s(s), k(scale * kLog2e), step(slope * scale), share(slope * scale / s.sum),
+        target(target), whole((((uintptr_t)out ^ (uintptr_t)z) & 15) == 0) {}
+
+  __device__ __forceinline__ void single(float z, int64_t at) const {
+    out[at] = from_f32<T>((at == target ? step : 0.0f) - share * ex2(k * (z - s.top)));
+  }
+  __device__ __forceinline__ void vector(uint4 r, int64_t at) const {
+    float2 v[Vec::kPairs];
+    Vec::read(r, v);
+    differentiate(v, s, k, share, step, target, at);
+    store(v, at);
+  }
+  __device__ __forceinline__ void zeros(int64_t at) const {
+    float2 v[Vec::kPairs] = {};
+    store(v, at);
+  }
+  __device__ __forceinline__ void store(const float2 (&v)[Vec::kPairs], int64_t at) const {
+    if (whole) {
+      *(uint4*)(out + at) = Vec::made(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < Vec::kPairs; ++j) {
+        out[at + 2 * j] = from_f32<T>(v[j].x);
+        out[at + 2 * j + 1] = from_f32<T>(v[j].y);
+      }
+    }
+  }
+};
+template <typename T, int THREADS>
+__device__ __forceinline__ void zero_row(T* out, const T* z, const RowShare<T>& row) {
+  const RowGradient<T> g(out, z, {0.0f, 1.0f}, 1.0f, 0.0f, -1);
+  if (row.single >= 0) out[row.single] = from_f32<T>(0.0f);
+  for (int64_t i = threadIdx.x; i < row.count; i += THREADS) g.zeros(row.element(i));
+}
+// The gradient of a row straight from memory.
+template <typename T, int THREADS>
+__device__ __forceinline__ void stream_gradient(const T* z, const RowShare<T>& row, const RowGradient<T>& g) {
+  constexpr int kAtOnce = 4;
+  const uint4* from = (const uint4*)(z + row.element(0));
+  if (row.single >= 0) g.single(to_f32(z[row.single]), row.single);
+  int64_t i = threadIdx.x;
+  for (; i + (kAtOnce - 1) * THREADS < row.count; i += kAtOnce * THREADS) {
+    uint4 r[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) r[j] = from[i + j * THREADS];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) g.vector(r[j], row.element(i + j * THREADS));
+  }
+  for (; i < row.count; i += THREADS) g.vector(from[i], row.element(i));
 }
 
 __device__ __forceinline__ float logp_of(float z, RowStats s, float scale) {
   return scale * (z - s.top) - logf(s.sum);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_token_logp(const T* logits, int64_t stride, const int32_t* targets,
-                                                         int64_t vocab, float scale, float* logp) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_token_logp(const T* logits, int64_t stride,
+                                                        const int32_t* targets, int64_t vocab,
+                                                        float scale, float* logp) {
   pdl_entry();
   const int64_t n = blockIdx.x, t = targets[n];
   float out = 0.0f;
   if (t >= 0) {
     const T* z = logits + n * stride;
-    const RowStats s = row_stats(z, vocab, scale);
+    const RowStats s = row_stats<T, THREADS>(z, vocab, scale * kLog2e);
     if (s.sum != 0.0f) out = t < vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) logp[n] = out;
@@ -79,36 +258,155 @@ __global__ void __launch_bounds__(kThreads) k_token_logp(const T* logits, int64_
 struct Term {
   float loss, slope;
 };
-__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, int64_t n, float logp, float w) {
-  const float a = d.advantages[n], r = expf(logp - d.old_logp[n]);
+struct TermInputs {
+  float advantage, old_logp, ref_logp, weight;
+  __device__ TermInputs(const tb_policy_desc& d, int64_t n)
+      : advantage(d.advantages[n]), old_logp(d.old_logp[n]), ref_logp(d.kl > 0 ? d.ref_logp[n] : 0.0f),
+        weight(d.weights[n]) {}
+};
+__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, const TermInputs& in, float logp) {
+  const float a = in.advantage, r = expf(logp - in.old_logp);
   const float held = fminf(fmaxf(r, 1.0f - (float)d.clip_low), 1.0f + (float)d.clip_high);
   const float plain = r * a, kept = (r != r ? r : held) * a;
   float loss = -(plain <= kept ? plain : kept), slope = plain <= kept ? -plain : 0.0f;
   if (plain != plain) loss = slope = plain;
   if (d.kl > 0) {
-    const float x = d.ref_logp[n] - logp, e = expm1f(x);
+    const float x = in.ref_logp - logp, e = expm1f(x);
     loss += (float)d.kl * (e - x);
     slope -= (float)d.kl * e;
   }
-  return {w * loss, w * slope};
+  return {in.weight * loss, in.weight * slope};
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_policy(tb_policy_desc d) {
+// The loss alone, a block a row.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x, t = d.targets[n];
-  const float w = d.weights[n], scale = (float)d.scale;
-  const T* z = (const T*)d.logits + n * d.logits_stride;
-  bool hidden = t < 0 || w == 0.0f;
-  RowStats s{0.0f, 1.0f};
+  const float scale = (float)d.scale;
   float logp = 0.0f;
   Term term{0.0f, 0.0f};
-  if (!hidden) {
-    s = row_stats(z, d.vocab, scale);
-    hidden = s.sum == 0.0f;
-    if (!hidden) {
+  const TermInputs in(d, n);
+  if (t >= 0 && in.weight != 0.0f) {
+    const T* z = (const T*)d.logits + n * d.logits_stride;
+    const RowStats s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
+    if (s.sum != 0.0f) {
       logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
-      term = policy_term(d, n, logp, w);
+      term = policy_term(d, in, logp);
+    }
+  }
+  if (threadIdx.x == 0) {
+    d.logp[n] = logp;
+    d.token_loss[n] = term.loss;
+  }
+}
+
+// The loss and its gradient in one reading of the logits: the blocks of a cluster share a row, each
+// keeps its part in shared memory until the row's statistics are known.  A thread copies and reads
+// its own vectors only, so that nothing but those statistics is waited for.  kKeep vectors a
+// thread let two blocks of 512 threads (four of 256, eight of 128) share a SM, one loading while
+// the other stores.
+constexpr int kKeep = 13, kGroups = 4;
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy(tb_policy_desc d, int ranks, int64_t per) {
+  pdl_entry();
+  typedef Vector<T> Vec;
+  extern __shared__ uint4 kept[];
+  __shared__ RowStats parts[8];
+  const int64_t n = blockIdx.x / ranks;
+  const int rank = blockIdx.x % ranks, keep = (int)((per + THREADS - 1) / THREADS);
+  const int64_t t = d.targets[n];
+  const TermInputs in(d, n);
+  const float scale = (float)d.scale, k = scale * kLog2e;
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  const RowShare<T> row(z, d.vocab, rank, ranks, per);
+  if (t < 0 || in.weight == 0.0f) {  // the same for all blocks of the cluster
+    zero_row<T, THREADS>(out, z, row);
+    if (rank == 0 && threadIdx.x == 0) d.logp[n] = d.token_loss[n] = 0.0f;
+    return;
+  }
+  const uint4* from = (const uint4*)(z + row.element(0));
+  const int each = (keep + kGroups - 1) / kGroups;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
+      const int64_t i = (int64_t)j * THREADS + threadIdx.x;
+      if (i < row.count)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         (unsigned)__cvta_generic_to_shared(kept + i)),
+                     "l"(from + i)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
+  const float single = row.single >= 0 ? to_f32(z[row.single]) : 0.0f;
+  RowStats s{-INFINITY, 0.0f};
+  if (row.single >= 0) add(s, single, k);
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    if (g == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    if (g == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    if (g == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (g == 3) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
+      const int64_t i = (int64_t)j * THREADS + threadIdx.x;
+      if (i < row.count) {
+        float2 v[Vec::kPairs];
+        Vec::read(kept[i], v);
+        add(s, v, k);
+      }
+    }
+  }
+  s = block_stats<THREADS>(s, k);
+  if (ranks > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&parts[rank], threadIdx.x) = s;
+    cluster.sync();
+    s = parts[0];
+    for (int r = 1; r < ranks; ++r) s = merge(s, parts[r], k);
+  }
+  float logp = 0.0f;
+  Term term{0.0f, 0.0f};
+  const bool hidden = s.sum == 0.0f;
+  if (!hidden) {
+    logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
+    term = policy_term(d, in, logp);
+  }
+  if (rank == 0 && threadIdx.x == 0) {
+    d.logp[n] = logp;
+    d.token_loss[n] = term.loss;
+  }
+  if (hidden) {
+    zero_row<T, THREADS>(out, z, row);
+    return;
+  }
+  const RowGradient<T> g(out, z, s, scale, term.slope, t);
+  if (row.single >= 0) g.single(single, row.single);
+#pragma unroll 2
+  for (int64_t i = threadIdx.x; i < row.count; i += THREADS) g.vector(kept[i], row.element(i));
+}
+
+// The same for rows that no cluster can keep: read twice.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_policy_twice(tb_policy_desc d) {
+  pdl_entry();
+  const int64_t n = blockIdx.x, t = d.targets[n];
+  const TermInputs in(d, n);
+  const float scale = (float)d.scale;
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
+  RowStats s{0.0f, 0.0f};
+  float logp = 0.0f;
+  Term term{0.0f, 0.0f};
+  if (t >= 0 && in.weight != 0.0f) {
+    s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
+    if (s.sum != 0.0f) {
+      logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+      term = policy_term(d, in, logp);
     }
   }
   __syncthreads();  // the gradient may overwrite the logits that others still read
@@ -116,8 +414,92 @@ __global__ void __launch_bounds__(kThreads) k_policy(tb_policy_desc d) {
     d.logp[n] = logp;
     d.token_loss[n] = term.loss;
   }
-  if (d.gradient)
-    row_gradient(z, (T*)d.gradient + n * d.gradient_stride, d.vocab, scale, s, t, term.slope, hidden);
+  if (s.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
+  else stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, scale, term.slope, t));
+}
+
+// ---- small vocabularies: a warp a row, ITEMS logits a lane in registers
+template <typename T, int ITEMS>
+struct WarpRow {
+  float v[ITEMS];
+  RowStats s;
+  __device__ WarpRow(const T* z, int vocab, float k) {
+    const int lane = threadIdx.x % 32;
+    s = {-INFINITY, 0.0f};
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) v[j] = lane + 32 * j < vocab ? to_f32(z[lane + 32 * j]) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) s.top = fmaxf(s.top, v[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.top = fmaxf(s.top, __shfl_xor_sync(~0u, s.top, o));
+    const float base = base_of(s.top);
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      v[j] = ex2(k * (v[j] - base));
+      s.sum += v[j];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.sum += __shfl_xor_sync(~0u, s.sum, o);
+  }
+  __device__ void gradient(T* out, int vocab, float scale, float slope, int64_t target) const {
+    const int lane = threadIdx.x % 32;
+    const float step = slope * scale, share = s.sum == 0.0f ? 0.0f : step / s.sum;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (lane + 32 * j < vocab)
+        out[lane + 32 * j] = from_f32<T>(s.sum == 0.0f ? 0.0f : (lane + 32 * j == target ? step : 0.0f) - share * v[j]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ void zero_warp_row(T* out, int64_t vocab) {
+  for (int v = threadIdx.x % 32; v < vocab; v += 32) out[v] = from_f32<T>(0.0f);
+}
+
+template <typename T, int ITEMS>
+__global__ void __launch_bounds__(256) k_policy_warps(tb_policy_desc d) {
+  pdl_entry();
+  const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (n >= d.rows) return;
+  const int64_t t = d.targets[n];
+  const TermInputs in(d, n);
+  const float scale = (float)d.scale;
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  float logp = 0.0f;
+  Term term{0.0f, 0.0f};
+  if (t >= 0 && in.weight != 0.0f) {
+    const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
+    const WarpRow<T, ITEMS> row(z, (int)d.vocab, scale * kLog2e);
+    if (row.s.sum != 0.0f) {
+      logp = t < d.vocab ? logp_of(zt, row.s, scale) : NAN;
+      term = policy_term(d, in, logp);
+    }
+    __syncwarp();  // the gradient may overwrite the logits that others still read
+    if (d.gradient) row.gradient(out, (int)d.vocab, scale, term.slope, t);
+  } else if (d.gradient) {
+    zero_warp_row(out, d.vocab);
+  }
+  if (threadIdx.x % 32 == 0) {
+    d.logp[n] = logp;
+    d.token_loss[n] = term.loss;
+  }
+}
+
+template <typename T, int ITEMS>
+__global__ void __launch_bounds__(256) k_token_logp_warps(const T* logits, int64_t stride, const int32_t* targets,
+                                                          int64_t rows, int64_t vocab, float scale, float* logp) {
+  pdl_entry();
+  const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (n >= rows) return;
+  const int64_t t = targets[n];
+  float out = 0.0f;
+  if (t >= 0) {
+    const T* z = logits + n * stride;
+    const float zt = t < vocab ? to_f32(z[t]) : 0.0f;
+    const WarpRow<T, ITEMS> row(z, (int)vocab, scale * kLog2e);
+    if (row.s.sum != 0.0f) out = t < vocab ? logp_of(zt, row.s, scale) : NAN;
+  }
+  if (threadIdx.x % 32 == 0) logp[n] = out;
 }
 
 // loss[0] = the sum of the terms, in a fixed order and f64.
@@ -141,8 +523,8 @@ __device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t rows) {
   return v < 0 ? 0 : v > rows ? rows : v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_preference_rows(tb_preference_desc d) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x;
   if (n < d.offsets[0] || n >= d.offsets[2 * d.pairs]) return;
@@ -152,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) k_preference_rows(tb_preference_desc
   float logp = 0.0f;
   if (t >= 0) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
-    s = row_stats(z, d.vocab, scale);
+    s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
     if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) {
@@ -202,16 +584,20 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(tb_preference_desc d)
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_preference_gradient(tb_preference_desc d) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_preference_gradient(tb_preference_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x;
   if (n < d.offsets[0] || n >= d.offsets[2 * d.pairs]) return;
   const RowStats s = ((const RowStats*)d.workspace)[n];
   const float slope = ((const float*)((const RowStats*)d.workspace + d.rows))[n];
   const int64_t t = d.targets[n];
-  row_gradient((const T*)d.logits + n * d.logits_stride, (T*)d.gradient + n * d.gradient_stride,
-               d.vocab, (float)d.scale, s, t, t < d.vocab ? slope : NAN, s.sum == 0.0f);
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
+  if (s.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
+  else
+    stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, (float)d.scale, t < d.vocab ? slope : NAN, t));
 }
 
 const char* check_logits(int64_t element, int64_t rows, int64_t vocab, int64_t stride, double scale,
@@ -241,6 +627,84 @@ bool words_ok(std::initializer_list<const void*> arrays) {
   return true;
 }
 
+// Threads of a block that streams a row: some 8 vectors a thread.
+template <typename T>
+int threads_of(int64_t vocab) {
+  const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
+  return vectors > 4096 ? 512 : vectors > 1024 ? 256 : 128;
+}
+#define TB_BY_THREADS(KERNEL, ...)                                                                 \
+  switch (threads_of<T>(vocab)) {                                                                  \
+    case 512: return launch_pdl(KERNEL<T, 512>, dim3((unsigned)rows), dim3(512), 0, stream, __VA_ARGS__); \
+    case 256: return launch_pdl(KERNEL<T, 256>, dim3((unsigned)rows), dim3(256), 0, stream, __VA_ARGS__); \
+    default: return launch_pdl(KERNEL<T, 128>, dim3((unsigned)rows), dim3(128), 0, stream, __VA_ARGS__);  \
+  }
+// Rows that fit a warp's registers.
+constexpr int64_t kWarpVocab = 1024;
+#define TB_BY_ITEMS(KERNEL, ...)                                                                   \
+  {                                                                                                \
+    const dim3 grid((unsigned)((rows + 7) / 8)), block(256);                                       \
+    if (vocab <= 32) return launch_pdl(KERNEL<T, 1>, grid, block, 0, stream, __VA_ARGS__);         \
+    if (vocab <= 128) return launch_pdl(KERNEL<T, 4>, grid, block, 0, stream, __VA_ARGS__);        \
+    if (vocab <= 512) return launch_pdl(KERNEL<T, 16>, grid, block, 0, stream, __VA_ARGS__);       \
+    return launch_pdl(KERNEL<T, 32>, grid, block, 0, stream, __VA_ARGS__);                         \
+  }
+
+template <typename T>
+cudaError_t enqueue_logp(const T* logits, int64_t stride, const int32_t* targets, int64_t rows, int64_t vocab,
+                         float scale, float* logp, cudaStream_t stream) {
+  if (vocab <= kWarpVocab)
+    TB_BY_ITEMS(k_token_logp_warps, logits, stride, targets, rows, vocab, scale, logp)
+  TB_BY_THREADS(k_token_logp, logits, stride, targets, vocab, scale, logp)
+}
+
+template <typename T, int THREADS>
+cudaError_t enqueue_kept(const tb_policy_desc& d, int ranks, int64_t per, cudaStream_t stream) {
+  const size_t bytes = (size_t)per * 16;
+  const auto kernel = k_policy<T, THREADS>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use the most it needs
+  if (const cudaError_t e = allow_shared((const void*)kernel, (size_t)kKeep * THREADS * 16, allowed)) return e;
+  if (d.rows * ranks > INT32_MAX) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(d.rows * ranks));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, d, ranks, per);
+}
+template <typename T>
+cudaError_t enqueue_policy(const tb_policy_desc& d, cudaStream_t stream) {
+  const int64_t rows = d.rows, vocab = d.vocab;
+  if (vocab <= kWarpVocab) TB_BY_ITEMS(k_policy_warps, d)
+  if (!d.gradient) TB_BY_THREADS(k_policy_terms, d)
+  const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
+  if (vectors <= kKeep * 128) return enqueue_kept<T, 128>(d, 1, vectors, stream);
+  if (vectors <= kKeep * 256) return enqueue_kept<T, 256>(d, 1, vectors, stream);
+  for (int ranks = 1; ranks <= 8; ranks *= 2) {
+    const int64_t per = (vectors + ranks - 1) / ranks;
+    if (per <= kKeep * 512) return enqueue_kept<T, 512>(d, ranks, per, stream);
+  }
+  return launch_pdl(k_policy_twice<T, 512>, dim3((unsigned)rows), dim3(512), 0, stream, d);
+}
+template <typename T>
+cudaError_t enqueue_preference_rows(const tb_preference_desc& d, cudaStream_t stream) {
+  const int64_t rows = d.rows, vocab = d.vocab;
+  TB_BY_THREADS(k_preference_rows, d)
+}
+template <typename T>
+cudaError_t enqueue_preference_gradient(const tb_preference_desc& d, cudaStream_t stream) {
+  const int64_t rows = d.rows, vocab = d.vocab;
+  TB_BY_THREADS(k_preference_gradient, d)
+}
+
 int token_logp(int64_t element, const void* logits, int64_t stride, const int32_t* targets,
                int64_t rows, int64_t vocab, double scale, float* logp, void* stream) {
   OperatorCall call("tb_token_logp", stream);
@@ -249,13 +713,10 @@ int token_logp(int64_t element, const void* logits, int64_t stride, const int32_
   if (rows > 0 && !words_ok({targets, logp})) return call.invalid("a row array is NULL or unaligned");
   if (const int code = call.ready()) return code;
   if (rows == 0) return TB_OK;
-  const dim3 grid((unsigned)rows), block(kThreads);
   return call.finish(
       element == TB_ELEMENT_F32
-          ? launch_pdl(k_token_logp<float>, grid, block, 0, call.stream(), (const float*)logits,
-                       stride, targets, vocab, (float)scale, logp)
-          : launch_pdl(k_token_logp<bf16>, grid, block, 0, call.stream(), (const bf16*)logits,
-                       stride, targets, vocab, (float)scale, logp));
+          ? enqueue_logp((const float*)logits, stride, targets, rows, vocab, (float)scale, logp, call.stream())
+          : enqueue_logp((const bf16*)logits, stride, targets, rows, vocab, (float)scale, logp, call.stream()));
 }
 
 int policy_loss(const tb_policy_desc* desc, void* stream) {
@@ -275,8 +736,7 @@ int policy_loss(const tb_policy_desc* desc, void* stream) {
   if (const int code = call.ready()) return code;
   cudaError_t e = cudaSuccess;
   if (d.rows > 0)
-    e = launch_pdl(d.element == TB_ELEMENT_F32 ? k_policy<float> : k_policy<bf16>,
-                   dim3((unsigned)d.rows), dim3(kThreads), 0, call.stream(), d);
+    e = d.element == TB_ELEMENT_F32 ? enqueue_policy<float>(d, call.stream()) : enqueue_policy<bf16>(d, call.stream());
   if (e == cudaSuccess)
     e = launch_pdl(k_sum_terms, dim3(1), dim3(1024), 0, call.stream(), (const float*)d.token_loss,
                    d.rows, d.loss);
@@ -304,15 +764,13 @@ int preference_loss(const tb_preference_desc* desc, void* stream) {
   }
   if (const int code = call.ready()) return code;
   const bool f32 = d.element == TB_ELEMENT_F32;
-  const dim3 grid((unsigned)d.rows), block(kThreads);
   cudaError_t e = cudaSuccess;
   if (d.rows > 0)
-    e = launch_pdl(f32 ? k_preference_rows<float> : k_preference_rows<bf16>, grid, block, 0,
-                   call.stream(), d);
+    e = f32 ? enqueue_preference_rows<float>(d, call.stream()) : enqueue_preference_rows<bf16>(d, call.stream());
   if (e == cudaSuccess) e = launch_pdl(k_preference_pairs, dim3(1), dim3(1024), 0, call.stream(), d);
   if (e == cudaSuccess && d.rows > 0 && d.gradient)
-    e = launch_pdl(f32 ? k_preference_gradient<float> : k_preference_gradient<bf16>, grid, block, 0,
-                   call.stream(), d);
+    e = f32 ? enqueue_preference_gradient<float>(d, call.stream())
+            : enqueue_preference_gradient<bf16>(d, call.stream());
   return call.finish(e);
 }
 

@@ -131,6 +131,19 @@ inline int guarded(F body) noexcept {
   }
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; `allowed` remembers the
+// devices where it already may.  48 KB may always be used, 16 KB of it static.
+inline cudaError_t allow_shared(const void* kernel, size_t bytes, std::atomic<uint64_t>& allowed) {
+  if (bytes <= 32 * 1024) return cudaSuccess;
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device)) return e;
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (device < 64 && (allowed.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && device < 64) allowed.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 inline bool aligned_to(const void* p, int64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 // Extents a request may have: each, and their product, far below what 64-bit sizes hold.
 inline bool extents_fit(std::initializer_list<int64_t> extents) {
