@@ -452,8 +452,8 @@ typedef struct tb_preference_desc {
  * loss = sum_i weight_i (-(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)).
  * `gradient` may be `logits` with its stride. */
 int tb_preference_loss(const tb_preference_desc* desc, void* stream);
-/* Bytes of 16-byte aligned workspace for a preference loss over `rows`. */
-int64_t tb_preference_workspace(int64_t rows);
+/* Bytes of 16-byte aligned workspace for a preference loss. */
+int64_t tb_preference_workspace(int64_t rows, int64_t pairs);
 
 #ifdef __cplusplus
 }

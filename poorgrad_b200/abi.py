@@ -285,7 +285,7 @@ def load_library() -> C.CDLL:
                                     P, P]),
         "tb_policy_loss": (C.c_int, [C.c_char_p, P]),
         "tb_preference_loss": (C.c_int, [C.c_char_p, P]),
-        "tb_preference_workspace": (C.c_int64, [C.c_int64]),
+        "tb_preference_workspace": (C.c_int64, [C.c_int64] * 2),
     }
     for name, (restype, argtypes) in sigs.items():
         fn = getattr(lib, name)

@@ -7,6 +7,8 @@
 // value do not overflow.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "operators.h"
 
 namespace tb {
@@ -45,6 +47,10 @@ struct Vector<float> {
     v[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
     v[1] = {__uint_as_float(r.z), __uint_as_float(r.w)};
   }
+  static __device__ __forceinline__ float top(uint4 r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                 fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
   static __device__ __forceinline__ uint4 made(const float2 (&v)[2]) {
     return {__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
             __float_as_uint(v[1].y)};
@@ -59,27 +65,44 @@ struct Vector<bf16> {
     v[2] = unpack_bf16(r.z);
     v[3] = unpack_bf16(r.w);
   }
+  static __device__ __forceinline__ unsigned top(unsigned a, unsigned b) {  // of each half; NaN last
+    unsigned r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(uint4 r) {
+    const float2 t = unpack_bf16(top(top(r.x, r.y), top(r.z, r.w)));
+    return fmaxf(t.x, t.y);
+  }
   static __device__ __forceinline__ uint4 made(const float2 (&v)[4]) {
     return {pack_bf16(v[0]), pack_bf16(v[1]), pack_bf16(v[2]), pack_bf16(v[3])};
   }
 };
 
-// Adds N pairs to a thread's statistics: one rescaling for all of them.
-template <int N>
-__device__ __forceinline__ void add(RowStats& s, const float2 (&v)[N], float k) {
-  float top = fmaxf(v[0].x, v[0].y);
+// Adds COUNT vectors to a thread's statistics: one rescaling for all of them.
+template <typename T, int COUNT>
+__device__ __forceinline__ void add(RowStats& s, const uint4 (&r)[COUNT], float k) {
+  typedef Vector<T> Vec;
+  float top = Vec::top(r[0]);
 #pragma unroll
-  for (int j = 1; j < N; ++j) top = fmaxf(top, fmaxf(v[j].x, v[j].y));
+  for (int j = 1; j < COUNT; ++j) top = fmaxf(top, Vec::top(r[j]));
   if (top > s.top) {
     s.sum *= ex2(k * (s.top - top));
     s.top = top;
   }
   const float2 minus = both(-base_of(s.top));
+  float2 sum = both(0.0f);
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float2 x = mul2(add2(v[j], minus), both(k));
-    s.sum += ex2(x.x) + ex2(x.y);
+  for (int j = 0; j < COUNT; ++j) {
+    float2 v[Vec::kPairs];
+    Vec::read(r[j], v);
+#pragma unroll
+    for (int i = 0; i < Vec::kPairs; ++i) {
+      const float2 x = mul2(add2(v[i], minus), both(k));
+      sum = add2(sum, {ex2(x.x), ex2(x.y)});
+    }
   }
+  s.sum += sum.x + sum.y;
 }
 __device__ __forceinline__ void add(RowStats& s, float z, float k) {
   if (z > s.top) {
@@ -130,8 +153,7 @@ __device__ __forceinline__ RowStats block_stats(RowStats s, float k) {
 // Statistics of a row straight from memory.
 template <typename T, int THREADS>
 __device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k) {
-  typedef Vector<T> Vec;
-  constexpr int N = Vec::kPairs, kAtOnce = 4;
+  constexpr int kAtOnce = 4;
   const RowShare<T> row(z, vocab, 0, 1, INT64_MAX / 2);
   const uint4* from = (const uint4*)(z + row.head);
   RowStats s{-INFINITY, 0.0f};
@@ -141,39 +163,16 @@ __device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k
     uint4 r[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) r[j] = from[i + j * THREADS];
-    float2 v[kAtOnce * N];
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) Vec::read(r[j], *(float2(*)[N])&v[j * N]);
-    add(s, v, k);
+    add<T>(s, r, k);
   }
   for (; i < row.count; i += THREADS) {
-    float2 v[N];
-    Vec::read(from[i], v);
-    add(s, v, k);
+    const uint4 r[1] = {from[i]};
+    add<T>(s, r, k);
   }
   return block_stats<THREADS>(s, k);
 }
 
-// c scale (1[v = t] - p_v) of one vector, whose first element is `at`.
-template <int N>
-__device__ __forceinline__ void differentiate(float2 (&v)[N], RowStats s, float k, float share, float step,
-                                              int64_t target, int64_t at) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float2 x = mul2(add2(v[j], both(-s.top)), both(k));
-    v[j] = mul2({ex2(x.x), ex2(x.y)}, both(-share));
-  }
-  if (target >= at && target < at + 2 * N) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (target == at + 2 * j) v[j].x += step;
-      if (target == at + 2 * j + 1) v[j].y += step;
-    }
-  }
-}
-
-// A row's gradient: where it goes, and what it is made of.  Rows of zeros have step = share = 0 and
-// read nothing.
+// A row's gradient c scale (1[v = t] - p_v): where it goes, and what it is made of.
 template <typename T>
 struct RowGradient {
   typedef Vector<T> Vec;
@@ -190,49 +189,66 @@ struct RowGradient {
   __device__ __forceinline__ void single(float z, int64_t at) const {
     out[at] = from_f32<T>((at == target ? step : 0.0f) - share * ex2(k * (z - s.top)));
   }
-  __device__ __forceinline__ void vector(uint4 r, int64_t at) const {
+  __device__ __forceinline__ uint4 of(uint4 r) const {
     float2 v[Vec::kPairs];
     Vec::read(r, v);
-    differentiate(v, s, k, share, step, target, at);
-    store(v, at);
-  }
-  __device__ __forceinline__ void zeros(int64_t at) const {
-    float2 v[Vec::kPairs] = {};
-    store(v, at);
-  }
-  __device__ __forceinline__ void store(const float2 (&v)[Vec::kPairs], int64_t at) const {
-    if (whole) {
-      *(uint4*)(out + at) = Vec::made(v);
-    } else {
 #pragma unroll
-      for (int j = 0; j < Vec::kPairs; ++j) {
-        out[at + 2 * j] = from_f32<T>(v[j].x);
-        out[at + 2 * j + 1] = from_f32<T>(v[j].y);
-      }
+    for (int j = 0; j < Vec::kPairs; ++j) {
+      const float2 x = mul2(add2(v[j], both(-s.top)), both(k));
+      v[j] = mul2({ex2(x.x), ex2(x.y)}, both(-share));
     }
+    return Vec::made(v);
+  }
+  __device__ __forceinline__ void store(uint4 r, int64_t at) const {
+    if (whole) {
+      *(uint4*)(out + at) = r;
+      return;
+    }
+    const T* v = (const T*)&r;
+#pragma unroll
+    for (int j = 0; j < 2 * Vec::kPairs; ++j) out[at + j] = v[j];
+  }
+  // The target's element, for the thread that wrote its vector without the step: `vector` gives the
+  // vectors of the row's share by number.
+  template <int THREADS, typename F>
+  __device__ __forceinline__ void mend(const RowShare<T>& row, F vector) const {
+    const int64_t i = (target - row.element(0)) / (2 * Vec::kPairs);
+    if (target < row.element(0) || i >= row.count || i % THREADS != (int)threadIdx.x) return;
+    const uint4 r = vector(i);
+    single(to_f32(((const T*)&r)[(target - row.element(0)) % (2 * Vec::kPairs)]), target);
   }
 };
 template <typename T, int THREADS>
 __device__ __forceinline__ void zero_row(T* out, const T* z, const RowShare<T>& row) {
   const RowGradient<T> g(out, z, {0.0f, 1.0f}, 1.0f, 0.0f, -1);
   if (row.single >= 0) out[row.single] = from_f32<T>(0.0f);
-  for (int64_t i = threadIdx.x; i < row.count; i += THREADS) g.zeros(row.element(i));
+  for (int64_t i = threadIdx.x; i < row.count; i += THREADS) g.store(uint4{0, 0, 0, 0}, row.element(i));
 }
-// The gradient of a row straight from memory.
+// The gradient of a row straight from memory, which may be written over as it is read.
 template <typename T, int THREADS>
 __device__ __forceinline__ void stream_gradient(const T* z, const RowShare<T>& row, const RowGradient<T>& g) {
   constexpr int kAtOnce = 4;
   const uint4* from = (const uint4*)(z + row.element(0));
   if (row.single >= 0) g.single(to_f32(z[row.single]), row.single);
+  const int64_t mine = (g.target - row.element(0)) / RowShare<T>::kVec;  // the target's vector
+  uint4 found{};
   int64_t i = threadIdx.x;
   for (; i + (kAtOnce - 1) * THREADS < row.count; i += kAtOnce * THREADS) {
     uint4 r[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) r[j] = from[i + j * THREADS];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) g.vector(r[j], row.element(i + j * THREADS));
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (i + j * THREADS == mine) found = r[j];
+      g.store(g.of(r[j]), row.element(i + j * THREADS));
+    }
   }
-  for (; i < row.count; i += THREADS) g.vector(from[i], row.element(i));
+  for (; i < row.count; i += THREADS) {
+    const uint4 r = from[i];
+    if (i == mine) found = r;
+    g.store(g.of(r), row.element(i));
+  }
+  g.template mend<THREADS>(row, [&](int64_t) { return found; });
 }
 
 __device__ __forceinline__ float logp_of(float z, RowStats s, float scale) {
@@ -309,9 +325,8 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
 constexpr int kKeep = 13, kGroups = 4;
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy(tb_policy_desc d, int ranks, int64_t per) {
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_desc d, int ranks, int64_t per) {
   pdl_entry();
-  typedef Vector<T> Vec;
   extern __shared__ uint4 kept[];
   __shared__ RowStats parts[8];
   const int64_t n = blockIdx.x / ranks;
@@ -328,12 +343,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy(tb_policy_de
     return;
   }
   const uint4* from = (const uint4*)(z + row.element(0));
-  const int each = (keep + kGroups - 1) / kGroups;
+  const int each = (keep + kGroups - 1) / kGroups, count = (int)row.count;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
     for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
-      const int64_t i = (int64_t)j * THREADS + threadIdx.x;
-      if (i < row.count)
+      const int i = j * THREADS + threadIdx.x;
+      if (i < count)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                          (unsigned)__cvta_generic_to_shared(kept + i)),
                      "l"(from + i)
@@ -352,11 +367,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy(tb_policy_de
     if (g == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     if (g == 3) asm volatile("cp.async.wait_group 0;" ::: "memory");
     for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
-      const int64_t i = (int64_t)j * THREADS + threadIdx.x;
-      if (i < row.count) {
-        float2 v[Vec::kPairs];
-        Vec::read(kept[i], v);
-        add(s, v, k);
+      const int i = j * THREADS + threadIdx.x;
+      if (i < count) {
+        const uint4 r[1] = {kept[i]};
+        add<T>(s, r, k);
       }
     }
   }
@@ -385,8 +399,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy(tb_policy_de
   }
   const RowGradient<T> g(out, z, s, scale, term.slope, t);
   if (row.single >= 0) g.single(single, row.single);
+  if (g.whole) {
+    uint4* to = (uint4*)(out + row.element(0));
 #pragma unroll 2
-  for (int64_t i = threadIdx.x; i < row.count; i += THREADS) g.vector(kept[i], row.element(i));
+    for (int i = threadIdx.x; i < count; i += THREADS) to[i] = g.of(kept[i]);
+  } else {
+    for (int i = threadIdx.x; i < count; i += THREADS) g.store(g.of(kept[i]), row.element(i));
+  }
+  g.template mend<THREADS>(row, [&](int64_t i) { return kept[i]; });
 }
 
 // The same for rows that no cluster can keep: read twice.
@@ -518,16 +538,26 @@ __global__ void __launch_bounds__(1024) k_sum_terms(const float* terms, int64_t 
   }
 }
 
-// Workspace of the preference loss: RowStats[rows], then float slopes[rows].
+// Workspace of the preference loss.
+struct PreferenceScratch {
+  double* terms;    // [pairs], the weighted losses
+  RowStats* stats;  // [rows]
+  float* slopes;    // [rows], of the loss by the row's log probability
+  __host__ __device__ explicit PreferenceScratch(const tb_preference_desc& d)
+      : terms((double*)d.workspace), stats((RowStats*)(terms + d.pairs)), slopes((float*)(stats + d.rows)) {}
+};
 __device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t rows) {
   return v < 0 ? 0 : v > rows ? rows : v;
+}
+__device__ __forceinline__ bool scored(const tb_preference_desc& d, int64_t n) {
+  return n >= d.offsets[0] && n < d.offsets[2 * d.pairs];
 }
 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x;
-  if (n < d.offsets[0] || n >= d.offsets[2 * d.pairs]) return;
+  if (!scored(d, n)) return;
   const int64_t t = d.targets[n];
   const float scale = (float)d.scale;
   RowStats s{0.0f, 0.0f};
@@ -538,66 +568,125 @@ __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc 
     if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) {
-    ((RowStats*)d.workspace)[n] = s;
+    PreferenceScratch(d).stats[n] = s;
+    d.logp[n] = logp;
+  }
+}
+template <typename T, int ITEMS>
+__global__ void __launch_bounds__(256) k_preference_rows_warps(tb_preference_desc d) {
+  pdl_entry();
+  const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (n >= d.rows || !scored(d, n)) return;
+  const int64_t t = d.targets[n];
+  const float scale = (float)d.scale;
+  RowStats s{0.0f, 0.0f};
+  float logp = 0.0f;
+  if (t >= 0) {
+    const T* z = (const T*)d.logits + n * d.logits_stride;
+    const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
+    s = WarpRow<T, ITEMS>(z, (int)d.vocab, scale * kLog2e).s;
+    if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
+  }
+  if (threadIdx.x % 32 == 0) {
+    PreferenceScratch(d).stats[n] = s;
     d.logp[n] = logp;
   }
 }
 
-__global__ void __launch_bounds__(1024) k_preference_pairs(tb_preference_desc d) {
+// A block a pair: both answers' sums in f64 (the margin is a small difference of long sums), the
+// pair's term, and its rows' slopes.
+constexpr int kPairThreads = 256;
+__global__ void __launch_bounds__(kPairThreads) k_preference_pairs(tb_preference_desc d) {
   pdl_entry();
-  __shared__ double terms[32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const RowStats* stats = (const RowStats*)d.workspace;
-  float* slopes = (float*)(stats + d.rows);
-  double total = 0;
-  for (int64_t i = warp; i < d.pairs; i += 32) {
-    double ratio[2];
-    int64_t lo[2], hi[2];
-    for (int k = 0; k < 2; ++k) {
-      const int64_t s = i + k * d.pairs;
-      lo[k] = clamp_row(d.offsets[s], d.rows);
-      hi[k] = clamp_row(d.offsets[s + 1], d.rows);
-      double r = 0;
-      for (int64_t n = lo[k] + lane; n < hi[k]; n += 32)
-        if (stats[n].sum != 0.0f) r += (double)d.logp[n] - (double)d.ref_logp[n];
+  __shared__ double part[2][kPairThreads / 32];
+  const PreferenceScratch scratch(d);
+  const int64_t i = blockIdx.x;
+  int64_t lo[2], hi[2];
+  double ratio[2];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(~0u, r, o);
-      ratio[k] = r;
-      if (lane == 0) d.ratios[s] = (float)r;
-    }
-    const double w = d.weights ? (double)d.weights[i] : 1.0 / (double)d.pairs;
-    const double m = d.beta * (ratio[0] - ratio[1]), e = exp(-fabs(m));
-    const double soft = log1p(e);  // -log sigmoid(|m|)
-    const double lose = m >= 0 ? e / (1 + e) : 1 / (1 + e);  // sigmoid(-m)
-    const double yes = m >= 0 ? soft : soft - m, no = m >= 0 ? soft + m : soft;
-    // a share of 0 adds nothing, whatever it would multiply
-    total += w * ((1 - d.smoothing) * yes + (d.smoothing > 0 ? d.smoothing * no : 0.0));
-    const float slope = (float)(w * d.beta * (d.smoothing * (1 - lose) - (1 - d.smoothing) * lose));
-    for (int k = 0; k < 2; ++k)
-      for (int64_t n = lo[k] + lane; n < hi[k]; n += 32) slopes[n] = k ? -slope : slope;
+  for (int k = 0; k < 2; ++k) {
+    lo[k] = clamp_row(d.offsets[i + k * d.pairs], d.rows);
+    hi[k] = clamp_row(d.offsets[i + k * d.pairs + 1], d.rows);
+    double r = 0;
+#pragma unroll 4
+    for (int64_t n = lo[k] + threadIdx.x; n < hi[k]; n += kPairThreads)
+      if (scratch.stats[n].sum != 0.0f) r += (double)d.logp[n] - (double)d.ref_logp[n];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(~0u, r, o);
+    if (threadIdx.x % 32 == 0) part[k][threadIdx.x / 32] = r;
   }
-  if (lane == 0) terms[warp] = total;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) total += terms[w];
-    d.loss[0] = (float)total;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    ratio[k] = part[k][0];
+    for (int w = 1; w < kPairThreads / 32; ++w) ratio[k] += part[k][w];
   }
+  const double w = d.weights ? (double)d.weights[i] : 1.0 / (double)d.pairs;
+  const double m = d.beta * (ratio[0] - ratio[1]), e = exp(-fabs(m));
+  const double soft = log1p(e);                            // -log sigmoid(|m|)
+  const double lose = m >= 0 ? e / (1 + e) : 1 / (1 + e);  // sigmoid(-m)
+  const double yes = m >= 0 ? soft : soft - m, no = m >= 0 ? soft + m : soft;
+  if (threadIdx.x == 0) {
+    d.ratios[i] = (float)ratio[0];
+    d.ratios[i + d.pairs] = (float)ratio[1];
+    // a share of 0 adds nothing, whatever it would multiply
+    scratch.terms[i] = w * ((1 - d.smoothing) * yes + (d.smoothing > 0 ? d.smoothing * no : 0.0));
+  }
+  const float slope = (float)(w * d.beta * (d.smoothing * (1 - lose) - (1 - d.smoothing) * lose));
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    for (int64_t n = lo[k] + threadIdx.x; n < hi[k]; n += kPairThreads) scratch.slopes[n] = k ? -slope : slope;
+}
+
+// The pairs' terms in a fixed order, by one warp.
+__device__ __forceinline__ void sum_pairs(const tb_preference_desc& d) {
+  const double* terms = PreferenceScratch(d).terms;
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < d.pairs; i += 32) s += terms[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  if (threadIdx.x == 0) d.loss[0] = (float)s;
+}
+__global__ void k_preference_sum(tb_preference_desc d) {
+  pdl_entry();
+  sum_pairs(d);
 }
 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_preference_gradient(tb_preference_desc d) {
   pdl_entry();
-  const int64_t n = blockIdx.x;
-  if (n < d.offsets[0] || n >= d.offsets[2 * d.pairs]) return;
-  const RowStats s = ((const RowStats*)d.workspace)[n];
-  const float slope = ((const float*)((const RowStats*)d.workspace + d.rows))[n];
+  if (blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(d);
+  // from the last row back: the rows that were read last are still in the L2 cache
+  const int64_t n = d.rows - 1 - blockIdx.x;
+  if (!scored(d, n)) return;
+  const PreferenceScratch scratch(d);
+  const RowStats s = scratch.stats[n];
   const int64_t t = d.targets[n];
+  const float slope = t < d.vocab ? scratch.slopes[n] : NAN;
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
   const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
   if (s.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
-  else
-    stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, (float)d.scale, t < d.vocab ? slope : NAN, t));
+  else stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, (float)d.scale, slope, t));
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_preference_gradient_warps(tb_preference_desc d) {
+  pdl_entry();
+  if (blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(d);
+  const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  if (n >= d.rows || !scored(d, n)) return;
+  const PreferenceScratch scratch(d);
+  const RowStats s = scratch.stats[n];
+  const int64_t t = d.targets[n];
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  if (s.sum == 0.0f) {
+    zero_warp_row(out, d.vocab);
+    return;
+  }
+  const RowGradient<T> g(out, z, s, (float)d.scale, t < d.vocab ? scratch.slopes[n] : NAN, t);
+#pragma unroll 4
+  for (int64_t v = threadIdx.x % 32; v < d.vocab; v += 32) g.single(to_f32(z[v]), v);
 }
 
 const char* check_logits(int64_t element, int64_t rows, int64_t vocab, int64_t stride, double scale,
@@ -686,22 +775,30 @@ cudaError_t enqueue_policy(const tb_policy_desc& d, cudaStream_t stream) {
   if (vocab <= kWarpVocab) TB_BY_ITEMS(k_policy_warps, d)
   if (!d.gradient) TB_BY_THREADS(k_policy_terms, d)
   const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
+  // one block a row while it holds one (8192 x 16000 bf16: 256 threads 111 us, two blocks of 128
+  // 130), else the smallest blocks whose clusters do (8192 x 50257 f32: 8 blocks of 128 threads
+  // 495 us, 4 of 256 501, 2 of 512 516; 4 of 512, half filled, 703)
   if (vectors <= kKeep * 128) return enqueue_kept<T, 128>(d, 1, vectors, stream);
   if (vectors <= kKeep * 256) return enqueue_kept<T, 256>(d, 1, vectors, stream);
-  for (int ranks = 1; ranks <= 8; ranks *= 2) {
-    const int64_t per = (vectors + ranks - 1) / ranks;
-    if (per <= kKeep * 512) return enqueue_kept<T, 512>(d, ranks, per, stream);
-  }
+  if (vectors <= kKeep * 512) return enqueue_kept<T, 512>(d, 1, vectors, stream);
+  const auto ranks = [&](int threads) { return (vectors + kKeep * threads - 1) / (kKeep * threads); };
+  const auto per = [&](int threads) { return (vectors + ranks(threads) - 1) / ranks(threads); };
+  if (ranks(128) <= 8) return enqueue_kept<T, 128>(d, (int)ranks(128), per(128), stream);
+  if (ranks(256) <= 8) return enqueue_kept<T, 256>(d, (int)ranks(256), per(256), stream);
+  if (ranks(512) <= 8) return enqueue_kept<T, 512>(d, (int)ranks(512), per(512), stream);
   return launch_pdl(k_policy_twice<T, 512>, dim3((unsigned)rows), dim3(512), 0, stream, d);
 }
 template <typename T>
 cudaError_t enqueue_preference_rows(const tb_preference_desc& d, cudaStream_t stream) {
   const int64_t rows = d.rows, vocab = d.vocab;
+  if (vocab <= kWarpVocab) TB_BY_ITEMS(k_preference_rows_warps, d)
   TB_BY_THREADS(k_preference_rows, d)
 }
 template <typename T>
 cudaError_t enqueue_preference_gradient(const tb_preference_desc& d, cudaStream_t stream) {
   const int64_t rows = d.rows, vocab = d.vocab;
+  if (vocab <= kWarpVocab)
+    return launch_pdl(k_preference_gradient_warps<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, d);
   TB_BY_THREADS(k_preference_gradient, d)
 }
 
@@ -757,20 +854,21 @@ int preference_loss(const tb_preference_desc* desc, void* stream) {
   if (!words_ok({d.loss, d.ratios, d.offsets}) || !aligned_to(d.weights, 4) ||
       (d.rows > 0 && !words_ok({d.targets, d.ref_logp, d.logp})))
     return call.invalid("a row array is NULL or unaligned");
-  if (tb_preference_workspace(d.rows) > 0) {
-    if (!d.workspace || d.workspace_bytes < tb_preference_workspace(d.rows))
-      return call.invalid("the workspace is too small");
-    if (!aligned_to(d.workspace, 16)) return call.invalid("the workspace is not 16-byte aligned");
-  }
+  if (!d.workspace || d.workspace_bytes < tb_preference_workspace(d.rows, d.pairs))
+    return call.invalid("the workspace is too small");
+  if (!aligned_to(d.workspace, 16)) return call.invalid("the workspace is not 16-byte aligned");
   if (const int code = call.ready()) return code;
   const bool f32 = d.element == TB_ELEMENT_F32;
   cudaError_t e = cudaSuccess;
   if (d.rows > 0)
     e = f32 ? enqueue_preference_rows<float>(d, call.stream()) : enqueue_preference_rows<bf16>(d, call.stream());
-  if (e == cudaSuccess) e = launch_pdl(k_preference_pairs, dim3(1), dim3(1024), 0, call.stream(), d);
+  if (e == cudaSuccess)
+    e = launch_pdl(k_preference_pairs, dim3((unsigned)d.pairs), dim3(kPairThreads), 0, call.stream(), d);
   if (e == cudaSuccess && d.rows > 0 && d.gradient)
     e = f32 ? enqueue_preference_gradient<float>(d, call.stream())
             : enqueue_preference_gradient<bf16>(d, call.stream());
+  else if (e == cudaSuccess)
+    e = launch_pdl(k_preference_sum, dim3(1), dim3(32), 0, call.stream(), d);
   return call.finish(e);
 }
 
@@ -790,4 +888,6 @@ extern "C" int tb_policy_loss(const tb_policy_desc* desc, void* stream) {
 extern "C" int tb_preference_loss(const tb_preference_desc* desc, void* stream) {
   return tb::guarded([&] { return tb::preference_loss(desc, stream); });
 }
-extern "C" int64_t tb_preference_workspace(int64_t rows) { return rows > 0 ? rows * 12 : 0; }
+extern "C" int64_t tb_preference_workspace(int64_t rows, int64_t pairs) {
+  return rows >= 0 && pairs > 0 && rows <= INT32_MAX && pairs <= INT32_MAX ? pairs * 8 + rows * 12 : 0;
+}

@@ -405,7 +405,7 @@ def preference_loss(logits, targets, offsets, ref_logp, *, beta: float = 0.1,
     ref = _words(ref_logp, "ref_logp", device, f32, (rows,))
     loss, ratios, logp = (ref_logp.new_empty(()), ref_logp.new_empty((2 * pairs,)),
                           torch.empty_like(ref_logp))
-    size = _entry("tb_preference_workspace")(rows)
+    size = _entry("tb_preference_workspace")(rows, pairs)
     workspace = logits.new_empty((size,), dtype=torch.uint8)
     request = (_ELEMENT[logits.dtype], rows, vocab, pairs, logits.stride(0), stride, scale, beta,
             smoothing, pointer, _words(targets, "targets", device, torch.int32, (rows,)),

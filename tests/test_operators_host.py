@@ -128,7 +128,7 @@ def test_entry_points_without_a_request(built):
                   "tb_head_rotate_backward", "tb_policy_loss", "tb_preference_loss"):
         assert getattr(lib, entry)(None, None) == INVALID
     assert lib.tb_head_rotate_workspace(-2) == lib.tb_head_rotate_workspace(514) == 0
-    assert lib.tb_preference_workspace(-1) == lib.tb_preference_workspace(0) == 0
+    assert lib.tb_preference_workspace(-1, 1) == lib.tb_preference_workspace(4, 0) == 0
     for bad in ((7, 256, 5, 256, 2, 5, 1.0, 256), (0, 0, 5, 256, 2, 5, 1.0, 256),
                 (0, 256, 5, 0, 2, 5, 1.0, 256), (0, 256, 5, 256, 2, 5, -1.0, 256),
                 (0, 256, 5, 256, -2, 5, 1.0, 256), (1, 257, 5, 256, 2, 5, 1.0, 256)):
