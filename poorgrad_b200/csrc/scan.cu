@@ -472,6 +472,79 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   }
 }
 
+// Short sequences, a decode step's single one among them: a thread takes V channels of one sequence
+// and walks it, kAtOnce rows loaded at a time.
+template <typename T, int V, int FORM, bool BACK>
+__global__ void __launch_bounds__(128) k_scan_short(tb_scan_desc d, int64_t lanes) {
+  pdl_entry();
+  typedef Raw<T, V> R;
+  typedef typename R::type Row;
+  constexpr int kAtOnce = 4;
+  const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x, b = i / lanes, c = (i - b * lanes) * V;
+  if (b >= d.batch) return;
+  const int length = (int)d.length;
+  const auto row = [&](const void* base, const int64_t s[2], int t) {
+    return (const Row*)((const T*)base + b * s[0] + t * s[1] + c);
+  };
+  const auto to = [&](void* base, const int64_t s[2], int t) {
+    return (Row*)((T*)base + b * s[0] + t * s[1] + c);
+  };
+  const auto state_of = [&](const float* from) {
+    Vec<V> r = splat<V>(0.0f);
+    if (from)
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.set(v, from[b * d.channels + c + v]);
+    return r;
+  };
+  const Vec<V> initial = BACK ? state_of(d.state) : splat<V>(0.0f);
+  Vec<V> value = state_of(BACK ? d.dfinal : d.state);
+  for (int first = 0; first < length; first += kAtOnce) {
+    Row g[kAtOnce], u[kAtOnce], before[kAtOnce], xs[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      g[j] = u[j] = before[j] = xs[j] = Row{};
+      if (first + j < length) {
+        const int t = BACK ? length - 1 - first - j : first + j;
+        g[j] = *row(d.gate, d.gate_strides, t);
+        u[j] = BACK ? *row(d.dh, d.dh_strides, t) : *row(d.x, d.x_strides, t);
+        if (BACK && t > 0) before[j] = *row(d.h, d.h_strides, t - 1);
+        if (BACK && FORM == TB_SCAN_SIGMOID) xs[j] = *row(d.x, d.x_strides, t);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (first + j >= length) break;
+      const int t = BACK ? length - 1 - first - j : first + j;
+      Vec<V> a = R::read(g[j]), w = splat<V>(1.0f);  // w: the form's 1 - a
+      const Vec<V> in = R::read(u[j]);
+      if (FORM == TB_SCAN_SIGMOID) {
+        const Gate<V> p = sigmoid_pair(a);
+        a = p.a;
+        w = p.b;
+      }
+      if (BACK) {
+        const Vec<V> gt = in + value;
+        const Vec<V> prior = t > 0 ? R::read(before[j]) : initial;
+        Vec<V> da = gt * prior, dv = gt;
+        if (FORM == TB_SCAN_SIGMOID) {
+          dv = gt * w;
+          da = dv * a * fma(R::read(xs[j]), splat<V>(-1.0f), prior);
+        }
+        value = a * gt;
+        *to(d.dgate, d.dgate_strides, t) = R::made(da);
+        *to(d.dx, d.dx_strides, t) = R::made(dv);
+      } else {
+        value = fma(a, value, FORM == TB_SCAN_SIGMOID ? in * w : in);
+        *to(d.h, d.h_strides, t) = R::made(value);
+      }
+    }
+  }
+  float* last = BACK ? d.dstate : d.final_state;
+  if (last)
+#pragma unroll
+    for (int v = 0; v < V; ++v) last[b * d.channels + c + v] = value.get(v);
+}
+
 // Blocks a cluster: as many as bring two blocks to every SM.
 int ranks_of(int64_t columns, int64_t spans) {
   int ranks = 1;
@@ -587,13 +660,23 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
   return launch<T, V, L, FORM, BACK, kWhole>(d, cut, stream);
 }
 
+// Measured, 64 sequences of 2048 f32 channels: 8 steps 2.9 us short and 9.6 tiled, 16 steps 5.8 and
+// 10.5, 32 steps 15.0 and 14.8; 4 sequences of 32 steps x 333 channels 3.2 and 2.7.
+constexpr int64_t kShort = 16;
+
 template <typename T, int FORM, bool BACK>
 cudaError_t enqueue_form(const tb_scan_desc& d, cudaStream_t stream) {
+  const bool pairs = lanes_fit(d, BACK, sizeof(T), 2 * sizeof(T));
+  if (d.sequences == 0 && d.length <= kShort) {
+    const int64_t lanes = pairs ? d.channels / 2 : d.channels, blocks = (d.batch * lanes + 127) / 128;
+    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    return launch_pdl(pairs ? k_scan_short<T, 2, FORM, BACK> : k_scan_short<T, 1, FORM, BACK>,
+                      dim3((unsigned)blocks), dim3(128), 0, stream, d, lanes);
+  }
   // as many steps a warp as 128 registers hold, with the next ones on their way
   constexpr int kPairs = sizeof(T) == 2 ? (BACK ? 8 : 16) : !BACK || FORM == TB_SCAN_DIRECT ? 8 : 4;
-  return lanes_fit(d, BACK, sizeof(T), 2 * sizeof(T))
-             ? enqueue<T, 2, kPairs, FORM, BACK>(d, stream)
-             : enqueue<T, 1, BACK ? 8 : 16, FORM, BACK>(d, stream);
+  return pairs ? enqueue<T, 2, kPairs, FORM, BACK>(d, stream)
+               : enqueue<T, 1, BACK ? 8 : 16, FORM, BACK>(d, stream);
 }
 
 template <typename T>

@@ -53,11 +53,13 @@ def _device_of(first, name: str):
 
 
 def _array(t, name: str, device, dtype, shape):
-    """Address of a large array of this type, device and shape whose last axis has stride 1."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
-            and t.device == device and (t.stride(-1) == 1 or shape[-1] <= 1)):
-        _unfit(t, name, device, dtype, shape, "stride 1 along the last axis")
-    return t.data_ptr()
+    """(strides, address) of a large array of this type, device and shape whose last axis has
+    stride 1."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        strides = t.stride()
+        if strides[-1] == 1 or shape[-1] <= 1:
+            return strides, t.data_ptr()
+    _unfit(t, name, device, dtype, shape, "stride 1 along the last axis")
 
 
 def _words(t, name: str, device, dtype, shape):
@@ -102,7 +104,7 @@ def _call(name: str, device, *arguments):
 
 
 # ------------------------------------------------------------------ gated scan
-def _scan_extents(x, offsets, device):
+def _scan_extents(x, offsets):
     """(batch, length, channels, sequences, rows of the states)."""
     if offsets is None:
         _need(x.dim() == 3, "x: expected [batch, length, channels], or packed [rows, channels] "
@@ -119,21 +121,17 @@ def _scan_extents(x, offsets, device):
 def _states(like, x, count, channels):
     """A new [count, channels] float32 array (a copy of `like`'s form is the quicker to make)."""
     if like is not None and like.shape == (count, channels) and like.dtype is torch.float32:
-        return torch.empty_like(like)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     return x.new_empty((count, channels), dtype=torch.float32)
 
 
 def _scan_workspace(x, batch, length, channels):
     """(tensor, address, bytes) of the scratch that a long call is cut along time with."""
-    size = _entry("tb_gated_scan_workspace")(batch, length, channels) if length >= 512 else 0
+    size = _entry("tb_gated_scan_workspace")(batch, length, channels) if length >= 256 else 0
     if not size:
         return None, 0, 0
     workspace = x.new_empty((size,), dtype=torch.uint8)
     return workspace, workspace.data_ptr(), size
-
-
-def _time_strides(t):
-    return (0, t.stride(0)) if t.dim() == 2 else (t.stride(0), t.stride(1))
 
 
 def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=None,
@@ -149,22 +147,27 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
     does.  ``out`` may be ``gate`` or ``x``."""
     device = _device_of(x, "x")
     _need(form in _FORM, "form: 'direct' or 'sigmoid' is expected")
-    batch, length, channels, sequences, count = _scan_extents(x, offsets, device)
+    batch, length, channels, sequences, count = _scan_extents(x, offsets)
+    shape, dtype, states = x.shape, x.dtype, (count, channels)
+    gate_s, gate_p = _array(gate, "gate", device, dtype, shape)
+    x_s, x_p = _array(x, "x", device, dtype, shape)
     if out is None:
         out = _like(x)
+    out_s, out_p = _array(out, "out", device, dtype, shape)
+    state_p = _words(state, "state", device, torch.float32, states)
     if final_state is None:
         final_state = _states(state, x, count, channels)
-    shape, dtype = x.shape, x.dtype
-    pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
-                _array(out, "out", device, dtype, shape),
-                _words(offsets, "offsets", device, torch.int32, (sequences + 1,)),
-                _words(state, "state", device, torch.float32, (count, channels)),
-                _words(final_state, "final_state", device, torch.float32, (count, channels)))
+        final_p = final_state.data_ptr()
+    else:
+        final_p = _words(final_state, "final_state", device, torch.float32, states)
+    offsets_p = _words(offsets, "offsets", device, torch.int32, (sequences + 1,))
+    if sequences:  # packed: no batch axis
+        gate_s, x_s, out_s = (0, *gate_s), (0, *x_s), (0, *out_s)
     workspace, scratch, size = _scan_workspace(x, batch, length, channels)
-    request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
-                    *_time_strides(gate), *_time_strides(x), *_time_strides(out),
-                    0, 0, 0, 0, 0, 0, *pointers, 0, 0, 0, 0, 0, scratch, size)
-    _call("tb_gated_scan", device, request)
+    _call("tb_gated_scan", device,
+          _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences, gate_s[0],
+                gate_s[1], x_s[0], x_s[1], out_s[0], out_s[1], 0, 0, 0, 0, 0, 0, gate_p, x_p, out_p,
+                offsets_p, state_p, final_p, 0, 0, 0, 0, 0, scratch, size))
     return out, final_state
 
 
@@ -175,29 +178,27 @@ def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, of
     sigmoid form only.  One of ``dgate`` and ``dx`` may be ``dh``."""
     device = _device_of(dh, "dh")
     _need(form in _FORM, "form: 'direct' or 'sigmoid' is expected")
-    batch, length, channels, sequences, count = _scan_extents(dh, offsets, device)
-    shape, dtype = dh.shape, dh.dtype
+    batch, length, channels, sequences, count = _scan_extents(dh, offsets)
+    shape, dtype, states = dh.shape, dh.dtype, (count, channels)
     if dgate is None:
         dgate = _like(dh)
     if dx is None:
         dx = _like(dh)
-    dstate = _states(state, dh, count, channels)
     if form == "direct" and x is None:
         x = gate  # not read
-    pointers = (_array(gate, "gate", device, dtype, shape), _array(x, "x", device, dtype, shape),
-                _array(h, "h", device, dtype, shape),
-                _words(offsets, "offsets", device, torch.int32, (sequences + 1,)),
-                _words(state, "state", device, torch.float32, (count, channels)), 0,
-                _array(dh, "dh", device, dtype, shape),
-                _words(dfinal, "dfinal", device, torch.float32, (count, channels)),
-                _array(dgate, "dgate", device, dtype, shape),
-                _array(dx, "dx", device, dtype, shape), dstate.data_ptr())
+    arrays = [_array(t, name, device, dtype, shape)
+              for t, name in ((gate, "gate"), (x, "x"), (h, "h"), (dh, "dh"), (dgate, "dgate"),
+                              (dx, "dx"))]
+    state_p = _words(state, "state", device, torch.float32, states)
+    dfinal_p = _words(dfinal, "dfinal", device, torch.float32, states)
+    dstate = _states(state, dh, count, channels)
+    offsets_p = _words(offsets, "offsets", device, torch.int32, (sequences + 1,))
     workspace, scratch, size = _scan_workspace(dh, batch, length, channels)
-    request = _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences,
-                    *_time_strides(gate), *_time_strides(x), *_time_strides(h),
-                    *_time_strides(dh), *_time_strides(dgate), *_time_strides(dx), *pointers,
-                    scratch, size)
-    _call("tb_gated_scan_backward", device, request)
+    strides = [n for s, _ in arrays for n in ((0, s[0]) if sequences else s[:2])]
+    _call("tb_gated_scan_backward", device,
+          _scan(_ELEMENT[dtype], _FORM[form], batch, length, channels, sequences, *strides,
+                arrays[0][1], arrays[1][1], arrays[2][1], offsets_p, state_p, 0, arrays[3][1],
+                dfinal_p, arrays[4][1], arrays[5][1], dstate.data_ptr(), scratch, size))
     return dgate, dx, dstate
 
 
@@ -217,37 +218,40 @@ def _heads(t):
     return t.unsqueeze(0) if t.dim() == 3 else t
 
 
-def _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon, style, q_out,
-                    k_out, dq, dk, dq_weight, dk_weight, workspace, workspace_bytes):
-    batch, length, q_heads, dim = q.shape
-    k_heads, dtype = k.shape[2], q.dtype
-    q_shape, k_shape = q.shape, (batch, length, k_heads, dim)
+def _rotate_call(entry, device, q, k, table, positions, q_weight, k_weight, epsilon, style, q_out,
+                 k_out, dq, dk, dq_weight, dk_weight, workspace, workspace_bytes):
+    q_shape, dtype = q.shape, q.dtype
+    batch, length, q_heads, dim = q_shape
+    k_heads = k.shape[2]
+    k_shape = (batch, length, k_heads, dim)
+    f32 = torch.float32
     _need(isinstance(table, torch.Tensor) and table.dim() == 2,
           "table: expected [positions, turned]")
     _need(style in _STYLE, "style: 'halves' or 'pairs' is expected")
-    pointers = (_array(q, "q", device, dtype, q_shape), _array(k, "k", device, dtype, k_shape),
-                _words(table, "table", device, torch.float32, table.shape),
-                _words(positions, "positions", device, torch.int32, (batch, length)),
-                _words(q_weight, "q_weight", device, torch.float32, (dim,)),
-                _words(k_weight, "k_weight", device, torch.float32, (dim,)),
-                _array(q_out, "q_out", device, dtype, q_shape),
-                _array(k_out, "k_out", device, dtype, k_shape))
-    if dq is None:
-        strides, more = (0,) * 6, (0, 0)
-    else:
-        more = (_array(dq, "dq", device, dtype, q_shape), _array(dk, "dk", device, dtype, k_shape))
-        strides = dq.stride()[:3] + dk.stride()[:3]
-    return _rotate(_ELEMENT[dtype], _STYLE[style], batch, length, q_heads, k_heads, dim,
-                   table.shape[1], table.shape[0], *q.stride()[:3], *k.stride()[:3],
-                   *q_out.stride()[:3], *k_out.stride()[:3], *strides, epsilon, *pointers, *more,
-                   dq_weight, dk_weight, workspace, workspace_bytes)
+    (qb, qt, qh, _), q_p = _array(q, "q", device, dtype, q_shape)
+    (kb, kt, kh, _), k_p = _array(k, "k", device, dtype, k_shape)
+    (ob, ot, oh, _), o_p = _array(q_out, "q_out", device, dtype, q_shape)
+    (pb, pt, ph, _), p_p = _array(k_out, "k_out", device, dtype, k_shape)
+    gb = gt = gh = g_p = rb = rt = rh = r_p = 0
+    if dq is not None:
+        (gb, gt, gh, _), g_p = _array(dq, "dq", device, dtype, q_shape)
+        (rb, rt, rh, _), r_p = _array(dk, "dk", device, dtype, k_shape)
+    table_shape = table.shape
+    _call(entry, device, _rotate(
+        _ELEMENT[dtype], _STYLE[style], batch, length, q_heads, k_heads, dim, table_shape[1],
+        table_shape[0], qb, qt, qh, kb, kt, kh, ob, ot, oh, pb, pt, ph, gb, gt, gh, rb, rt, rh,
+        epsilon, q_p, k_p, _words(table, "table", device, f32, table_shape),
+        _words(positions, "positions", device, torch.int32, (batch, length)),
+        _words(q_weight, "q_weight", device, f32, (dim,)),
+        _words(k_weight, "k_weight", device, f32, (dim,)), o_p, p_p, g_p, r_p, dq_weight, dk_weight,
+        workspace, workspace_bytes))
 
 
 def _rotate_inputs(q, k, positions):
     device = _device_of(q, "q")
     _need(q.dim() in (3, 4) and isinstance(k, torch.Tensor) and k.dim() == q.dim(),
           "q, k: expected [tokens, heads, dim] or [batch, length, heads, dim]")
-    if isinstance(positions, torch.Tensor) and positions.dim() == 1 and q.dim() == 3:
+    if q.dim() == 3 and isinstance(positions, torch.Tensor) and positions.dim() == 1:
         positions = positions.unsqueeze(0)
     return device, positions
 
@@ -270,13 +274,11 @@ def head_rotate(q, k, table, positions=None, *, q_weight=None, k_weight=None,
     if k_out is None:
         k_out = _like(k)
     if q.dim() == 4:
-        request = _rotate_request(device, q, k, table, positions, q_weight, k_weight, epsilon,
-                                  style, q_out, k_out, None, None, 0, 0, 0, 0)
+        _rotate_call("tb_head_rotate", device, q, k, table, positions, q_weight, k_weight, epsilon,
+                     style, q_out, k_out, None, None, 0, 0, 0, 0)
     else:
-        request = _rotate_request(device, _heads(q), _heads(k), table, positions, q_weight,
-                                  k_weight, epsilon, style, _heads(q_out), _heads(k_out), None,
-                                  None, 0, 0, 0, 0)
-    _call("tb_head_rotate", device, request)
+        _rotate_call("tb_head_rotate", device, _heads(q), _heads(k), table, positions, q_weight,
+                     k_weight, epsilon, style, _heads(q_out), _heads(k_out), None, None, 0, 0, 0, 0)
     return q_out, k_out
 
 
@@ -287,22 +289,24 @@ def head_rotate_backward(dq, dk, q, k, table, positions=None, *, q_weight=None, 
     gradients ``dq`` and ``dk`` of its outputs; the last two are float32 ``[dim]``, or None with
     ``weights=False``.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
     device, positions = _rotate_inputs(q, k, positions)
+    _need(isinstance(dq, torch.Tensor) and isinstance(dk, torch.Tensor)
+          and dq.dim() == dk.dim() == q.dim(), "dq, dk: expected the shapes of q and k")
     if q_out is None:
         q_out = _like(q)
     if k_out is None:
         k_out = _like(k)
     dq_weight = dk_weight = workspace = None
-    p = [0, 0, 0, 0]
+    given = (0, 0, 0, 0)
     if weights:
         dim = q.shape[-1]
         dq_weight = q.new_empty((dim,), dtype=torch.float32)
         dk_weight = torch.empty_like(dq_weight)
-        workspace = q.new_empty((_entry("tb_head_rotate_workspace")(dim),), dtype=torch.uint8)
-        p = [dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), workspace.numel()]
-    request = _rotate_request(device, _heads(q), _heads(k), table, positions, q_weight, k_weight,
-                              epsilon, style, _heads(q_out), _heads(k_out), _heads(dq), _heads(dk),
-                              *p)
-    _call("tb_head_rotate_backward", device, request)
+        size = _entry("tb_head_rotate_workspace")(dim)
+        workspace = q.new_empty((size,), dtype=torch.uint8)
+        given = dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), size
+    _rotate_call("tb_head_rotate_backward", device, _heads(q), _heads(k), table, positions, q_weight,
+                 k_weight, epsilon, style, _heads(q_out), _heads(k_out), _heads(dq), _heads(dk),
+                 *given)
     return q_out, k_out, dq_weight, dk_weight
 
 
@@ -322,30 +326,32 @@ class PreferenceLoss(NamedTuple):
 
 
 def _logits(logits):
+    """(device, row stride, address)."""
     device = _device_of(logits, "logits")
     _need(logits.dim() == 2, "logits: expected [rows, vocab]")
-    return device, _array(logits, "logits", device, logits.dtype, logits.shape)
+    strides, address = _array(logits, "logits", device, logits.dtype, logits.shape)
+    return device, strides[0], address
 
 
 def _gradient_of(logits, gradient, device):
-    """(tensor, pointer, row stride) of a gradient that is wanted (True), given, or neither."""
+    """(tensor, row stride, address) of a gradient that is wanted (True), given, or neither."""
     if gradient is None or gradient is False:
         return None, 0, 0
     if gradient is True:
         gradient = _like(logits)
-    return gradient, _array(gradient, "gradient", device, logits.dtype,
-                            logits.shape), gradient.stride(0)
+    strides, address = _array(gradient, "gradient", device, logits.dtype, logits.shape)
+    return gradient, strides[0], address
 
 
 def token_logp(logits, targets, *, scale: float = 1.0):
     """Float32 log probabilities of ``targets`` (int32 ``[rows]``) under ``softmax(scale * logits)``
     of each row.  A hidden row -- a negative target, or no logit above -inf -- gives 0, a target
     beyond the vocabulary NaN."""
-    device, pointer = _logits(logits)
+    device, row, pointer = _logits(logits)
     rows, vocab = logits.shape
     _need(targets is not None, "targets: missing")
     logp = logits.new_empty((rows,), dtype=torch.float32)
-    _call("tb_token_logp", device, _ELEMENT[logits.dtype], pointer, logits.stride(0),
+    _call("tb_token_logp", device, _ELEMENT[logits.dtype], pointer, row,
           _words(targets, "targets", device, torch.int32, (rows,)), rows, vocab, scale,
           logp.data_ptr())
     return logp
@@ -361,17 +367,17 @@ def policy_loss(logits, targets, old_logp, advantages, weights, *, ref_logp=None
     weights hold the normalizer (1 / tokens, say) and hide a row where they are 0.  A hidden row,
     also one as in :func:`token_logp`, adds nothing whatever it holds and has a gradient of 0.
     ``gradient`` is True, False, or the array to write, which may be ``logits`` itself."""
-    device, pointer = _logits(logits)
+    device, row, pointer = _logits(logits)
     rows, vocab = logits.shape
     _need(targets is not None and old_logp is not None and advantages is not None
           and weights is not None and (kl == 0 or ref_logp is not None),
           "targets, old_logp, advantages and weights are needed, and ref_logp where kl is not 0")
-    gradient, to, stride = _gradient_of(logits, gradient, device)
+    gradient, stride, to = _gradient_of(logits, gradient, device)
     f32, shape = torch.float32, (rows,)
     old = _words(old_logp, "old_logp", device, f32, shape)
     loss, token_loss, logp = (old_logp.new_empty(()), torch.empty_like(old_logp),
                               torch.empty_like(old_logp))
-    request = _policy(_ELEMENT[logits.dtype], rows, vocab, logits.stride(0), stride, scale, clip_low,
+    request = _policy(_ELEMENT[logits.dtype], rows, vocab, row, stride, scale, clip_low,
                       clip_high, kl, pointer,
                       _words(targets, "targets", device, torch.int32, shape),
                       old,
@@ -394,20 +400,20 @@ def preference_loss(logits, targets, offsets, ref_logp, *, beta: float = 0.1,
     ``m = beta (ratio_chosen - ratio_rejected)`` the loss is the weighted sum (``weights`` float32
     per pair, 1 / pairs when None) of ``-(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m)``.
     Rows outside every answer are left as they were.  ``gradient`` as in :func:`policy_loss`."""
-    device, pointer = _logits(logits)
+    device, row, pointer = _logits(logits)
     rows, vocab = logits.shape
     _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 3
           and offsets.shape[0] % 2 == 1, "offsets: expected 2 pairs + 1 row numbers")
     _need(targets is not None and ref_logp is not None, "targets and ref_logp are needed")
     pairs = offsets.shape[0] // 2
-    gradient, to, stride = _gradient_of(logits, gradient, device)
+    gradient, stride, to = _gradient_of(logits, gradient, device)
     f32 = torch.float32
     ref = _words(ref_logp, "ref_logp", device, f32, (rows,))
     loss, ratios, logp = (ref_logp.new_empty(()), ref_logp.new_empty((2 * pairs,)),
                           torch.empty_like(ref_logp))
     size = _entry("tb_preference_workspace")(rows, pairs)
     workspace = logits.new_empty((size,), dtype=torch.uint8)
-    request = (_ELEMENT[logits.dtype], rows, vocab, pairs, logits.stride(0), stride, scale, beta,
+    request = (_ELEMENT[logits.dtype], rows, vocab, pairs, row, stride, scale, beta,
             smoothing, pointer, _words(targets, "targets", device, torch.int32, (rows,)),
             _words(offsets, "offsets", device, torch.int32, (2 * pairs + 1,)), ref,
             _words(weights, "weights", device, f32, (pairs,)),
