@@ -1,4 +1,5 @@
-"""Builds ``libtopos_b200.so`` in-tree with nvcc for sm_100a.
+"""Builds ``libtopos_b200.so`` in-tree with nvcc for sm_100a, and ``_operators.so``, the binding of
+its device operators to torch tensors.
 
 Host files (``csrc/*.cpp``) and CUDA files (``csrc/*.cu``) compile to objects
 under ``_build/`` in parallel, then link into one shared library with a static
@@ -8,15 +9,18 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 OUT = os.path.join(HERE, "libtopos_b200.so")
+BINDING = os.path.join(HERE, "_operators.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-contract=off",
@@ -39,7 +43,33 @@ def _compile(src: str) -> str:
     return obj
 
 
+def build_binding(force: bool = False) -> str:
+    """Compiles ``csrc/python/operators_binding.cpp`` against torch and the library."""
+    src = os.path.join(CSRC, "python", "operators_binding.cpp")
+    deps = [src, os.path.join(ROOT, "include", "topos_b200.h")]
+    if (not force and os.path.exists(BINDING)
+            and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps)):
+        return BINDING
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", src, "-o", BINDING,
+           f"-I{os.path.join(torch, 'include')}", f"-I{sysconfig.get_paths()['include']}",
+           "-I/usr/local/cuda/include", f"-L{os.path.join(torch, 'lib')}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           f"-L{HERE}", "-l:libtopos_b200.so", "-Wl,-rpath,$ORIGIN",
+           f"-Wl,-rpath,{os.path.join(torch, 'lib')}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n{res.stdout}\n{res.stderr}")
+    return BINDING
+
+
 def build(force: bool = False) -> str:
+    out = build_library(force)
+    build_binding(force)
+    return out
+
+
+def build_library(force: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cpp")) + glob.glob(os.path.join(CSRC, "*.cu")))
     if force:
