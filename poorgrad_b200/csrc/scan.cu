@@ -129,53 +129,64 @@ struct Marks {
   int sequence;
 };
 // How many of the first `sequences` offsets are at or below t (32 are looked at a time).
-__device__ __forceinline__ int64_t begun_by(const tb_scan_desc& d, int64_t t) {
+__device__ __forceinline__ int begun_by(const tb_scan_desc& d, int t) {
   const int lane = threadIdx.x % 32;
-  int64_t lo = 0, n = d.sequences;  // the answer lies in [lo, lo + n]
+  int lo = 0, n = (int)d.sequences;  // the answer lies in [lo, lo + n]
   while (n > 0) {
-    const int64_t stride = (n + 31) / 32, i = lo + (lane + 1) * stride - 1;
+    const int stride = (n + 31) / 32, i = lo + (lane + 1) * stride - 1;
     const bool below = i < lo + n && d.offsets[i] <= t;
-    const int64_t k = __popc(__ballot_sync(~0u, below));
+    const int k = __popc(__ballot_sync(~0u, below));
     lo += k * stride;
     n = min(n - k * stride, stride - 1);
   }
   return lo;
 }
+// The sequence that a warp's last run lay in: most runs lie in the same one and need no search.
+struct Known {
+  int sequence = 0, from = 0, to = 0;
+  // Whether rows [low, high] lie strictly inside it.
+  __device__ __forceinline__ bool holds(int low, int high) const { return from < low && high < to - 1; }
+};
 template <int L, bool BACK>
-__device__ __forceinline__ Marks marks_of(const tb_scan_desc& d, int64_t b, int64_t first) {
-  const int lane = threadIdx.x % 32;
-  constexpr unsigned kAll = L == 32 ? ~0u : (1u << L) - 1;
-  const int64_t left = d.length - first;
-  const unsigned here = left >= L ? kAll : left <= 0 ? 0u : (1u << (int)left) - 1;
+__device__ __forceinline__ Marks marks_of(const tb_scan_desc& d, int b, int first, Known& known) {
+  const int lane = threadIdx.x % 32, length = (int)d.length;
+  constexpr unsigned kAll = (1u << L) - 1;
+  const int left = length - first;
+  const unsigned here = left >= L ? kAll : left <= 0 ? 0u : (1u << left) - 1;
   Marks m;
   if (d.sequences == 0) {
-    m.sequence = (int)b;
+    m.sequence = b;
     m.inside = here;
     m.enters = first == 0 ? here & 1 : 0u;
-    m.leaves = left > 0 && left <= L ? 1u << (int)(left - 1) : 0u;
+    m.leaves = left > 0 && left <= L ? 1u << (left - 1) : 0u;
     return m;
   }
-  const int64_t low = BACK ? d.length - first - L : first, high = low + L - 1;  // rows
-  const int64_t begun = begun_by(d, low), s = max(begun - 1, (int64_t)0);
-  const int64_t from = d.offsets[s], to = d.offsets[s + 1];
-  if (here == kAll && begun > 0 && from < low && high < to - 1 && low > 0 && high < d.length - 1) {
-    m.sequence = (int)s;  // the run lies within one sequence
-    m.inside = kAll;
-    m.enters = m.leaves = 0;
+  m.inside = kAll;
+  m.enters = m.leaves = 0;
+  const int low = BACK ? length - first - L : first, high = low + L - 1;  // rows
+  if (here == kAll && known.holds(low, high)) {
+    m.sequence = known.sequence;
     return m;
   }
-  const int64_t step = first + lane, t = BACK ? d.length - 1 - step : step;
+  const int begun = begun_by(d, low), s = max(begun - 1, 0);
+  // offsets are data: whatever they hold, the first and last rows of the array are borders
+  known = {s, max(d.offsets[s], 0), min(d.offsets[s + 1], length)};
+  if (here == kAll && begun > 0 && known.holds(low, high)) {
+    m.sequence = s;
+    return m;
+  }
+  const int t = BACK ? length - 1 - first - lane : first + lane;
   const bool mine = here >> lane & 1;
   // the last sequence that starts at or before t
-  int64_t lo = s, hi = d.sequences;
+  int lo = s, hi = (int)d.sequences;
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
+    const int mid = (lo + hi) / 2;
     if (mine && d.offsets[mid] <= t) lo = mid; else hi = mid;
   }
-  const int64_t mine_from = d.offsets[lo], mine_to = d.offsets[lo + 1];
-  const bool inside = mine && mine_from <= t && t < mine_to;
-  const bool starts = t == mine_from || t == 0, ends = t == mine_to - 1 || t == d.length - 1;
-  m.sequence = (int)lo;
+  const int from = d.offsets[lo], to = d.offsets[lo + 1];
+  const bool inside = mine && from <= t && t < to;
+  const bool starts = t == from || t == 0, ends = t == to - 1 || t == length - 1;
+  m.sequence = lo;
   m.inside = __ballot_sync(~0u, inside);
   m.enters = __ballot_sync(~0u, inside && (BACK ? ends : starts));
   m.leaves = __ballot_sync(~0u, inside && (BACK ? starts : ends));
@@ -381,6 +392,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
 
   Vec<V> carry = splat<V>(0.0f);
   if (PASS == kFromMaps && s.in)
+#pragma unroll 8
     for (int p = 0; p < part; ++p) {
       const float2* from = cut.maps + (b * cut.parts + p) * d.channels + s.c;
       Affine<V> f;
@@ -395,25 +407,28 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   bool whole_begins = false;
 
   int parity = 0;
-  const int64_t from = part * cut.part_steps, to = min(from + cut.part_steps, d.length);
-  const int64_t span = (int64_t)ranks * kWarps * L;
+  const int from = (int)(part * cut.part_steps), to = (int)min(from + cut.part_steps, d.length);
+  const int span = ranks * kWarps * L;
   // a part is a whole number of spans, so that no step belongs to two
   const bool whole_warp = __all_sync(~0u, s.in);
-  typename Scan<T, V, L, FORM, BACK, PASS>::Rows rows, next;
-  int64_t first = from + (rank * kWarps + warp) * L;
+  // forwards, a step's rows are done with once it is reduced, and the next take their place
+  typename Scan<T, V, L, FORM, BACK, PASS>::Rows rows, after;
+  auto& next = BACK && PASS != kMaps ? after : rows;
+  int first = from + (rank * kWarps + warp) * L;
   bool all = whole_warp && first + L <= d.length;
   if (all) s.template load<true>(rows, first); else s.template load<false>(rows, first);
-  Marks m = marks_of<L, BACK>(d, b, first), next_m = m;
-  for (int64_t base = from; base < to; base += span, parity ^= 1) {
+  Known known;
+  Marks m = marks_of<L, BACK>(d, (int)b, first, known), next_m = m;
+  for (int base = from; base < to; base += span, parity ^= 1) {
     const bool marked = m.enters | m.leaves | (m.inside != (1u << L) - 1);
     const Affine<V> map = m.enters ? s.template reduce<true>(rows, m) : s.template reduce<false>(rows, m);
     // the next steps are on their way while these are finished
-    const int64_t next_first = first + span;
+    const int next_first = first + span;
     const bool next_all = whole_warp && next_first + L <= d.length;
     if (base + span < to) {
       if (next_all) s.template load<true>(next, next_first);
       else s.template load<false>(next, next_first);
-      next_m = marks_of<L, BACK>(d, b, next_first);
+      next_m = marks_of<L, BACK>(d, (int)b, next_first, known);
     }
     maps[parity][warp][lane] = map;
     if (lane == 0) begins[parity][warp] = m.enters != 0;
@@ -432,7 +447,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       if (PASS == kMaps) {
         whole = {whole.A * block.A, apply(block, any, whole.H)};
         whole_begins |= any;
-        rows = next, m = next_m, first = next_first, all = next_all;
+        m = next_m, first = next_first, all = next_all;
         continue;
       }
       cg::cluster_group cluster = cg::this_cluster();
@@ -461,7 +476,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
     }
     if (all && !marked) s.template write<true, false>(rows, m, first, value);
     else s.template write<false, true>(rows, m, first, value);
-    rows = next, m = next_m, first = next_first, all = next_all;
+    if (BACK && PASS != kMaps) rows = next;
+    m = next_m, first = next_first, all = next_all;
   }
   if (PASS == kMaps && warp == 0) {
     if (s.in)
@@ -554,12 +570,17 @@ int ranks_of(int64_t columns, int64_t spans) {
 // Into how many parts the time axis is cut, each part two launches' work: its map, then its
 // outputs.  1 where one launch fills the GPU and its clusters do not walk long: measured, 256
 // columns of 64 spans take 101 us in one launch and 146 cut, 96 of 16 spans 16 and 21; but 96
-// columns of 65 spans 46 and 38, 16 of 63 spans 25 and 13, 12 of 2048 spans 728 and 217.
-constexpr int64_t kMaxParts = 64;
+// columns of 65 spans 46 and 38, 16 of 63 spans 25 and 13, 12 of 2048 spans 728 and 217.  Four
+// blocks run on a SM: parts that fill them once, or twice where that leaves long ones (12 columns:
+// 49 parts 176 us, 64 parts 217; 96 columns: 12 parts 39.8, 6 parts 43), and at least four spans
+// each, for every part reads the maps of those before it (one column of 256 spans: 64 parts 14.2 us,
+// 256 parts 21; of 2048 spans: 296 parts 37, 592 parts 47).
+constexpr int64_t kMaxParts = 296;
 int parts_of(int64_t columns, int64_t spans) {
   const int ranks = ranks_of(columns, spans);
   if (columns >= 148 || spans <= 2 * ranks || (columns * ranks >= 148 && spans <= 8 * ranks)) return 1;
-  return (int)std::max<int64_t>(1, std::min({kMaxParts, (spans + 1) / 2, 8 * 148 / columns}));
+  const int64_t wave = 4 * 148 / columns, fill = wave >= 16 ? wave : 8 * 148 / columns;
+  return (int)std::max<int64_t>(1, std::min({kMaxParts, (spans + 3) / 4, fill}));
 }
 
 bool strides_ok(const tb_scan_desc& d, const int64_t s[2], bool written) {
@@ -568,10 +589,12 @@ bool strides_ok(const tb_scan_desc& d, const int64_t s[2], bool written) {
   return (d.length <= 1 || s[1] >= d.channels) && (d.batch <= 1 || s[0] >= d.channels);
 }
 
+constexpr int64_t kMaxLength = INT32_MAX - (1 << 16);  // steps are counted in 32 bits, a span past the end
+
 const char* check(const tb_scan_desc& d, bool backward) {
   if (d.element != TB_ELEMENT_F32 && d.element != TB_ELEMENT_BF16) return "unknown element type";
   if (d.form != TB_SCAN_DIRECT && d.form != TB_SCAN_SIGMOID) return "unknown form";
-  if (!extents_fit({d.batch, d.length, d.channels}) || d.length > INT32_MAX ||
+  if (!extents_fit({d.batch, d.length, d.channels}) || d.length > kMaxLength || d.batch > INT32_MAX ||
       !extents_fit({d.sequences, d.channels}) || d.sequences > INT32_MAX)
     return "extents out of range";
   if (d.sequences ? !d.offsets || d.batch != 1 : d.offsets != nullptr)
