@@ -218,7 +218,56 @@ struct Cut {
   int* begins;   // [batch][parts]
 };
 
-enum { kWhole = 0, kMaps = 1, kFromMaps = 2 };
+// A launch's part: a block walks its columns alone, or the blocks of a cluster together; or one of
+// the two launches over parts.
+enum { kWhole = 0, kMaps = 1, kFromMaps = 2, kCluster = 3 };
+
+// The exchange of maps between the blocks of a cluster: a lane sends its words straight into every
+// block's shared memory, and those count them in at a barrier of their own.  A cluster-wide barrier
+// would first wait for the outputs written so far to reach memory, a quarter of the time.
+__device__ __forceinline__ unsigned shared_address(const void* p) {
+  return (unsigned)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ unsigned of_rank(unsigned address, int rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void send(unsigned to, unsigned barrier, Affine<2> f) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(to), "r"(__float_as_uint(f.A.x.x)), "r"(__float_as_uint(f.A.x.y)),
+               "r"(__float_as_uint(f.H.x.x)), "r"(__float_as_uint(f.H.x.y)), "r"(barrier)
+               : "memory");
+}
+__device__ __forceinline__ void send(unsigned to, unsigned barrier, Affine<1> f) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+               ::"r"(to), "r"(__float_as_uint(f.A.x)), "r"(__float_as_uint(f.H.x)), "r"(barrier)
+               : "memory");
+}
+__device__ __forceinline__ void send(unsigned to, unsigned barrier, int v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+               ::"r"(to), "r"(v), "r"(barrier)
+               : "memory");
+}
+// Whether all that was expected has arrived; false after 4 seconds, which nothing but a fault
+// explains (the caller then makes its outputs NaN and goes on).
+__device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
+  unsigned long long since = 0;
+  while (true) {
+    int done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.s32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(barrier), "r"(phase)
+        : "memory");
+    if (done) return true;
+    unsigned long long now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (since == 0) since = now;
+    if (now - since > 4000000000ull) return false;
+  }
+}
 
 // The recurrence, or with BACK the gradients, walked backwards: there the carried value is
 // c_t = a_t (dh_t + c_{t+1}), g_t = dh_t + c_{t+1}.
@@ -367,16 +416,27 @@ struct Scan {
 template <typename T, int V, int L, int FORM, bool BACK, int PASS>
 __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut) {
   pdl_entry();
-  __shared__ Affine<V> maps[2][kWarps][32];
+  __shared__ alignas(16) Affine<V> maps[2][kWarps][32];
   __shared__ int begins[2][kWarps];
-  __shared__ Affine<V> rank_maps[2][kMaxRanks][32];
-  __shared__ int rank_begins[2][kMaxRanks];
+  constexpr int kHeld = PASS == kCluster ? kMaxRanks : 1;
+  __shared__ alignas(16) Affine<V> rank_maps[2][kHeld][32];
+  __shared__ int rank_begins[2][kHeld];
+  __shared__ alignas(8) uint64_t counted[2];  // barriers of the exchange, one a parity
   const int lane = threadIdx.x % 32, warp = __shfl_sync(~0u, threadIdx.x / 32, 0);
-  const int ranks = cut.ranks;
+  const int ranks = PASS == kCluster ? cut.ranks : 1;
   const int rank = blockIdx.x % ranks, tile = blockIdx.x / ranks % cut.tiles;
   const int part = blockIdx.x / ranks / cut.tiles % cut.parts;
   const int64_t b = blockIdx.x / ranks / cut.tiles / cut.parts;
   Scan<T, V, L, FORM, BACK, PASS> s(d, b, (int64_t)(tile * 32 + lane) * V);
+
+  if constexpr (PASS == kCluster) {
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&counted[i])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    cg::this_cluster().sync();
+  }
 
   // sequences without a step hand their entry state on
   if (PASS != kMaps && s.exit_state && rank == 0 && part == 0 && (d.sequences || d.length == 0)) {
@@ -406,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   Affine<V> whole{splat<V>(1.0f), splat<V>(0.0f)};  // the part's map so far
   bool whole_begins = false;
 
-  int parity = 0;
+  int parity = 0, phase = 0;  // of the exchange's buffers, and of their barriers
   const int from = (int)(part * cut.part_steps), to = (int)min(from + cut.part_steps, d.length);
   const int span = ranks * kWarps * L;
   // a part is a whole number of spans, so that no step belongs to two
@@ -433,7 +493,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
     maps[parity][warp][lane] = map;
     if (lane == 0) begins[parity][warp] = m.enters != 0;
     __syncthreads();
-    if (ranks > 1 || PASS == kMaps) {
+    if constexpr (PASS == kCluster || PASS == kMaps) {
       // this block's map
       Affine<V> block{splat<V>(1.0f), splat<V>(0.0f)};
       bool any = false;
@@ -444,22 +504,28 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
         any |= begun;
         block = {block.A * f.A, apply(f, begun, block.H)};
       }
-      if (PASS == kMaps) {
+      if constexpr (PASS == kMaps) {
         whole = {whole.A * block.A, apply(block, any, whole.H)};
         whole_begins |= any;
         m = next_m, first = next_first, all = next_all;
         continue;
       }
-      cg::cluster_group cluster = cg::this_cluster();
+      const unsigned barrier = shared_address(&counted[parity]);
+      if (threadIdx.x == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier),
+                     "r"(ranks * (32 * (int)sizeof(Affine<V>) + 4))
+                     : "memory");
       for (int r = warp; r < ranks; r += kWarps) {  // to every block of the cluster
-        cluster.map_shared_rank(&rank_maps[parity][rank][0], r)[lane] = block;
-        if (lane == 0) *cluster.map_shared_rank(&rank_begins[parity][rank], r) = any;
+        const unsigned there = of_rank(barrier, r);
+        send(of_rank(shared_address(&rank_maps[parity][rank][lane]), r), there, block);
+        if (lane == 0) send(of_rank(shared_address(&rank_begins[parity][rank]), r), there, (int)any);
       }
-      cluster.sync();
+      if (!arrived(barrier, phase)) carry = splat<V>(NAN);
+      phase ^= parity;
     }
     // the value carried into this warp's steps, and past all blocks' steps
     Vec<V> value = carry;
-    if (ranks > 1) {
+    if constexpr (PASS == kCluster) {
       for (int r = 0; r < ranks; ++r) {
         if (r == rank) value = carry;
         carry = apply(rank_maps[parity][r][lane], rank_begins[parity][r], carry);
@@ -568,17 +634,18 @@ int ranks_of(int64_t columns, int64_t spans) {
   return ranks;
 }
 // Into how many parts the time axis is cut, each part two launches' work: its map, then its
-// outputs.  1 where one launch fills the GPU and its clusters do not walk long: measured, 256
-// columns of 64 spans take 101 us in one launch and 146 cut, 96 of 16 spans 16 and 21; but 96
-// columns of 65 spans 46 and 38, 16 of 63 spans 25 and 13, 12 of 2048 spans 728 and 217.  Four
-// blocks run on a SM: parts that fill them once, or twice where that leaves long ones (12 columns:
-// 49 parts 176 us, 64 parts 217; 96 columns: 12 parts 39.8, 6 parts 43), and at least four spans
-// each, for every part reads the maps of those before it (one column of 256 spans: 64 parts 14.2 us,
-// 256 parts 21; of 2048 spans: 296 parts 37, 592 parts 47).
+// outputs.  1 where clusters bring two blocks to every SM, however long they walk, for a cut call
+// reads its inputs twice (256 columns of 64 spans: 80 us in one launch, 133 cut; 128 of 128 spans
+// 93 and 111; 48 of 65 spans 31 and 33), or where there is little to walk (16 columns of 16 spans: 8
+// and 8).  But 16 columns of 125 spans take 21 us in one launch and 16 cut, 32 of 128 spans 41 and 31,
+// 12 of 2048 spans 728 and 172.  Four blocks run on a SM: parts that fill them once, or twice where
+// that leaves long ones (12 columns: 49 parts 176 us, 64 parts 217; 96 columns: 12 parts 39.8, 6 parts
+// 43), and at least four spans each, for every part reads the maps of those before it (one column of
+// 256 spans: 64 parts 14.2 us, 256 parts 21; of 2048 spans: 296 parts 37, 592 parts 47).
 constexpr int64_t kMaxParts = 296;
 int parts_of(int64_t columns, int64_t spans) {
   const int ranks = ranks_of(columns, spans);
-  if (columns >= 148 || spans <= 2 * ranks || (columns * ranks >= 148 && spans <= 8 * ranks)) return 1;
+  if (columns * ranks >= 2 * 148 || spans <= 2 * ranks || (columns * ranks >= 148 && spans <= 8 * ranks)) return 1;
   const int64_t wave = 4 * 148 / columns, fill = wave >= 16 ? wave : 8 * 148 / columns;
   return (int)std::max<int64_t>(1, std::min({kMaxParts, (spans + 3) / 4, fill}));
 }
@@ -650,13 +717,20 @@ cudaError_t launch(const tb_scan_desc& d, const Cut& cut, cudaStream_t stream) {
   cfg.blockDim = dim3(kWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cut.ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  unsigned attrs = 0;
+  if (PASS == kCluster) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = cut.ranks;
+    attr[attrs].val.clusterDim.y = attr[attrs].val.clusterDim.z = 1;
+    ++attrs;
+  }
+  if (pdl_enabled()) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs].val.programmaticStreamSerializationAllowed = 1;
+    ++attrs;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  cfg.numAttrs = attrs;
   return cudaLaunchKernelEx(&cfg, k_scan<T, V, L, FORM, BACK, PASS>, d, cut);
 }
 
@@ -680,7 +754,8 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
     return e != cudaSuccess ? e : launch<T, V, L, FORM, BACK, kFromMaps>(d, cut, stream);
   }
   cut.ranks = ranks_of(columns, spans);
-  return launch<T, V, L, FORM, BACK, kWhole>(d, cut, stream);
+  return cut.ranks > 1 ? launch<T, V, L, FORM, BACK, kCluster>(d, cut, stream)
+                       : launch<T, V, L, FORM, BACK, kWhole>(d, cut, stream);
 }
 
 // Measured, 64 sequences of 2048 f32 channels: 8 steps 2.9 us short and 9.6 tiled, 16 steps 5.8 and
