@@ -99,9 +99,10 @@ class OperatorCall {
   int finish(cudaError_t e) const {
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e == cudaSuccess) return TB_OK;
-    // a handle of another device or none at all: nothing ran, and the device is well
-    if (e == cudaErrorInvalidResourceHandle || e == cudaErrorContextIsDestroyed)
+    // refused before anything ran, and the device is well
+    if (e == cudaErrorInvalidResourceHandle)
       return invalid("the stream is not one of the current device");
+    if (e == cudaErrorInvalidConfiguration) return invalid("more work than one launch takes");
     char text[256];
     snprintf(text, sizeof text, "%s: %s", name_, cudaGetErrorString(e));
     poison_library(text);
@@ -153,6 +154,31 @@ inline bool extents_fit(std::initializer_list<int64_t> extents) {
     product *= e > 0 ? (double)e : 1.0;
   }
   return product < (double)(int64_t(1) << 44);
+}
+
+// Whether rows of `inner` elements, counted along each axis and set `strides` apart, keep clear of
+// one another: along the axes by rising stride, each step passes all that the ones before reach.
+template <int N>
+inline bool rows_apart(int64_t inner, const int64_t (&counts)[N], const int64_t (&strides)[N]) {
+  int64_t count[N], stride[N];
+  int axes = 0;
+  for (int i = 0; i < N; ++i) {
+    if (counts[i] == 0) return true;
+    if (counts[i] == 1) continue;
+    int at = axes++;
+    for (; at > 0 && stride[at - 1] > strides[i]; --at) {
+      stride[at] = stride[at - 1];
+      count[at] = count[at - 1];
+    }
+    stride[at] = strides[i];
+    count[at] = counts[i];
+  }
+  double reach = (double)inner;  // sizes may pass 64 bits in a malformed request
+  for (int i = 0; i < axes; ++i) {
+    if ((double)stride[i] < reach) return false;
+    reach += (double)stride[i] * (double)(count[i] - 1);
+  }
+  return true;
 }
 
 }  // namespace tb

@@ -34,6 +34,10 @@ void need(bool condition, const char* why) {
 }
 void checked(int code, const char* entry) {
   if (code == TB_OK) return;
+  if (!g_backend_error) {
+    PyErr_Format(PyExc_RuntimeError, "%s: %s", entry, tb_last_error());
+    throw python_error();
+  }
   if (PyObject* error = PyObject_CallFunction(g_backend_error, "is", code, entry)) {
     PyErr_SetObject(g_backend_error, error);
     Py_DECREF(error);

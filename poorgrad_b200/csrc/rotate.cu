@@ -544,9 +544,7 @@ int64_t workspace_bytes(const tb_rotate_desc& d) {
 
 bool strides_ok(const tb_rotate_desc& d, const int64_t s[3], int64_t heads, bool written) {
   if (!extents_fit({s[0]}) || !extents_fit({s[1]}) || !extents_fit({s[2]})) return false;
-  if (!written) return true;
-  return (heads <= 1 || s[2] >= d.dim) && (d.length <= 1 || s[1] >= d.dim) &&
-         (d.batch <= 1 || s[0] >= d.dim);
+  return !written || rows_apart<3>(d.dim, {d.batch, d.length, heads}, {s[0], s[1], s[2]});
 }
 
 const char* check(const tb_rotate_desc& d, bool backward) {

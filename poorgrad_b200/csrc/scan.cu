@@ -652,8 +652,7 @@ int parts_of(int64_t columns, int64_t spans) {
 
 bool strides_ok(const tb_scan_desc& d, const int64_t s[2], bool written) {
   if (!extents_fit({s[0]}) || !extents_fit({s[1]})) return false;
-  if (!written) return true;
-  return (d.length <= 1 || s[1] >= d.channels) && (d.batch <= 1 || s[0] >= d.channels);
+  return !written || rows_apart<2>(d.channels, {d.batch, d.length}, {s[0], s[1]});
 }
 
 constexpr int64_t kMaxLength = INT32_MAX - (1 << 16);  // steps are counted in 32 bits, a span past the end

@@ -860,3 +860,172 @@ def test_wrappers_refuse_what_does_not_fit(device):
         with pytest.raises((ValueError, BackendError)) as error:
             call()
         assert not isinstance(error.value, BackendError) or error.value.code == 6, n
+
+
+# ------------------------------------------------- larger extents, other paths
+LONG = [(1, 3000, 64), (2, 2500, 34), (1, 20000, 3), (48, 700, 130), (160, 260, 40), (300, 40, 33),
+        (1, 700, 4099), (3, 2049, 67)]
+
+
+@pytest.mark.parametrize("dtype,form", [("f32", "direct"), ("bf16", "sigmoid")])
+@pytest.mark.parametrize("size", LONG)
+def test_scan_over_long_and_wide_arrays(device, dtype, form, size):
+    batch, length, channels = size
+    t, k = TYPES[dtype], PER_STEP[form]
+    gate, x, state = scan_inputs(201, form, dtype, *size)
+    h, final, m, fm = oc.scan(form, gate, x, state)
+    got, got_final = operators.gated_scan(cuda(gate, t), cuda(x, t), form=form, state=cuda(state))
+    n = steps_of(batch, length)
+    within(got, h, (k * n + k) * EPS * m + half_step(t) * h.abs(), "h")
+    within(got_final, final, (k * length + k) * EPS * fm, "final state")
+    # the entry state's own array as the final one, however the time axis is cut
+    s = cuda(state)
+    operators.gated_scan(cuda(gate, t), cuda(x, t), form=form, state=s, final_state=s)
+    within(s, final, (k * length + k) * EPS * fm, "carried state")
+    h = h.to(t).double()
+    dh = normal(203, *size).to(t).double()
+    expected, sizes = oc.scan_backward(form, dh, gate, x, h, state, state)
+    got = operators.gated_scan_backward(cuda(dh, t), cuda(gate, t), cuda(x, t), cuda(h, t), form=form,
+                                        state=cuda(state), dfinal=cuda(state))
+    for name, a, e, m, half in zip(("dgate", "dx", "dstate"), got, expected, sizes,
+                                   (half_step(t), half_step(t), 0.0)):
+        within(a, e, (k * length + 3 * k) * EPS * m + half * e.abs(), name)
+
+
+@pytest.mark.parametrize("dtype,form", [("f32", "sigmoid"), ("bf16", "direct")])
+@pytest.mark.parametrize("length,channels,count", [(5000, 72, 40), (5000, 3, 700), (700, 8200, 9),
+                                                   (2049, 330, 300), (900, 66, 900)])
+def test_long_packed_batches_keep_sequences_apart(device, dtype, form, length, channels, count):
+    t, k = TYPES[dtype], PER_STEP[form]
+    cuts = torch.randint(0, length + 1, (count - 1,), generator=torch.Generator().manual_seed(7))
+    offsets = [0] + sorted(cuts.tolist()) + [length]
+    gate, x, state = scan_inputs(211, form, dtype, 1, length, channels, count)
+    # what overflows or is undefined in one sequence stays there
+    ill = [i for i in range(count) if offsets[i + 1] > offsets[i]][1::5]
+    sane = torch.ones(length, dtype=torch.bool)
+    for i in ill:
+        x[0, offsets[i]] = float("inf") if i % 2 else float("nan")
+        sane[offsets[i]:offsets[i + 1]] = False
+    well = torch.tensor([i not in ill for i in range(count)])
+    h, final, m, fm = oc.scan(form, gate, x, state, offsets)
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    got, got_final = operators.gated_scan(cuda(gate[0], t), cuda(x[0], t), form=form,
+                                          state=cuda(state), offsets=off)
+    n = steps_of(1, length, offsets)[0]
+    tol = (k * n + k) * EPS * m[0] + half_step(t) * h[0].abs()
+    within(got[sane.cuda()], h[0, sane], tol[sane], "h")
+    within(got_final[well.cuda()], final[well], ((k * length + k) * EPS * fm)[well], "final state")
+    for i in ill:
+        assert not bool(got[offsets[i]].isfinite().any())
+    h = torch.where(sane[None, :, None], h, torch.zeros_like(h)).to(t).double()
+    dh = normal(213, 1, length, channels).to(t).double()
+    for i in ill:
+        dh[0, offsets[i + 1] - 1] = float("nan")
+    dfinal = normal(214, count, channels).float().double()
+    expected, sizes = oc.scan_backward(form, dh, gate, x, h, state, dfinal, offsets)
+    got = operators.gated_scan_backward(cuda(dh[0], t), cuda(gate[0], t), cuda(x[0], t),
+                                        cuda(h[0], t), form=form, state=cuda(state), offsets=off,
+                                        dfinal=cuda(dfinal))
+    for name, a, e, m in zip(("dgate", "dx"), got, expected, sizes):
+        within(a[sane.cuda()], e[0, sane], (k * length + 3 * k) * EPS * m[0, sane]
+               + half_step(t) * e[0, sane].abs(), name)
+    within(got[2][well.cuda()], expected[2][well], ((k * length + 3 * k) * EPS * sizes[2])[well], "dstate")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1027, 2048, 4101, 20011])
+def test_targets_at_every_place_of_a_row(device, dtype, vocab):
+    """The first and last elements, which lie before and behind the vectors of a row, and some vectors
+    in between, with rows that start at every place of 16 bytes."""
+    t = TYPES[dtype]
+    places = list(range(20)) + list(range(vocab - 20, vocab)) + list(range(500, 1000, 31))
+    rows = len(places)
+    logits, _ = loss_inputs(221, dtype, rows, vocab)
+    targets = torch.tensor(places)
+    old, ref, advantages, weights = policy_inputs(222, logits, targets, 1.0)
+    args = (cuda(targets, torch.int32), cuda(old), cuda(advantages), cuda(weights))
+    for shift in range(0, 8 if dtype == "bf16" else 4, 3):
+        z = torch.empty(rows * vocab + shift, dtype=t, device="cuda")[shift:].view(rows, vocab)
+        z.copy_(logits)
+        for into in (True, z):
+            got = operators.policy_loss(z, *args, clip_low=0.2, clip_high=0.25, gradient=into)
+            check_policy(logits, targets, old, advantages, weights, ref, 0, 1.0, t, got)
+    z = cuda(logits, t)
+    off = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device="cuda")
+    got = operators.preference_loss(z, args[0], off, cuda(ref), beta=0.3)
+    total, ratios, logp, grad, slope = oc.preference(logits, targets, off.tolist(), ref, 0.3, 0.0,
+                                                     torch.ones(1, dtype=torch.float64), 1.0)
+    bar, sum_bar = logp_bar(logits, targets, 1.0)
+    p = oc.rows(logits, targets, 1.0)[1]
+    off_by = torch.full((rows,), 0.3 * float((bar + EPS * (logp.abs() + 1)).sum()), dtype=torch.float64)
+    within(got.gradient, grad, gradient_bar(logits, p, slope.abs(), off_by, 1.0, sum_bar, t, grad), "gradient")
+
+
+@pytest.mark.parametrize("dtype,vocab", [("f32", 60007), ("f32", 130003), ("f32", 500009),
+                                         ("bf16", 60007), ("bf16", 130003), ("bf16", 500009)])
+def test_losses_over_large_vocabularies(device, dtype, vocab):
+    t, rows = TYPES[dtype], 6
+    logits, targets = loss_inputs(231, dtype, rows, vocab)
+    targets[1], targets[2] = 0, vocab - 1
+    old, ref, advantages, weights = policy_inputs(232, logits, targets, 1.0)
+    weights[3] = 0.0
+    logits[4] = -float("inf")
+    args = (cuda(targets, torch.int32), cuda(old), cuda(advantages), cuda(weights))
+    keep = torch.tensor([0, 1, 2, 3, 5])
+    z = cuda(logits, t)
+    got = operators.policy_loss(z, *args, clip_low=0.2, clip_high=0.25)
+    assert float(got.logp[4]) == 0 and bool((got.gradient[4] == 0).all())
+    sub = [v[keep] for v in (logits, targets, old, advantages, weights, ref)]
+    part = got._replace(token_loss=got.token_loss[keep.cuda()], logp=got.logp[keep.cuda()],
+                        gradient=got.gradient[keep.cuda()])
+    check_policy(*sub, 0, 1.0, t, part)
+    over = operators.policy_loss(z, *args, clip_low=0.2, clip_high=0.25, gradient=z)
+    assert torch.equal(over.gradient, got.gradient)
+
+
+def test_many_pairs(device):
+    rows, vocab, pairs = 3000, 40, 400
+    logits, targets = loss_inputs(241, "f32", rows, vocab)
+    cuts = torch.randint(0, rows + 1, (2 * pairs - 1,), generator=torch.Generator().manual_seed(3))
+    offsets = [0] + sorted(cuts.tolist()) + [rows]
+    ref = (oc.rows(logits, targets, 1.0)[0] + 0.2 * normal(242, rows)).float().double()
+    w = torch.full((pairs,), 1 / pairs, dtype=torch.float64)
+    total, ratios, logp, grad, slope = oc.preference(logits, targets, offsets, ref, 0.1, 0.0, w, 1.0)
+    got = operators.preference_loss(cuda(logits), cuda(targets, torch.int32),
+                                    torch.tensor(offsets, dtype=torch.int32, device="cuda"), cuda(ref))
+    bar, sum_bar = logp_bar(logits, targets, 1.0)
+    each = bar + EPS * (logp.abs() + 1)
+    cut = torch.stack([each[lo:hi].sum() for lo, hi in zip(offsets[:-1], offsets[1:])])
+    within(got.ratios, ratios, cut + EPS * ratios.abs(), "ratios")
+    within(got.loss, total, 0.1 * cut.sum() / pairs + 8 * EPS * total.abs(), "loss")
+    p = oc.rows(logits, targets, 1.0)[1]
+    off_by = torch.full((rows,), 0.1 * float(cut.max()) / pairs * 2 + EPS, dtype=torch.float64)
+    within(got.gradient, grad, gradient_bar(logits, p, slope.abs(), off_by, 1.0, sum_bar,
+                                            torch.float32, grad), "gradient")
+
+
+def test_rotate_over_many_tokens(device):
+    """Warps that take several tokens, weight gradients summed over blocks."""
+    q, k, wq, wk, _, _ = rotate_inputs(251, "bf16", 3, 1500, 5, 2, 64, 64)
+    table = oc.table(2000, 64)
+    positions = torch.randint(0, 2000, (3, 1500), generator=torch.Generator().manual_seed(5))
+    t = torch.bfloat16
+    named = dict(q_weight=cuda(wq), k_weight=cuda(wk))
+    pos = cuda(positions, torch.int32)
+    got = operators.head_rotate(cuda(q, t), cuda(k, t), cuda(table), pos, **named)
+    dq, dk = (normal(255 + i, *v.shape).to(t).double() for i, v in enumerate((q, k)))
+    back = operators.head_rotate_backward(cuda(dq, t), cuda(dk, t), cuda(q, t), cuda(k, t),
+                                          cuda(table), pos, **named)
+    for i, (x, w, dy) in enumerate(((q, wq, dq), (k, wk, dk))):
+        e = oc.rotate(x, w, table.double(), positions, 1e-5, "halves")
+        within(got[i], e, rotate_bar(x, w, e, t), "rotate")
+        dx, dw, size_w = oc.rotate_backward(dy, x, w, table.double(), positions, 1e-5, "halves")
+        heads = x.shape[0] * x.shape[1] * x.shape[2]
+        big = float(oc.turn(dy, table.double(), positions, "halves", True).abs().amax())
+        # a lane adds heads / (8 * 148) terms, then 3 shuffles, 8 warps and 37 + 8 blocks
+        within(back[2 + i], dw, EPS * ((heads / 1000 + 80) * size_w + 8 * heads * big), "weight gradient")
+        r = 1 / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-5)
+        dn = oc.turn(dy, table.double(), positions, "halves", True) * w
+        inner = (dn * x * r).abs().mean(-1, keepdim=True)
+        bar = 192 * EPS * r * (dn.abs().amax(-1, keepdim=True) + (x * r).abs().amax(-1, keepdim=True) * inner)
+        within(back[i], dx, bar + half_step(t) * dx.abs(), "dx")

@@ -91,6 +91,7 @@ REFUSED = (
         dict(gate=0), dict(x=0), dict(h=0), dict(gate=257), dict(state=258),
         dict(sequences=1, batch=1), dict(offsets=256), dict(sequences=1, offsets=256),
         dict(gate_strides=[-1, 4]), dict(h_strides=[12, 3]), dict(h_strides=[0, 4]),
+        dict(h_strides=[4, 4]), dict(h_strides=[8, 4]), dict(h_strides=[4, 7]),
         dict(batch=1 << 40, length=1 << 30), dict(x_strides=[1 << 62, 4]))]
     + [("tb_gated_scan_backward", scan_request(**c)) for c in (
         dict(dh=0), dict(dgate=0), dict(dx=0), dict(dgate_strides=[12, 1]),
@@ -99,7 +100,8 @@ REFUSED = (
         dict(element=5), dict(style=2), dict(dim=7), dict(dim=514), dict(turned=10),
         dict(turned=3), dict(turned=-2), dict(epsilon=-1.0), dict(epsilon=NAN), dict(q=0),
         dict(k_out=0), dict(table=0), dict(table=2), dict(length=-1), dict(q_heads=-1),
-        dict(q_out_strides=[32, 16, 4]), dict(k_out_strides=[32, 0, 8]), dict(q=254),
+        dict(q_out_strides=[32, 16, 4]), dict(k_out_strides=[32, 0, 8]),
+        dict(q_out_strides=[0, 8, 8]), dict(q_out_strides=[0, 8, 15]), dict(q=254),
         dict(q_weight=1))]
     + [("tb_head_rotate_backward", rotate_request(**c)) for c in (
         dict(dq=0), dict(dq_weight=256), dict(dq_weight=256, workspace=256, workspace_bytes=8),
@@ -139,6 +141,8 @@ def test_entry_points_without_a_request(built):
 def test_well_formed_requests_without_a_device(built):
     lib = abi.load_library()
     for entry, request in (("tb_gated_scan", scan_request()),
+                           ("tb_gated_scan", scan_request(h_strides=[4, 8])),
+                           ("tb_head_rotate", rotate_request(q_out_strides=[0, 8, 16])),
                            ("tb_gated_scan_backward", scan_request()),
                            ("tb_head_rotate", rotate_request()),
                            ("tb_head_rotate_backward", rotate_request()),
