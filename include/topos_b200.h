@@ -336,7 +336,8 @@ typedef struct tb_scan_desc {
   int64_t element, form;
   int64_t batch, length, channels;  /* arrays [batch][length][channels] */
   int64_t sequences;                /* packed sequences in a batch of 1, or 0: each batch row is one */
-  /* (batch, time) strides of gate, x, h, dh, dgate, dx; unused ones are ignored */
+  /* (batch, time) strides of gate, x, h, dh, dgate, dx, the latter below 2^29; unused ones are
+   * ignored */
   int64_t gate_strides[2], x_strides[2], h_strides[2], dh_strides[2], dgate_strides[2], dx_strides[2];
   const void* gate;
   const void* x;
