@@ -666,8 +666,13 @@ cudaError_t enqueue(tb_rotate_desc d, bool backward, cudaStream_t stream) {
   };
   side(sides.q, d.q, d.dq, d.q_out, d.q_weight, d.q_strides, d.dq_strides, d.q_out_strides, d.q_heads);
   side(sides.k, d.k, d.dk, d.k_out, d.k_weight, d.k_strides, d.dk_strides, d.k_out_strides, d.k_heads);
-  constexpr int kVec = 16 / sizeof(T);
-  if (vectors_fit<T, kVec>(d, sides, backward)) return enqueue_vectors<T, kVec>(d, sides, backward, stream);
+  constexpr int kVec = 16 / sizeof(T), kHalf = kVec == 8 ? 4 : kVec;
+  // Small bf16 heads spread over twice the lanes, with fewer registers each: 8 x 1024 tokens x 24 heads
+  // of 64 backwards 21.8 us in 8-byte lanes and 24.7 in 16-byte ones (of 96: 41.5 and 39.7), x 32
+  // heads of 32 forwards 10.5 and 12.2 (24 of 64: 13.5 and 13.4).
+  const bool spread = kVec == 8 && d.dim <= (backward ? 64 : 32) && vectors_fit<T, kHalf>(d, sides, backward);
+  if (!spread && vectors_fit<T, kVec>(d, sides, backward))
+    return enqueue_vectors<T, kVec>(d, sides, backward, stream);
   if constexpr (kVec == 8)
     if (vectors_fit<T, 4>(d, sides, backward)) return enqueue_vectors<T, 4>(d, sides, backward, stream);
   if (vectors_fit<T, 1>(d, sides, backward)) return enqueue_vectors<T, 1>(d, sides, backward, stream);
