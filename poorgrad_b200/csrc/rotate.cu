@@ -337,7 +337,32 @@ __global__ void __launch_bounds__(256, 3) k_rotate_vectors(tb_rotate_desc d, Sid
 
 constexpr int64_t kBackwardBlocks = 2 * 148;  // of each side, at most: rows of partials
 
-// The same division of work; a lane holds its part of the weight gradient in registers.
+// A lane's copy of one vector into its own place in shared memory.
+template <typename Raw>
+__device__ __forceinline__ void copy_own(Raw* to, const Raw* from) {
+  if constexpr (sizeof(Raw) == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
+  else if constexpr (sizeof(Raw) >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)),
+                 "l"(from), "n"((int)sizeof(Raw))
+                 : "memory");
+  else
+    *to = *from;
+}
+
+// The same division of work; a lane holds its part of the weight gradient in registers.  That and the
+// two rows of every head leave sixteen warps to a SM, too few to wait for their rows by turns, so
+// where a lane holds 8 elements of a vector it copies those of its next items into its own places in
+// shared memory (40 heads of 128 in bf16: 56 us without, 49 with; 24 heads of 64 in f32, where four
+// sets fit the registers: 31 without, 45 with).
+constexpr int kCopies = 3;  // items a lane has under way
+template <int VEC>
+constexpr bool kCopied = VEC == 8;
+// Shared memory of a block: the places, then (or alone) its warps' sums of the weight gradient.
+template <typename Raw, int VEC, int G, int UNROLL>
+constexpr size_t kBackwardBytes = kCopied<VEC> ? (size_t)kCopies * UNROLL * 4 * 256 * sizeof(Raw)
+                                               : (size_t)8 * 2 * ((VEC + 1) / 2) * G * sizeof(float2);
 template <typename T, int VEC, int G, bool ADJACENT, int UNROLL>
 __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_desc d, Sides sides,
                                                                     int q_blocks) {
@@ -345,7 +370,6 @@ __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_de
   typedef Part<T, VEC, ADJACENT> P;
   typedef typename P::Raw Raw;
   constexpr int kRows = 32 / G, kWarps = 8, N = (VEC + 1) / 2;
-  __shared__ float2 sums[kWarps][2 * N][G];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, chunk = lane % G;
   const bool key = (int)blockIdx.x >= q_blocks;
   const Side& side = key ? sides.k : sides.q;
@@ -357,36 +381,74 @@ __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_de
 #pragma unroll
   for (int j = 0; j < N; ++j) du[j] = dv[j] = both(0.0f);
   const unsigned items = (unsigned)sides.tokens * side.blocks;
+  extern __shared__ uint4 places[];
+  [[maybe_unused]] const auto place = [&](int copy, int h, int which) -> Raw& {
+    return ((Raw*)places)[((copy * UNROLL + h) * 4 + which) * 256 + threadIdx.x];
+  };
+  const unsigned step = of * kWarps;
+  [[maybe_unused]] const auto fetch = [&](int copy, unsigned at) {
+    if (at < items) {
+      const Item item(d, side, at, kRows * UNROLL);
+      const int head0 = item.from + lane / G;
+      const T* x = (const T*)side.in + item.offset(side.in_s, head0);
+      const T* dy = (const T*)side.grad + item.offset(side.grad_s, head0);
+#pragma unroll
+      for (int h = 0; h < UNROLL; ++h)
+        if (part.in && head0 + h * kRows < side.heads) {
+          const T *row = x + h * kRows * side.in_s[2], *grad = dy + h * kRows * side.grad_s[2];
+          copy_own(&place(copy, h, 0), (const Raw*)(row + part.first));
+          copy_own(&place(copy, h, 1), (const Raw*)(row + part.second));
+          copy_own(&place(copy, h, 2), (const Raw*)(grad + part.first));
+          copy_own(&place(copy, h, 3), (const Raw*)(grad + part.second));
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   unsigned i = mine * kWarps + warp;
+  if constexpr (kCopied<VEC>)
+#pragma unroll
+    for (int copy = 0; copy < kCopies - 1; ++copy) fetch(copy, i + copy * step);
   int position = i < items ? Item(d, side, i, kRows * UNROLL).position(d) : 0;
-  for (; i < items; i += of * kWarps) {
+  int now = 0;
+  for (; i < items; i += step) {
     const Item item(d, side, i, kRows * UNROLL);
     const int from = item.from, head0 = from + lane / G;
-    const T* x = (const T*)side.in + item.offset(side.in_s, head0);
-    const T* dy = (const T*)side.grad + item.offset(side.grad_s, head0);
-    T* dx = (T*)side.out + item.offset(side.out_s, head0);
-    Raw r1[UNROLL], r2[UNROLL], g1[UNROLL], g2[UNROLL];
+    Raw held[kCopied<VEC> ? 1 : UNROLL][4];
+    if constexpr (kCopied<VEC>) {
+      fetch(now == 0 ? kCopies - 1 : now - 1, i + (kCopies - 1) * step);
+    } else {
+      const T* x = (const T*)side.in + item.offset(side.in_s, head0);
+      const T* dy = (const T*)side.grad + item.offset(side.grad_s, head0);
 #pragma unroll
-    for (int h = 0; h < UNROLL; ++h) {
-      r1[h] = r2[h] = g1[h] = g2[h] = Raw{};
-      if (part.in && head0 + h * kRows < side.heads) {
-        const T *row = x + h * kRows * side.in_s[2], *grad = dy + h * kRows * side.grad_s[2];
-        r1[h] = *(const Raw*)(row + part.first);
-        r2[h] = *(const Raw*)(row + part.second);
-        g1[h] = *(const Raw*)(grad + part.first);
-        g2[h] = *(const Raw*)(grad + part.second);
+      for (int h = 0; h < UNROLL; ++h) {
+        held[h][0] = held[h][1] = held[h][2] = held[h][3] = Raw{};
+        if (part.in && head0 + h * kRows < side.heads) {
+          const T *row = x + h * kRows * side.in_s[2], *grad = dy + h * kRows * side.grad_s[2];
+          held[h][0] = *(const Raw*)(row + part.first);
+          held[h][1] = *(const Raw*)(row + part.second);
+          held[h][2] = *(const Raw*)(grad + part.first);
+          held[h][3] = *(const Raw*)(grad + part.second);
+        }
       }
     }
+    T* dx = (T*)side.out + item.offset(side.out_s, head0);
     float2 cosine[N], sine[N];
     part.angles(d, position, chunk, cosine, sine);
-    if (i + of * kWarps < items) position = Item(d, side, i + of * kWarps, kRows * UNROLL).position(d);
+    if (i + step < items) position = Item(d, side, i + step, kRows * UNROLL).position(d);
+    if constexpr (kCopied<VEC>) asm volatile("cp.async.wait_group %0;" ::"n"(kCopies - 1) : "memory");
 #pragma unroll
     for (int h = 0; h < UNROLL; ++h) {
       if (from + h * kRows >= side.heads) break;
       const bool here = part.in && head0 + h * kRows < side.heads;
       float2 u[N], v[N], gu[N], gv[N];
-      part.read(r1[h], r2[h], u, v);
-      part.read(g1[h], g2[h], gu, gv);
+      Raw raw[4] = {};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (!kCopied<VEC>) raw[w] = held[h][w];
+        else if (here) raw[w] = place(now, h, w);
+      }
+      part.read(raw[0], raw[1], u, v);
+      part.read(raw[2], raw[3], gu, gv);
       const float scale = rsqrtf(group_sum<G>(squares_of(u, v)) * share + epsilon);
       float2 inner = both(0.0f);
 #pragma unroll
@@ -417,6 +479,7 @@ __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_de
         *(Raw*)(row + part.second) = o2;
       }
     }
+    now = now + 1 == kCopies ? 0 : now + 1;
   }
   if (!d.workspace) return;
   // lanes of one chunk, then the warps, in a fixed order; the elements in their places
@@ -429,6 +492,10 @@ __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_de
     }
   }
   if (ADJACENT) P::joined(du, dv);
+  typedef float2 Sums[2 * N][G];
+  Sums* sums = (Sums*)places;  // [warps], where the copies were
+  static_assert(kWarps * sizeof(Sums) <= kBackwardBytes<Raw, VEC, G, UNROLL>);
+  __syncthreads();
   if (lane < G)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -609,7 +676,7 @@ cudaError_t enqueue_weights(const tb_rotate_desc& d, int64_t q_blocks, int64_t b
 
 template <typename T, int VEC, int G, bool ADJACENT>
 cudaError_t enqueue_vectors(const tb_rotate_desc& d, Sides sides, bool backward, cudaStream_t stream) {
-  // sets of heads a warp takes in one go: as many loads as its registers hold
+  // sets of heads a warp takes in one go: as many loads as its registers or places hold
   constexpr int kUnroll = VEC == 8 ? 2 : 4;
   const int kHeads = 32 / G * kUnroll;
   sides.q.blocks = (sides.q.heads + kHeads - 1) / kHeads;
@@ -624,9 +691,13 @@ cudaError_t enqueue_vectors(const tb_rotate_desc& d, Sides sides, bool backward,
   if (!backward)
     return launch_pdl(k_rotate_vectors<T, VEC, G, ADJACENT, kUnroll>,
                       dim3((unsigned)(q_blocks + k_blocks)), dim3(256), 0, stream, d, sides, (int)q_blocks);
-  cudaError_t e = launch_pdl(k_rotate_vectors_backward<T, VEC, G, ADJACENT, kUnroll>,
-                             dim3((unsigned)(q_blocks + k_blocks)), dim3(256), 0, stream, d, sides,
-                             (int)q_blocks);
+  constexpr size_t kShared = kBackwardBytes<typename Chunk<T, VEC>::type, VEC, G, kUnroll>;
+  const auto kernel = k_rotate_vectors_backward<T, VEC, G, ADJACENT, kUnroll>;
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use that much
+  cudaError_t e = allow_shared((const void*)kernel, kShared, allowed);
+  if (e == cudaSuccess)
+    e = launch_pdl(kernel, dim3((unsigned)(q_blocks + k_blocks)), dim3(256), kShared, stream, d, sides,
+                   (int)q_blocks);
   return e == cudaSuccess && d.workspace ? enqueue_weights(d, q_blocks, q_blocks + k_blocks, stream) : e;
 }
 
