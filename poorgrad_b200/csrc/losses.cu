@@ -716,14 +716,20 @@ bool words_ok(std::initializer_list<const void*> arrays) {
   return true;
 }
 
-// Threads of a block that streams a row: some 8 vectors a thread.
+// Threads of a block that reads a row, or reads and writes one.  Reading, many small blocks hide one
+// another's ends (8192 x 50257 bf16: 102 us with 256 threads, 123 with 512); reading and writing, few
+// large ones keep to the rows that lie side by side (4099 x 50257 f32: 512 threads 320 us, 256 332).
 template <typename T>
-int threads_of(int64_t vocab) {
+int reading_threads(int64_t vocab) {
+  return vocab * (int64_t)sizeof(T) / 16 > 1024 ? 256 : 128;
+}
+template <typename T>
+int writing_threads(int64_t vocab) {
   const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
   return vectors > 4096 ? 512 : vectors > 1024 ? 256 : 128;
 }
-#define TB_BY_THREADS(KERNEL, ...)                                                                 \
-  switch (threads_of<T>(vocab)) {                                                                  \
+#define TB_BY_THREADS(THREADS, KERNEL, ...)                                                         \
+  switch (THREADS) {                                                                                \
     case 512: return launch_pdl(KERNEL<T, 512>, dim3((unsigned)rows), dim3(512), 0, stream, __VA_ARGS__); \
     case 256: return launch_pdl(KERNEL<T, 256>, dim3((unsigned)rows), dim3(256), 0, stream, __VA_ARGS__); \
     default: return launch_pdl(KERNEL<T, 128>, dim3((unsigned)rows), dim3(128), 0, stream, __VA_ARGS__);  \
@@ -744,7 +750,7 @@ cudaError_t enqueue_logp(const T* logits, int64_t stride, const int32_t* targets
                          float scale, float* logp, cudaStream_t stream) {
   if (vocab <= kWarpVocab)
     TB_BY_ITEMS(k_token_logp_warps, logits, stride, targets, rows, vocab, scale, logp)
-  TB_BY_THREADS(k_token_logp, logits, stride, targets, vocab, scale, logp)
+  TB_BY_THREADS(reading_threads<T>(vocab), k_token_logp, logits, stride, targets, vocab, scale, logp)
 }
 
 template <typename T, int THREADS>
@@ -773,7 +779,7 @@ template <typename T>
 cudaError_t enqueue_policy(const tb_policy_desc& d, cudaStream_t stream) {
   const int64_t rows = d.rows, vocab = d.vocab;
   if (vocab <= kWarpVocab) TB_BY_ITEMS(k_policy_warps, d)
-  if (!d.gradient) TB_BY_THREADS(k_policy_terms, d)
+  if (!d.gradient) TB_BY_THREADS(reading_threads<T>(vocab), k_policy_terms, d)
   const int64_t vectors = vocab * (int64_t)sizeof(T) / 16;
   // one block a row while it holds one (8192 x 16000 bf16: 256 threads 111 us, two blocks of 128
   // 130), else the smallest blocks whose clusters do (8192 x 50257 f32: 8 blocks of 128 threads
@@ -792,14 +798,14 @@ template <typename T>
 cudaError_t enqueue_preference_rows(const tb_preference_desc& d, cudaStream_t stream) {
   const int64_t rows = d.rows, vocab = d.vocab;
   if (vocab <= kWarpVocab) TB_BY_ITEMS(k_preference_rows_warps, d)
-  TB_BY_THREADS(k_preference_rows, d)
+  TB_BY_THREADS(reading_threads<T>(vocab), k_preference_rows, d)
 }
 template <typename T>
 cudaError_t enqueue_preference_gradient(const tb_preference_desc& d, cudaStream_t stream) {
   const int64_t rows = d.rows, vocab = d.vocab;
   if (vocab <= kWarpVocab)
     return launch_pdl(k_preference_gradient_warps<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, d);
-  TB_BY_THREADS(k_preference_gradient, d)
+  TB_BY_THREADS(writing_threads<T>(vocab), k_preference_gradient, d)
 }
 
 int token_logp(int64_t element, const void* logits, int64_t stride, const int32_t* targets,

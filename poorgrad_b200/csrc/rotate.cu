@@ -517,24 +517,23 @@ __global__ void __launch_bounds__(256, 2) k_rotate_vectors_backward(tb_rotate_de
   }
 }
 
-// Weight gradients: the blocks' partials in their order, 8 threads an element.
-__global__ void __launch_bounds__(256) k_rotate_weights(tb_rotate_desc d, int q_blocks, int blocks) {
+// Weight gradients: the blocks' partials in a fixed order, 32 threads an element.
+__global__ void __launch_bounds__(1024) k_rotate_weights(tb_rotate_desc d, int q_blocks, int blocks) {
   pdl_entry();
-  __shared__ float sums[8][32];
-  const int dim = (int)d.dim, per_side = (dim + 31) / 32;
+  __shared__ float sums[32][33];
+  const int dim = (int)d.dim, per_side = (dim + 31) / 32, lane = threadIdx.x % 32, row = threadIdx.x / 32;
   const bool key = (int)blockIdx.x >= per_side;
-  const int j = (blockIdx.x - (key ? per_side : 0)) * 32 + threadIdx.x % 32, row = threadIdx.x / 32;
+  const int first = (blockIdx.x - (key ? per_side : 0)) * 32, j = first + lane;
   const int from = key ? q_blocks : 0, to = key ? blocks : q_blocks;
   float s = 0;
   if (j < dim)
-    for (int b = from + row; b < to; b += 8) s += ((const float*)d.workspace)[(int64_t)b * dim + j];
-  sums[row][threadIdx.x % 32] = s;
+#pragma unroll 8
+    for (int b = from + row; b < to; b += 32) s += ((const float*)d.workspace)[(int64_t)b * dim + j];
+  sums[row][lane] = s;
   __syncthreads();
+  s = warp_sum(sums[lane][row]);  // element `row` of this block's 32
   float* out = key ? d.dk_weight : d.dq_weight;
-  if (row == 0 && j < dim && out) {
-    for (int r = 1; r < 8; ++r) s += sums[r][threadIdx.x];
-    out[j] = s;
-  }
+  if (lane == 0 && first + row < dim && out) out[first + row] = s;
 }
 
 // ---- any other head: a warp each
@@ -670,7 +669,7 @@ bool vectors_fit(const tb_rotate_desc& d, const Sides& sides, bool backward) {
 }
 
 cudaError_t enqueue_weights(const tb_rotate_desc& d, int64_t q_blocks, int64_t blocks, cudaStream_t stream) {
-  return launch_pdl(k_rotate_weights, dim3((unsigned)(2 * ((d.dim + 31) / 32))), dim3(256), 0, stream,
+  return launch_pdl(k_rotate_weights, dim3((unsigned)(2 * ((d.dim + 31) / 32))), dim3(1024), 0, stream,
                     d, (int)q_blocks, (int)blocks);
 }
 
