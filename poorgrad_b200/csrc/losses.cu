@@ -43,6 +43,7 @@ struct Vector;
 template <>
 struct Vector<float> {
   static constexpr int kPairs = 2;
+  static __device__ __forceinline__ uint4 nothing() { return {0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
   static __device__ __forceinline__ void read(uint4 r, float2 (&v)[2]) {
     v[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
     v[1] = {__uint_as_float(r.z), __uint_as_float(r.w)};
@@ -59,6 +60,7 @@ struct Vector<float> {
 template <>
 struct Vector<bf16> {
   static constexpr int kPairs = 4;
+  static __device__ __forceinline__ uint4 nothing() { return {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
   static __device__ __forceinline__ void read(uint4 r, float2 (&v)[4]) {
     v[0] = unpack_bf16(r.x);
     v[1] = unpack_bf16(r.y);
@@ -134,23 +136,23 @@ struct RowShare {
   __device__ __forceinline__ int64_t element(int64_t vector) const { return head + (first + vector) * kVec; }
 };
 
-// The statistics of all threads, in a fixed order; every thread gets them.
-template <int THREADS>
-__device__ __forceinline__ RowStats block_stats(RowStats s, float k) {
-  __shared__ RowStats part[THREADS / 32];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, k);
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
-  __syncthreads();
-  s = part[threadIdx.x % (THREADS / 32)];
-#pragma unroll
-  for (int o = THREADS / 64; o > 0; o >>= 1)
+__device__ __forceinline__ RowStats warp_stats(RowStats s, float k, int lanes = 32) {
+  for (int o = lanes / 2; o > 0; o >>= 1)
     s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, k);
   return s;
 }
+// The statistics of all threads, in a fixed order; the first warp gets them (what follows is one
+// thread's work, and on small blocks a good part of all if every thread does it).
+template <int THREADS>
+__device__ __forceinline__ RowStats block_stats(RowStats s, float k) {
+  __shared__ RowStats part[THREADS / 32];
+  s = warp_stats(s, k);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
+  __syncthreads();
+  return threadIdx.x < 32 ? warp_stats(part[threadIdx.x % (THREADS / 32)], k, THREADS / 32) : s;
+}
 
-// Statistics of a row straight from memory.
+// Statistics of a row straight from memory, for the first warp.
 template <typename T, int THREADS>
 __device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k) {
   constexpr int kAtOnce = 4;
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(THREADS) k_token_logp(const T* logits, int64_t
   if (t >= 0) {
     const T* z = logits + n * stride;
     const RowStats s = row_stats<T, THREADS>(z, vocab, scale * kLog2e);
-    if (s.sum != 0.0f) out = t < vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+    if (threadIdx.x == 0 && s.sum != 0.0f) out = t < vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) logp[n] = out;
 }
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
   if (t >= 0 && in.weight != 0.0f) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     const RowStats s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
-    if (s.sum != 0.0f) {
+    if (threadIdx.x == 0 && s.sum != 0.0f) {
       logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
@@ -346,14 +348,11 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
   const int each = (keep + kGroups - 1) / kGroups, count = (int)row.count;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
-      const int i = j * THREADS + threadIdx.x;
-      if (i < count)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         (unsigned)__cvta_generic_to_shared(kept + i)),
-                     "l"(from + i)
-                     : "memory");
-    }
+    const int last = min(count, min(keep, (g + 1) * each) * THREADS);
+    for (int i = g * each * THREADS + threadIdx.x; i < last; i += THREADS)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(kept + i)),
+                   "l"(from + i)
+                   : "memory");
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
@@ -366,12 +365,11 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
     if (g == 1) asm volatile("cp.async.wait_group 2;" ::: "memory");
     if (g == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     if (g == 3) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    for (int j = g * each; j < min(keep, (g + 1) * each); ++j) {
-      const int i = j * THREADS + threadIdx.x;
-      if (i < count) {
-        const uint4 r[1] = {kept[i]};
-        add<T>(s, r, k);
-      }
+    // by twos, so that they share a rescaling; one past the end is -inf, whose share is 0
+    const int last = min(count, min(keep, (g + 1) * each) * THREADS);
+    for (int i = g * each * THREADS + threadIdx.x; i < last; i += 2 * THREADS) {
+      const uint4 r[2] = {kept[i], i + THREADS < last ? kept[i + THREADS] : Vector<T>::nothing()};
+      add<T>(s, r, k);
     }
   }
   s = block_stats<THREADS>(s, k);
@@ -379,25 +377,33 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
     cg::cluster_group cluster = cg::this_cluster();
     if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&parts[rank], threadIdx.x) = s;
     cluster.sync();
-    s = parts[0];
-    for (int r = 1; r < ranks; ++r) s = merge(s, parts[r], k);
   }
-  float logp = 0.0f;
-  Term term{0.0f, 0.0f};
-  const bool hidden = s.sum == 0.0f;
-  if (!hidden) {
-    logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
-    term = policy_term(d, in, logp);
+  __shared__ RowStats whole;
+  __shared__ float slope;
+  if (threadIdx.x < 32) {
+    const RowStats none{-INFINITY, 0.0f};
+    if (ranks > 1) s = warp_stats((int)threadIdx.x < ranks ? parts[threadIdx.x] : none, k, 8);
+    if (threadIdx.x == 0) {
+      float logp = 0.0f;
+      Term term{0.0f, 0.0f};
+      if (s.sum != 0.0f) {
+        logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
+        term = policy_term(d, in, logp);
+      }
+      if (rank == 0) {
+        d.logp[n] = logp;
+        d.token_loss[n] = term.loss;
+      }
+      whole = s;
+      slope = term.slope;
+    }
   }
-  if (rank == 0 && threadIdx.x == 0) {
-    d.logp[n] = logp;
-    d.token_loss[n] = term.loss;
-  }
-  if (hidden) {
+  __syncthreads();
+  if (whole.sum == 0.0f) {
     zero_row<T, THREADS>(out, z, row);
     return;
   }
-  const RowGradient<T> g(out, z, s, scale, term.slope, t);
+  const RowGradient<T> g(out, z, whole, scale, slope, t);
   if (row.single >= 0) g.single(single, row.single);
   if (g.whole) {
     uint4* to = (uint4*)(out + row.element(0));
@@ -419,23 +425,25 @@ __global__ void __launch_bounds__(THREADS) k_policy_twice(tb_policy_desc d) {
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
   const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
+  __shared__ RowStats whole;
+  __shared__ float slope;
   RowStats s{0.0f, 0.0f};
-  float logp = 0.0f;
-  Term term{0.0f, 0.0f};
-  if (t >= 0 && in.weight != 0.0f) {
-    s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
+  if (t >= 0 && in.weight != 0.0f) s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
+  if (threadIdx.x == 0) {
+    float logp = 0.0f;
+    Term term{0.0f, 0.0f};
     if (s.sum != 0.0f) {
       logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
-  }
-  __syncthreads();  // the gradient may overwrite the logits that others still read
-  if (threadIdx.x == 0) {
     d.logp[n] = logp;
     d.token_loss[n] = term.loss;
+    whole = s;
+    slope = term.slope;
   }
-  if (s.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
-  else stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, scale, term.slope, t));
+  __syncthreads();  // the gradient may overwrite the logits that others still read
+  if (whole.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
+  else stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, whole, scale, slope, t));
 }
 
 // ---- small vocabularies: a warp a row, ITEMS logits a lane in registers
@@ -565,7 +573,7 @@ __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc 
   if (t >= 0) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
-    if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+    if (threadIdx.x == 0 && s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) {
     PreferenceScratch(d).stats[n] = s;
