@@ -4,7 +4,14 @@
 // With p = softmax(scale z) and L = scale z_t - lse, every loss reaches the logits through L
 // alone: dz_v = c scale (1[v = t] - p_v) with c = d loss / d L of the row.  Maxima are taken of
 // the raw logits and scale multiplies differences from them, so masks of the type's lowest
-// value do not overflow.
+// value do not overflow.  The statistics of a row are a running maximum and sum of exponentials.
+//
+// Measured on B200 (against a copy's 6.55 TB/s): the policy loss with its gradient over 8192 x 50257
+// logits, a quarter of the rows hidden, f32 472 us, 6.1 TB/s, bf16 267 us, 5.4 TB/s; the log
+// probabilities alone f32 180 us, bf16 102 us, 6.0 TB/s.  Memory bounds the f32 forms (under load the
+// power cap too: 490 to 540 us in a long run), issue slots and the two exponentials a logit the bf16
+// ones.  The preference loss cannot know a row's slope before its pair's last row, and rows of a pair
+// do not fit the chip: it reads the logits twice, 4099 x 50257 bf16 in 181 us, 988 MB at 5.5 TB/s.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -1,5 +1,17 @@
 // rotate.cu -- the root-mean-square norm of every query and key head with the rotation by the
 // token's position, and its backward pass.
+//
+// With n = x / sqrt(mean(x^2) + eps) and z = w n, each turned pair (u, v) of z becomes
+// (u c - v s, v c + u s).  Back: dz is dy turned by -s, dw = sum dz n over tokens and heads, and
+// dx = (w dz - n mean(w dz n)) / sqrt(mean(x^2) + eps); the norm is worked out again from x, so that
+// nothing is kept from the forward pass.  Every row is read once and written once.
+//
+// Measured on B200 (against a copy's 6.55 TB/s): 8 x 1024 tokens x (32 + 8) heads of 128 in bf16
+// forward 31 us, 5.4 TB/s, backward 50 us, 5.0 TB/s; (12 + 12) heads of 64 in f32 backward 29 us,
+// 5.2 TB/s.  Memory latency bounds it: a lane holds a head's angles, weights and both rows, so few
+// warps fit a SM (24 forwards, 16 backwards).  Heads whose chunks are no power of two leave lanes idle
+// (24 heads of 80 in bf16 forward 22 us, 2.9 TB/s), and heads of odd halves go element by element (24
+// heads of 34 in f32 29 us, 1.8 TB/s).
 #include <algorithm>
 
 #include "operators.h"

@@ -1,5 +1,19 @@
 // scan.cu -- the gated linear recurrence h_t = a_t h_{t-1} + b_t over time, per channel and
-// sequence, and its backward pass.
+// sequence, and its backward pass g_t = dh_t + a_{t+1} g_{t+1}.
+//
+// A run of steps maps the value v carried into it to A v + H, and two such maps compose into one, so
+// the time axis is cut: a warp takes a few steps of 32 or 64 channels into registers, reduces them to
+// their map, learns the value carried into them from the maps before, and walks them again to write.
+// Each element is read once and written once, but for calls of few channels and many steps, whose
+// parts are reduced by a launch of their own first.
+//
+// Measured on B200 (bytes moved over time, against a copy's 6.55 TB/s): 16 x 512 x 4096 bf16 direct
+// forward 36 us, 5.6 TB/s; 32 x 4096 x 512 bf16 sigmoid forward 82 us, 4.9 TB/s, backward 160 us,
+// 5.0 TB/s; a packed 131072 x 768 bf16 forward in two launches 169 us, which read 403 MB at 5.7 and
+// read and write 604 MB at 6.0 TB/s.  What bounds it: some 15 to 45 instructions a pair of elements,
+// issued by the sixteen warps a SM that 128 registers each leave (issue slots half busy, the rest
+// waiting for rows and for the exchange of maps).  Copies through shared memory several runs ahead
+// were slower (16 x 512 x 4096: 44 us), and so were lanes of four bf16 (8 x 1024 x 768: 25 us for 15).
 #include <cooperative_groups.h>
 
 #include <algorithm>
