@@ -333,6 +333,11 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
 // the other stores.
 constexpr int kKeep = 13, kGroups = 4;
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_desc d, int ranks, int64_t per) {
   pdl_entry();
@@ -346,7 +351,11 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
   const RowShare<T> row(z, d.vocab, rank, ranks, per);
+  // a block may be written to once all of its cluster have started
+  cg::cluster_group cluster = cg::this_cluster();
+  if (ranks > 1) cluster_arrive();
   if (t < 0 || in.weight == 0.0f) {  // the same for all blocks of the cluster
+    if (ranks > 1) cluster_wait();
     zero_row<T, THREADS>(out, z, row);
     if (rank == 0 && threadIdx.x == 0) d.logp[n] = d.token_loss[n] = 0.0f;
     return;
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
   }
   s = block_stats<THREADS>(s, k);
   if (ranks > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
+    cluster_wait();
     if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&parts[rank], threadIdx.x) = s;
     cluster.sync();
   }

@@ -10,8 +10,8 @@
 // Measured on B200 (bytes moved over time, against a copy's 6.55 TB/s): 16 x 512 x 4096 bf16 direct
 // forward 36 us, 5.6 TB/s; 32 x 4096 x 512 bf16 sigmoid forward 82 us, 4.9 TB/s, backward 160 us,
 // 5.0 TB/s; a packed 131072 x 768 bf16 forward in two launches 169 us, which read 403 MB at 5.7 and
-// read and write 604 MB at 6.0 TB/s.  What bounds it: some 15 to 45 instructions a pair of elements,
-// issued by the sixteen warps a SM that 128 registers each leave (issue slots half busy, the rest
+// read and write 604 MB at 6.0 TB/s.  What bounds it: 31 (direct forward) to 94 (sigmoid backward)
+// instructions a pair of elements, issued by the sixteen warps a SM that 128 registers each leave (issue slots half busy, the rest
 // waiting for rows and for the exchange of maps).  Copies through shared memory several runs ahead
 // were slower (16 x 512 x 4096: 44 us), and so were lanes of four bf16 (8 x 1024 x 768: 25 us for 15).
 #include <cooperative_groups.h>
@@ -264,6 +264,9 @@ __device__ __forceinline__ void send(unsigned to, unsigned barrier, int v) {
                ::"r"(to), "r"(v), "r"(barrier)
                : "memory");
 }
+// Set where a wait of the exchange ran out.
+__device__ int g_wait_expired;
+
 // Whether all that was expected has arrived; false after 4 seconds, which nothing but a fault
 // explains (the caller then makes its outputs NaN and goes on).
 __device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
@@ -280,7 +283,10 @@ __device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
     unsigned long long now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (since == 0) since = now;
-    if (now - since > 4000000000ull) return false;
+    if (now - since > 4000000000ull) {
+      g_wait_expired = 1;
+      return false;
+    }
   }
 }
 
@@ -856,4 +862,11 @@ extern "C" int tb_gated_scan_backward(const tb_scan_desc* desc, void* stream) {
 }
 extern "C" int64_t tb_gated_scan_workspace(int64_t batch, int64_t length, int64_t channels) {
   return tb::scan_workspace(batch, length, channels);
+}
+
+// ---- internal hook for tests (not part of the public ABI): whether a wait between the blocks of a
+// cluster ever ran out on the current device (1), or the flag cannot be read (-1).
+extern "C" int tbx_scan_error(void) {
+  int expired = 0;
+  return cudaMemcpyFromSymbol(&expired, tb::g_wait_expired, sizeof expired) == cudaSuccess ? expired : -1;
 }

@@ -737,6 +737,52 @@ def test_captured_graphs_replay_on_new_inputs(device):
         assert all(torch.equal(p, q) for p, q in zip(out, e))
 
 
+def test_no_wait_between_blocks_ran_out(device):
+    from poorgrad_b200.abi import load_library
+    x = torch.randn(8, 2000, 768, device="cuda").bfloat16()
+    h, _ = operators.gated_scan(x, x)
+    operators.gated_scan_backward(h, x, x, h)
+    torch.cuda.synchronize()
+    assert load_library().tbx_scan_error() == 0
+
+
+LARGE_CHILD = r"""
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+import operator_cases as oc
+from poorgrad_b200 import operators
+torch.manual_seed(1)
+q, k = (torch.randn(2, 64, h, 128, device="cuda").bfloat16() for h in (8, 2))
+x = torch.randn(8, 600, 768, device="cuda").bfloat16()
+p = torch.randn(1, 4000, 64, device="cuda")
+z = torch.randn(5, 50257, device="cuda")
+at, row = torch.randint(0, 50257, (5,), device="cuda").int(), torch.randn(5, device="cuda")
+table = torch.from_numpy(operators.rotation_table(64, 128)).cuda()
+def calls():
+    out = list(operators.head_rotate_backward(q, k, q, k, table))
+    out += operators.gated_scan_backward(x, x, x, x)
+    out += operators.gated_scan(p, p) + operators.gated_scan(x, x)
+    for logits in (z, z.bfloat16()):
+        out += operators.policy_loss(logits, at, row, row, row)
+    return out
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):   # first calls of kernels with large shared memory, clusters, parts
+    out = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, calls()))
+print("same")
+"""
+
+
+def test_first_calls_of_the_large_kernels_can_be_captured(device):
+    out = subprocess.run([sys.executable, "-c", LARGE_CHILD % (ROOT, os.path.join(ROOT, "tests"))],
+                         capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0 and out.stdout.split() == ["same"], out.stderr[-2000:]
+
+
 CHILD = r"""
 import sys
 sys.path[:0] = [%r, %r]
