@@ -758,7 +758,8 @@ int writing_threads(int64_t vocab) {
     case 256: return launch_pdl(KERNEL<T, 256>, dim3((unsigned)rows), dim3(256), 0, stream, __VA_ARGS__); \
     default: return launch_pdl(KERNEL<T, 128>, dim3((unsigned)rows), dim3(128), 0, stream, __VA_ARGS__);  \
   }
-// Rows that fit a warp's registers.
+// Rows that fit a warp's registers (8192 x 1100 f32 with the gradient: 29 us in 64 registers a lane, 27
+// by blocks; bf16 40 and 28).
 constexpr int64_t kWarpVocab = 1024;
 #define TB_BY_ITEMS(KERNEL, ...)                                                                   \
   {                                                                                                \
