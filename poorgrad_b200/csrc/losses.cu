@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(1024) k_sum_terms(const float* terms, int64_t 
   pdl_entry();
   __shared__ double part[32];
   double s = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < count; i += 1024) s += terms[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);

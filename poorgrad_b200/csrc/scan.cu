@@ -702,6 +702,7 @@ const char* check(const tb_scan_desc& d, bool backward) {
   if (d.element != TB_ELEMENT_F32 && d.element != TB_ELEMENT_BF16) return "unknown element type";
   if (d.form != TB_SCAN_DIRECT && d.form != TB_SCAN_SIGMOID) return "unknown form";
   if (!extents_fit({d.batch, d.length, d.channels}) || d.length > kMaxLength || d.batch > INT32_MAX ||
+      d.channels > INT32_MAX ||
       !extents_fit({d.sequences, d.channels}) || d.sequences > INT32_MAX)
     return "extents out of range";
   if (d.sequences ? !d.offsets || d.batch != 1 : d.offsets != nullptr)

@@ -92,7 +92,8 @@ REFUSED = (
         dict(sequences=1, batch=1), dict(offsets=256), dict(sequences=1, offsets=256),
         dict(gate_strides=[-1, 4]), dict(h_strides=[12, 3]), dict(h_strides=[0, 4]),
         dict(h_strides=[4, 4]), dict(h_strides=[8, 4]), dict(h_strides=[4, 7]),
-        dict(batch=1 << 40, length=1 << 30), dict(x_strides=[1 << 62, 4]))]
+        dict(batch=1 << 40, length=1 << 30), dict(x_strides=[1 << 62, 4]),
+        dict(channels=1 << 31, batch=1), dict(gate_strides=[0, 1 << 29]))]
     + [("tb_gated_scan_backward", scan_request(**c)) for c in (
         dict(dh=0), dict(dgate=0), dict(dx=0), dict(dgate_strides=[12, 1]),
         dict(dx_strides=[1, 4]), dict(dh=255), dict(x=0, form=1))]
