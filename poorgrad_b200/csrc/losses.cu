@@ -31,17 +31,28 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// max z, and the sum of exp(scale (z - top)); k = scale log2(e).  A sum of 0: no logit above -inf.
+// A row's statistics, with k = scale log2(e): top, the largest z, and sum, that of 2^(k (z - top) - f).
+// f, from 1 to 2, lifts k top to a whole number m, so that a sum is carried over to another top by a
+// factor 2^(m - m'), which is exact: ex2 is low by 5e-8 on average (measured below -1), and a sum that
+// went through it once for its terms and two or three times more for its tops made all log
+// probabilities of an answer too large, by 7e-8 to 1.6e-7.  The once is undone by the top's own term,
+// 2^-f, which is as low: it is what the sum is divided by in the end, and a row of one likely token comes
+// out right to the last bit.  Where k top is past 2^21, f is 0 and the factors are rounded.
+// A sum of 0: no logit above -inf.
 struct RowStats {
   float top, sum;
 };
 // What differences are taken from: -inf would make NaN of -inf logits, and any finite number does.
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }
-// A NaN logit makes the sum NaN (the maximum passes it over, the exponential does not), and so does
-// +inf, by inf - inf.
-__device__ __forceinline__ RowStats merge(RowStats p, RowStats q, float k) {
-  const float top = fmaxf(p.top, q.top), base = base_of(top);
-  return {top, p.sum * ex2(k * (p.top - base)) + q.sum * ex2(k * (q.top - base))};
+__device__ __forceinline__ float lift_of(float top, float k) {
+  const float at = k * top;
+  return fabsf(at) < 2097152.0f ? fmaf(-k, top, ceilf(at) + 1.0f) : 0.0f;
+}
+// The factor that carries a sum over from a top to one that is `less` below it, with their f's.  m - m' is
+// whole but for this line's rounding.
+__device__ __forceinline__ float carry(float less, float from, float to, float k) {
+  const float power = fmaf(k, less, from - to);
+  return ex2(from * to != 0.0f ? rintf(power) : power);
 }
 
 // 16 bytes of a row.
@@ -88,18 +99,28 @@ struct Vector<bf16> {
   }
 };
 
-// Adds COUNT vectors to a thread's statistics: one rescaling for all of them.
+// A thread's statistics, and its top's f.
+struct ThreadStats {
+  RowStats s{-INFINITY, 0.0f};
+  float base = 0.0f, lift = 0.0f;
+  __device__ __forceinline__ void raise(float top, float k) {
+    if (top > s.top) {
+      const float to = lift_of(top, k);
+      s.sum *= carry(s.top - top, lift, to, k);
+      s.top = base = top;
+      lift = to;
+    }
+  }
+};
+// Adds COUNT vectors: one rescaling for all of them.
 template <typename T, int COUNT>
-__device__ __forceinline__ void add(RowStats& s, const uint4 (&r)[COUNT], float k) {
+__device__ __forceinline__ void add(ThreadStats& of, const uint4 (&r)[COUNT], float k) {
   typedef Vector<T> Vec;
   float top = Vec::top(r[0]);
 #pragma unroll
   for (int j = 1; j < COUNT; ++j) top = fmaxf(top, Vec::top(r[j]));
-  if (top > s.top) {
-    s.sum *= ex2(k * (s.top - top));
-    s.top = top;
-  }
-  const float2 minus = both(-base_of(s.top));
+  of.raise(top, k);
+  const float2 minus = both(-of.base), lift = both(-of.lift);
   float2 sum = both(0.0f);
 #pragma unroll
   for (int j = 0; j < COUNT; ++j) {
@@ -107,18 +128,15 @@ __device__ __forceinline__ void add(RowStats& s, const uint4 (&r)[COUNT], float 
     Vec::read(r[j], v);
 #pragma unroll
     for (int i = 0; i < Vec::kPairs; ++i) {
-      const float2 x = mul2(add2(v[i], minus), both(k));
+      const float2 x = fma2(add2(v[i], minus), both(k), lift);
       sum = add2(sum, {ex2(x.x), ex2(x.y)});
     }
   }
-  s.sum += sum.x + sum.y;
+  of.s.sum += sum.x + sum.y;
 }
-__device__ __forceinline__ void add(RowStats& s, float z, float k) {
-  if (z > s.top) {
-    s.sum *= ex2(k * (s.top - z));
-    s.top = z;
-  }
-  s.sum += ex2(k * (z - base_of(s.top)));
+__device__ __forceinline__ void add(ThreadStats& of, float z, float k) {
+  of.raise(z, k);
+  of.s.sum += ex2(fmaf(z - of.base, k, -of.lift));
 }
 
 // A row as single elements up to a 16-byte boundary, vectors, and single elements again; the
@@ -143,9 +161,15 @@ struct RowShare {
   __device__ __forceinline__ int64_t element(int64_t vector) const { return head + (first + vector) * kVec; }
 };
 
+// A NaN logit makes the sum NaN (the maximum passes it over, the exponential does not), and so does
+// +inf, by inf - inf.
 __device__ __forceinline__ RowStats warp_stats(RowStats s, float k, int lanes = 32) {
-  for (int o = lanes / 2; o > 0; o >>= 1)
-    s = merge(s, {__shfl_xor_sync(~0u, s.top, o), __shfl_xor_sync(~0u, s.sum, o)}, k);
+  float top = s.top;
+  for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  const float base = base_of(top);
+  s.sum *= carry(s.top - base, lift_of(s.top, k), lift_of(base, k), k);
+  s.top = top;
+  for (int o = lanes / 2; o > 0; o >>= 1) s.sum += __shfl_xor_sync(~0u, s.sum, o);
   return s;
 }
 // The statistics of all threads, in a fixed order; the first warp gets them (what follows is one
@@ -165,7 +189,7 @@ __device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k
   constexpr int kAtOnce = 4;
   const RowShare<T> row(z, vocab, 0, 1, INT64_MAX / 2);
   const uint4* from = (const uint4*)(z + row.head);
-  RowStats s{-INFINITY, 0.0f};
+  ThreadStats s;
   if (row.single >= 0) add(s, to_f32(z[row.single]), k);
   int64_t i = threadIdx.x;
   for (; i + (kAtOnce - 1) * THREADS < row.count; i += kAtOnce * THREADS) {
@@ -178,7 +202,7 @@ __device__ __forceinline__ RowStats row_stats(const T* z, int64_t vocab, float k
     const uint4 r[1] = {from[i]};
     add<T>(s, r, k);
   }
-  return block_stats<THREADS>(s, k);
+  return block_stats<THREADS>(s.s, k);
 }
 
 // A row's gradient c scale (1[v = t] - p_v): where it goes, and what it is made of.
@@ -187,23 +211,23 @@ struct RowGradient {
   typedef Vector<T> Vec;
   T* out;
   RowStats s;
-  float k, step, share;
+  float k, lift, step, share;
   int64_t target;
   bool whole;  // the output's rows start where the input's do, counted in 16 bytes
 
   __device__ RowGradient(T* out, const T* z, RowStats s, float scale, float slope, int64_t target)
-      : out(out), s(s), k(scale * kLog2e), step(slope * scale), share(slope * scale / s.sum),
+      : out(out), s(s), k(scale * kLog2e), lift(lift_of(s.top, k)), step(slope * scale), share(slope * scale / s.sum),
         target(target), whole((((uintptr_t)out ^ (uintptr_t)z) & 15) == 0) {}
 
   __device__ __forceinline__ void single(float z, int64_t at) const {
-    out[at] = from_f32<T>((at == target ? step : 0.0f) - share * ex2(k * (z - s.top)));
+    out[at] = from_f32<T>((at == target ? step : 0.0f) - share * ex2(fmaf(z - s.top, k, -lift)));
   }
   __device__ __forceinline__ uint4 of(uint4 r) const {
     float2 v[Vec::kPairs];
     Vec::read(r, v);
 #pragma unroll
     for (int j = 0; j < Vec::kPairs; ++j) {
-      const float2 x = mul2(add2(v[j], both(-s.top)), both(k));
+      const float2 x = fma2(add2(v[j], both(-s.top)), both(k), both(-lift));
       v[j] = mul2({ex2(x.x), ex2(x.y)}, both(-share));
     }
     return Vec::made(v);
@@ -260,8 +284,17 @@ __device__ __forceinline__ void stream_gradient(const T* z, const RowShare<T>& r
   g.template mend<THREADS>(row, [&](int64_t) { return found; });
 }
 
-__device__ __forceinline__ float logp_of(float z, RowStats s, float scale) {
-  return scale * (z - s.top) - logf(s.sum);
+// Sums up to 64 bits: a log probability of some -10 has a rounding of 5e-7 in 32, and the losses' terms
+// are made of differences from others.  Of the sum's logarithm the power of two goes that way, and 32 bits
+// hold the rest, up to 0.35, to 3e-8 (a logarithm in 64 bits, which a whole block waits for, made
+// 8192 x 50257 in f32 20% slower).  z goes by the k that the sum's terms went by, and not by scale: what
+// k's rounding does to the two then cancels where z is a token as likely as the row says.
+__device__ __forceinline__ double logp_of(float z, RowStats s, float scale) {
+  const float k = scale * kLog2e, sum = s.sum / ex2(-lift_of(s.top, k));  // at least 1
+  if (!(sum < INFINITY)) return NAN;
+  const int power = (__float_as_int(sum) - 0x3f3504f3) >> 23;  // leaves sqrt(1/2) to sqrt(2)
+  const float rest = __int_as_float(__float_as_int(sum) - (power << 23));
+  return 0.6931471805599453 * ((double)k * ((double)z - (double)s.top) - (double)power) - (double)logf(rest);
 }
 
 template <typename T, int THREADS>
@@ -274,7 +307,7 @@ __global__ void __launch_bounds__(THREADS) k_token_logp(const T* logits, int64_t
   if (t >= 0) {
     const T* z = logits + n * stride;
     const RowStats s = row_stats<T, THREADS>(z, vocab, scale * kLog2e);
-    if (threadIdx.x == 0 && s.sum != 0.0f) out = t < vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+    if (threadIdx.x == 0 && s.sum != 0.0f) out = t < vocab ? (float)logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) logp[n] = out;
 }
@@ -289,14 +322,14 @@ struct TermInputs {
       : advantage(d.advantages[n]), old_logp(d.old_logp[n]), ref_logp(d.kl > 0 ? d.ref_logp[n] : 0.0f),
         weight(d.weights[n]) {}
 };
-__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, const TermInputs& in, float logp) {
-  const float a = in.advantage, r = expf(logp - in.old_logp);
+__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, const TermInputs& in, double logp) {
+  const float a = in.advantage, r = expf((float)(logp - (double)in.old_logp));
   const float held = fminf(fmaxf(r, 1.0f - (float)d.clip_low), 1.0f + (float)d.clip_high);
   const float plain = r * a, kept = (r != r ? r : held) * a;
   float loss = -(plain <= kept ? plain : kept), slope = plain <= kept ? -plain : 0.0f;
   if (plain != plain) loss = slope = plain;
   if (d.kl > 0) {
-    const float x = in.ref_logp - logp, e = expm1f(x);
+    const float x = (float)((double)in.ref_logp - logp), e = expm1f(x);
     loss += (float)d.kl * (e - x);
     slope -= (float)d.kl * e;
   }
@@ -309,7 +342,7 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x, t = d.targets[n];
   const float scale = (float)d.scale;
-  float logp = 0.0f;
+  double logp = 0.0;
   Term term{0.0f, 0.0f};
   const TermInputs in(d, n);
   if (t >= 0 && in.weight != 0.0f) {
@@ -321,7 +354,7 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
     }
   }
   if (threadIdx.x == 0) {
-    d.logp[n] = logp;
+    d.logp[n] = (float)logp;
     d.token_loss[n] = term.loss;
   }
 }
@@ -347,7 +380,8 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
   const int rank = blockIdx.x % ranks, keep = (int)((per + THREADS - 1) / THREADS);
   const int64_t t = d.targets[n];
   const TermInputs in(d, n);
-  const float scale = (float)d.scale, k = scale * kLog2e;
+  const float scale = (float)d.scale;
+  const float k = scale * kLog2e;
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
   const RowShare<T> row(z, d.vocab, rank, ranks, per);
@@ -373,8 +407,8 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
   }
   const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
   const float single = row.single >= 0 ? to_f32(z[row.single]) : 0.0f;
-  RowStats s{-INFINITY, 0.0f};
-  if (row.single >= 0) add(s, single, k);
+  ThreadStats mine;
+  if (row.single >= 0) add(mine, single, k);
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
     if (g == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -385,10 +419,10 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
     const int last = min(count, min(keep, (g + 1) * each) * THREADS);
     for (int i = g * each * THREADS + threadIdx.x; i < last; i += 2 * THREADS) {
       const uint4 r[2] = {kept[i], i + THREADS < last ? kept[i + THREADS] : Vector<T>::nothing()};
-      add<T>(s, r, k);
+      add<T>(mine, r, k);
     }
   }
-  s = block_stats<THREADS>(s, k);
+  RowStats s = block_stats<THREADS>(mine.s, k);
   if (ranks > 1) {
     cluster_wait();
     if ((int)threadIdx.x < ranks) *cluster.map_shared_rank(&parts[rank], threadIdx.x) = s;
@@ -400,14 +434,14 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
     const RowStats none{-INFINITY, 0.0f};
     if (ranks > 1) s = warp_stats((int)threadIdx.x < ranks ? parts[threadIdx.x] : none, k, 8);
     if (threadIdx.x == 0) {
-      float logp = 0.0f;
+      double logp = 0.0;
       Term term{0.0f, 0.0f};
       if (s.sum != 0.0f) {
         logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
         term = policy_term(d, in, logp);
       }
       if (rank == 0) {
-        d.logp[n] = logp;
+        d.logp[n] = (float)logp;
         d.token_loss[n] = term.loss;
       }
       whole = s;
@@ -446,13 +480,13 @@ __global__ void __launch_bounds__(THREADS) k_policy_twice(tb_policy_desc d) {
   RowStats s{0.0f, 0.0f};
   if (t >= 0 && in.weight != 0.0f) s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
   if (threadIdx.x == 0) {
-    float logp = 0.0f;
+    double logp = 0.0;
     Term term{0.0f, 0.0f};
     if (s.sum != 0.0f) {
       logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
-    d.logp[n] = logp;
+    d.logp[n] = (float)logp;
     d.token_loss[n] = term.loss;
     whole = s;
     slope = term.slope;
@@ -476,10 +510,10 @@ struct WarpRow {
     for (int j = 0; j < ITEMS; ++j) s.top = fmaxf(s.top, v[j]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s.top = fmaxf(s.top, __shfl_xor_sync(~0u, s.top, o));
-    const float base = base_of(s.top);
+    const float base = base_of(s.top), lift = lift_of(base, k);
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
-      v[j] = ex2(k * (v[j] - base));
+      v[j] = ex2(fmaf(v[j] - base, k, -lift));
       s.sum += v[j];
     }
 #pragma unroll
@@ -509,7 +543,7 @@ __global__ void __launch_bounds__(256) k_policy_warps(tb_policy_desc d) {
   const float scale = (float)d.scale;
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
-  float logp = 0.0f;
+  double logp = 0.0;
   Term term{0.0f, 0.0f};
   if (t >= 0 && in.weight != 0.0f) {
     const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
@@ -524,7 +558,7 @@ __global__ void __launch_bounds__(256) k_policy_warps(tb_policy_desc d) {
     zero_warp_row(out, d.vocab);
   }
   if (threadIdx.x % 32 == 0) {
-    d.logp[n] = logp;
+    d.logp[n] = (float)logp;
     d.token_loss[n] = term.loss;
   }
 }
@@ -541,7 +575,7 @@ __global__ void __launch_bounds__(256) k_token_logp_warps(const T* logits, int64
     const T* z = logits + n * stride;
     const float zt = t < vocab ? to_f32(z[t]) : 0.0f;
     const WarpRow<T, ITEMS> row(z, (int)vocab, scale * kLog2e);
-    if (row.s.sum != 0.0f) out = t < vocab ? logp_of(zt, row.s, scale) : NAN;
+    if (row.s.sum != 0.0f) out = t < vocab ? (float)logp_of(zt, row.s, scale) : NAN;
   }
   if (threadIdx.x % 32 == 0) logp[n] = out;
 }
@@ -567,7 +601,7 @@ __global__ void __launch_bounds__(1024) k_sum_terms(const float* terms, int64_t 
 struct PreferenceScratch {
   double* terms;    // [pairs], the weighted losses
   RowStats* stats;  // [rows]
-  float* slopes;    // [rows], of the loss by the row's log probability
+  float* slopes;    // [rows], logp - ref, then the loss's slope by the row's log probability
   __host__ __device__ explicit PreferenceScratch(const tb_preference_desc& d)
       : terms((double*)d.workspace), stats((RowStats*)(terms + d.pairs)), slopes((float*)(stats + d.rows)) {}
 };
@@ -586,15 +620,17 @@ __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc 
   const int64_t t = d.targets[n];
   const float scale = (float)d.scale;
   RowStats s{0.0f, 0.0f};
-  float logp = 0.0f;
+  double logp = 0.0;
   if (t >= 0) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
     if (threadIdx.x == 0 && s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) {
-    PreferenceScratch(d).stats[n] = s;
-    d.logp[n] = logp;
+    const PreferenceScratch scratch(d);
+    scratch.stats[n] = s;
+    if (s.sum != 0.0f) scratch.slopes[n] = (float)(logp - (double)d.ref_logp[n]);
+    d.logp[n] = (float)logp;
   }
 }
 template <typename T, int ITEMS>
@@ -605,7 +641,7 @@ __global__ void __launch_bounds__(256) k_preference_rows_warps(tb_preference_des
   const int64_t t = d.targets[n];
   const float scale = (float)d.scale;
   RowStats s{0.0f, 0.0f};
-  float logp = 0.0f;
+  double logp = 0.0;
   if (t >= 0) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
@@ -613,8 +649,10 @@ __global__ void __launch_bounds__(256) k_preference_rows_warps(tb_preference_des
     if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
   }
   if (threadIdx.x % 32 == 0) {
-    PreferenceScratch(d).stats[n] = s;
-    d.logp[n] = logp;
+    const PreferenceScratch scratch(d);
+    scratch.stats[n] = s;
+    if (s.sum != 0.0f) scratch.slopes[n] = (float)(logp - (double)d.ref_logp[n]);
+    d.logp[n] = (float)logp;
   }
 }
 
@@ -635,7 +673,7 @@ __global__ void __launch_bounds__(kPairThreads) k_preference_pairs(tb_preference
     double r = 0;
 #pragma unroll 4
     for (int64_t n = lo[k] + threadIdx.x; n < hi[k]; n += kPairThreads)
-      if (scratch.stats[n].sum != 0.0f) r += (double)d.logp[n] - (double)d.ref_logp[n];
+      if (scratch.stats[n].sum != 0.0f) r += (double)scratch.slopes[n];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(~0u, r, o);
     if (threadIdx.x % 32 == 0) part[k][threadIdx.x / 32] = r;

@@ -1075,3 +1075,37 @@ def test_rotate_over_many_tokens(device):
         inner = (dn * x * r).abs().mean(-1, keepdim=True)
         bar = 192 * EPS * r * (dn.abs().amax(-1, keepdim=True) + (x * r).abs().amax(-1, keepdim=True) * inner)
         within(back[i], dx, bar + half_step(t) * dx.abs(), "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [500, 4000, 15001])
+def test_long_answers_add_up_no_error_of_one_sign(vocab, dtype):
+    rows, t = 8192, TYPES[dtype]
+    z = (2 * torch.randn(rows, vocab, generator=torch.Generator().manual_seed(vocab))).to(t)
+    at = torch.multinomial(torch.softmax(z.float(), -1), 1, generator=torch.Generator().manual_seed(1))
+    exact = (z.double().gather(1, at) - torch.logsumexp(z.double(), -1, keepdim=True))[:, 0]
+    ref = (exact - 0.1).float()
+    got = operators.preference_loss(cuda(z, t), cuda(at[:, 0], torch.int32),
+                                    torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda"),
+                                    cuda(ref))
+    # A row's roundings (its terms' arguments and sum, its top's term, the rest of the logarithm, the
+    # difference from the reference) go either way and come to 1.5e-7 at most, so their mean over the
+    # rows has a deviation of at most 1.5e-7 / sqrt(8192) = 1.7e-9; six of those.  The fast exponential
+    # is low by 5e-8 on average, and that must not be left.
+    ratio = float((exact - ref.double()).sum())
+    within(got.ratios.flatten()[:1], torch.tensor([ratio]), 1e-8 * rows + EPS / 2 * abs(ratio), "log ratio")
+
+
+@pytest.mark.parametrize("vocab", [40, 5000])
+@pytest.mark.parametrize("scale", [1.0, 0.3])
+@pytest.mark.parametrize("middle", [1453635.0, -1453635.0, 4845450.0, 1e30, -3e38])
+def test_log_probabilities_of_large_logits(middle, scale, vocab):
+    # tops on both sides of where k top passes 2^21, and far past it, within a row
+    z = (middle + 6 * torch.randn(9, vocab, generator=torch.Generator().manual_seed(vocab))).float()
+    z[3] = torch.finfo(torch.float32).min
+    at = torch.arange(9) % vocab
+    exact = torch.log_softmax(z.double() * scale, -1).gather(1, at[:, None])[:, 0]
+    got = operators.token_logp(cuda(z), cuda(at, torch.int32), scale=scale)
+    # each term is off by 2 + 1.2 |x| steps, |x| below 40 where it counts, and so is the factor that
+    # carries it over where that is rounded, up to 12 times; k by half a step of the differences
+    within(got, exact, EPS * (50 * 13 + 2 * exact.abs()), "log probability")
