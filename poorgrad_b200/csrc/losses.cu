@@ -284,17 +284,18 @@ __device__ __forceinline__ void stream_gradient(const T* z, const RowShare<T>& r
   g.template mend<THREADS>(row, [&](int64_t) { return found; });
 }
 
-// Sums up to 64 bits: a log probability of some -10 has a rounding of 5e-7 in 32, and the losses' terms
-// are made of differences from others.  Of the sum's logarithm the power of two goes that way, and 32 bits
-// hold the rest, up to 0.35, to 3e-8 (a logarithm in 64 bits, which a whole block waits for, made
-// 8192 x 50257 in f32 20% slower).  z goes by the k that the sum's terms went by, and not by scale: what
-// k's rounding does to the two then cancels where z is a token as likely as the row says.
-__device__ __forceinline__ double logp_of(float z, RowStats s, float scale) {
+// Of the sum's logarithm the power of two is added to the logit's share, and 32 bits hold the rest, up
+// to 0.35, to 3e-8.  z goes by the k that the sum's terms went by, and not by scale: what k's rounding
+// does to the two then cancels where z is a token as likely as the row says.  Real: 64 bits where many
+// rows are added up, as one near -10 has a rounding of 5e-7 in 32; 32 where a block waits for it (in
+// 64, 16384 x 27 f32 took 8.5 us for 8.0).
+template <typename Real>
+__device__ __forceinline__ Real logp_of(float z, RowStats s, float scale) {
   const float k = scale * kLog2e, sum = s.sum / ex2(-lift_of(s.top, k));  // at least 1
   if (!(sum < INFINITY)) return NAN;
   const int power = (__float_as_int(sum) - 0x3f3504f3) >> 23;  // leaves sqrt(1/2) to sqrt(2)
   const float rest = __int_as_float(__float_as_int(sum) - (power << 23));
-  return 0.6931471805599453 * ((double)k * ((double)z - (double)s.top) - (double)power) - (double)logf(rest);
+  return (Real)0.6931471805599453 * ((Real)k * ((Real)z - (Real)s.top) - (Real)power) - (Real)logf(rest);
 }
 
 template <typename T, int THREADS>
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(THREADS) k_token_logp(const T* logits, int64_t
   if (t >= 0) {
     const T* z = logits + n * stride;
     const RowStats s = row_stats<T, THREADS>(z, vocab, scale * kLog2e);
-    if (threadIdx.x == 0 && s.sum != 0.0f) out = t < vocab ? (float)logp_of(to_f32(z[t]), s, scale) : NAN;
+    if (threadIdx.x == 0 && s.sum != 0.0f) out = t < vocab ? (float)logp_of<double>(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) logp[n] = out;
 }
@@ -322,14 +323,14 @@ struct TermInputs {
       : advantage(d.advantages[n]), old_logp(d.old_logp[n]), ref_logp(d.kl > 0 ? d.ref_logp[n] : 0.0f),
         weight(d.weights[n]) {}
 };
-__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, const TermInputs& in, double logp) {
-  const float a = in.advantage, r = expf((float)(logp - (double)in.old_logp));
+__device__ __forceinline__ Term policy_term(const tb_policy_desc& d, const TermInputs& in, float logp) {
+  const float a = in.advantage, r = expf(logp - in.old_logp);
   const float held = fminf(fmaxf(r, 1.0f - (float)d.clip_low), 1.0f + (float)d.clip_high);
   const float plain = r * a, kept = (r != r ? r : held) * a;
   float loss = -(plain <= kept ? plain : kept), slope = plain <= kept ? -plain : 0.0f;
   if (plain != plain) loss = slope = plain;
   if (d.kl > 0) {
-    const float x = (float)((double)in.ref_logp - logp), e = expm1f(x);
+    const float x = in.ref_logp - logp, e = expm1f(x);
     loss += (float)d.kl * (e - x);
     slope -= (float)d.kl * e;
   }
@@ -342,19 +343,19 @@ __global__ void __launch_bounds__(THREADS) k_policy_terms(tb_policy_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x, t = d.targets[n];
   const float scale = (float)d.scale;
-  double logp = 0.0;
+  float logp = 0.0f;
   Term term{0.0f, 0.0f};
   const TermInputs in(d, n);
   if (t >= 0 && in.weight != 0.0f) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     const RowStats s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
     if (threadIdx.x == 0 && s.sum != 0.0f) {
-      logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+      logp = t < d.vocab ? logp_of<float>(to_f32(z[t]), s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
   }
   if (threadIdx.x == 0) {
-    d.logp[n] = (float)logp;
+    d.logp[n] = logp;
     d.token_loss[n] = term.loss;
   }
 }
@@ -434,14 +435,14 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_policy(tb_policy_de
     const RowStats none{-INFINITY, 0.0f};
     if (ranks > 1) s = warp_stats((int)threadIdx.x < ranks ? parts[threadIdx.x] : none, k, 8);
     if (threadIdx.x == 0) {
-      double logp = 0.0;
+      float logp = 0.0f;
       Term term{0.0f, 0.0f};
       if (s.sum != 0.0f) {
-        logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
+        logp = t < d.vocab ? logp_of<float>(zt, s, scale) : NAN;
         term = policy_term(d, in, logp);
       }
       if (rank == 0) {
-        d.logp[n] = (float)logp;
+        d.logp[n] = logp;
         d.token_loss[n] = term.loss;
       }
       whole = s;
@@ -480,13 +481,13 @@ __global__ void __launch_bounds__(THREADS) k_policy_twice(tb_policy_desc d) {
   RowStats s{0.0f, 0.0f};
   if (t >= 0 && in.weight != 0.0f) s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
   if (threadIdx.x == 0) {
-    double logp = 0.0;
+    float logp = 0.0f;
     Term term{0.0f, 0.0f};
     if (s.sum != 0.0f) {
-      logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+      logp = t < d.vocab ? logp_of<float>(to_f32(z[t]), s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
-    d.logp[n] = (float)logp;
+    d.logp[n] = logp;
     d.token_loss[n] = term.loss;
     whole = s;
     slope = term.slope;
@@ -543,13 +544,13 @@ __global__ void __launch_bounds__(256) k_policy_warps(tb_policy_desc d) {
   const float scale = (float)d.scale;
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;
-  double logp = 0.0;
+  float logp = 0.0f;
   Term term{0.0f, 0.0f};
   if (t >= 0 && in.weight != 0.0f) {
     const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
     const WarpRow<T, ITEMS> row(z, (int)d.vocab, scale * kLog2e);
     if (row.s.sum != 0.0f) {
-      logp = t < d.vocab ? logp_of(zt, row.s, scale) : NAN;
+      logp = t < d.vocab ? logp_of<float>(zt, row.s, scale) : NAN;
       term = policy_term(d, in, logp);
     }
     __syncwarp();  // the gradient may overwrite the logits that others still read
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(256) k_policy_warps(tb_policy_desc d) {
     zero_warp_row(out, d.vocab);
   }
   if (threadIdx.x % 32 == 0) {
-    d.logp[n] = (float)logp;
+    d.logp[n] = logp;
     d.token_loss[n] = term.loss;
   }
 }
@@ -575,7 +576,7 @@ __global__ void __launch_bounds__(256) k_token_logp_warps(const T* logits, int64
     const T* z = logits + n * stride;
     const float zt = t < vocab ? to_f32(z[t]) : 0.0f;
     const WarpRow<T, ITEMS> row(z, (int)vocab, scale * kLog2e);
-    if (row.s.sum != 0.0f) out = t < vocab ? (float)logp_of(zt, row.s, scale) : NAN;
+    if (row.s.sum != 0.0f) out = t < vocab ? (float)logp_of<double>(zt, row.s, scale) : NAN;
   }
   if (threadIdx.x % 32 == 0) logp[n] = out;
 }
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc 
   if (t >= 0) {
     const T* z = (const T*)d.logits + n * d.logits_stride;
     s = row_stats<T, THREADS>(z, d.vocab, scale * kLog2e);
-    if (threadIdx.x == 0 && s.sum != 0.0f) logp = t < d.vocab ? logp_of(to_f32(z[t]), s, scale) : NAN;
+    if (threadIdx.x == 0 && s.sum != 0.0f) logp = t < d.vocab ? logp_of<double>(to_f32(z[t]), s, scale) : NAN;
   }
   if (threadIdx.x == 0) {
     const PreferenceScratch scratch(d);
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(256) k_preference_rows_warps(tb_preference_des
     const T* z = (const T*)d.logits + n * d.logits_stride;
     const float zt = t < d.vocab ? to_f32(z[t]) : 0.0f;
     s = WarpRow<T, ITEMS>(z, (int)d.vocab, scale * kLog2e).s;
-    if (s.sum != 0.0f) logp = t < d.vocab ? logp_of(zt, s, scale) : NAN;
+    if (s.sum != 0.0f) logp = t < d.vocab ? logp_of<double>(zt, s, scale) : NAN;
   }
   if (threadIdx.x % 32 == 0) {
     const PreferenceScratch scratch(d);
