@@ -7,10 +7,12 @@
 // value do not overflow.  The statistics of a row are a running maximum and sum of exponentials.
 //
 // Measured on B200 (against a copy's 6.55 TB/s): the policy loss with its gradient over 8192 x 50257
-// logits, a quarter of the rows hidden, f32 472 us, 6.1 TB/s, bf16 267 us, 5.4 TB/s; the log
-// probabilities alone f32 180 us, bf16 102 us, 6.0 TB/s.  Memory bounds the f32 forms (under load the
-// power cap too: 490 to 540 us in a long run), issue slots and the two exponentials a logit the bf16
-// ones.  The preference loss cannot know a row's slope before its pair's last row, and rows of a pair
+// logits, a quarter of the rows hidden, f32 485 us, 5.9 TB/s, bf16 280 us, 5.1 TB/s; the loss
+// alone f32 182 us, bf16 103 us, 6.0 TB/s.  Memory bounds the f32 forms (under load the power cap too:
+// up to 540 us in a long run), issue slots and the two exponentials a logit the bf16 ones.  Sums that
+// are carried over exactly cost rows that leave a thread two or three vectors most: 8192 x 4099 bf16
+// took 36 us before, 43 now, 3000 x 130000 f32 477 and 522; the longer bf16 rows that are only read
+// gained (123 -> 103).  The preference loss cannot know a row's slope before its pair's last row, and rows of a pair
 // do not fit the chip: it reads the logits twice, 4099 x 50257 bf16 in 181 us, 988 MB at 5.5 TB/s.
 #include <cooperative_groups.h>
 
