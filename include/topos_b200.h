@@ -355,7 +355,9 @@ typedef struct tb_scan_desc {
 } tb_scan_desc;
 /* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
  * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
- * final state is its state.  A wait between blocks that runs out (4 s, a fault) makes the outputs
+ * final state is its state.  Gates of the direct form may be larger than 1: steps are taken together, but
+ * outputs are finite wherever the recurrence is.  Steps that together shrink what they are handed by
+ * more than 2^126 may hand on nothing of it.  A wait between blocks that runs out (4 s, a fault) makes the outputs
  * behind it NaN. */
 int tb_gated_scan(const tb_scan_desc* desc, void* stream);
 /* Its gradients from dh and dfinal: with g_t = dh_t + a_{t+1} g_{t+1}, d a_t = g_t h_{t-1},

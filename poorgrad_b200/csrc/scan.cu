@@ -221,6 +221,121 @@ template <int V>
 __device__ __forceinline__ Vec<V> apply(Affine<V> f, bool begins, Vec<V> v) {
   return select(begins, f.H, fma(f.A, v, f.H));
 }
+template <int V>
+__device__ __forceinline__ bool finite(Vec<V> a) {
+  bool r = true;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r &= fabsf(a.get(i)) < INFINITY;
+  return r;
+}
+
+// Gates of the direct form may be larger than 1, and their product A may pass the range of 32 bits
+// although every step of the recurrence stays within it: an infinite A would make NaN of a carried 0, and
+// infinity of a small carried value.  A warp that meets one works its maps out again with A multiplied out
+// in 64 bits.  Such a map is marked kWide, and A's place holds the high word, rounded: 21 bits of precision,
+// which is what the roundings of sixteen gates in 32 bits leave too.  An A past the range of 64 bits takes
+// every value but 0 out of the range of 32 on its way, and of a 0 nothing is left but H.  Products too small
+// for 32 bits vanish: a run that shrinks what it is handed by more than 2^126 may hand on nothing of it.
+// None of this is inlined: it hardly ever runs, and the kernels have no registers for it.
+enum { kBegins = 1, kWide = 2 };  // what is said of a map; one that begins a sequence is never wide
+template <int V>
+struct Product {
+  double x[V];
+};
+template <int V>
+__device__ __forceinline__ Product<V> product_of(Vec<V> a, int said) {
+  Product<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    r.x[i] = said & kWide ? __hiloint2double(__float_as_int(a.get(i)), 0) : (double)a.get(i);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Product<V> operator*(Product<V> a, Product<V> b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.x[i] *= b.x[i];
+  return a;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> wide(Product<V> p) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const long long bits = __double_as_longlong(p.x[i]);
+    // an infinity or NaN is not rounded, for it might become another value
+    r.set(i, __int_as_float((int)((fabs(p.x[i]) < INFINITY ? bits + 0x80000000ll : bits) >> 32)));
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> apply_any(Affine<V> f, int said, Vec<V> v) {
+  if (!(said & kWide)) return apply(f, said & kBegins, v);
+  const Product<V> p = product_of(f.A, said);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    v.set(i, v.get(i) == 0.0f ? f.H.get(i) : (float)::fma(p.x[i], (double)v.get(i), (double)f.H.get(i)));
+  return v;
+}
+template <int V>
+__device__ __noinline__ Vec<V> applied(Affine<V> f, int said, Vec<V> v) {
+  return apply_any(f, said, v);
+}
+template <int V>
+struct Said {
+  Affine<V> map;
+  int said;
+};
+// The map of one run and another behind it.
+template <int V>
+__device__ __noinline__ Said<V> joined(Said<V> a, Said<V> b) {
+  if (b.said & kBegins) return b;
+  const Vec<V> H = apply_any(b.map, b.said, a.map.H);
+  if (a.said & kBegins) return {{splat<V>(1.0f), H}, kBegins};
+  return {{wide(product_of(a.map.A, a.said) * product_of(b.map.A, b.said)), H}, kWide};
+}
+// A lane's product of `count` gates, `bytes` apart.
+template <typename T, int V>
+__device__ __noinline__ Vec<V> wide_run(const char* gate, int64_t bytes, int count) {
+  typedef Raw<T, V> R;
+  Product<V> p = product_of(splat<V>(1.0f), 0);
+  for (int i = 0; i < count; ++i)
+    p = p * product_of(R::read(*(const typename R::type*)(gate + bytes * i)), 0);
+  return wide(p);
+}
+// A lane's value carried through `count` maps, and what it is before number `at`.
+template <int V>
+struct Carried {
+  Vec<V> after, before;
+};
+template <int V>
+__device__ __forceinline__ Carried<V> wide_walk(const Affine<V> (*maps)[32], const int* said, int count, int at,
+                                                Vec<V> v) {
+  Carried<V> r{v, v};
+  for (int i = 0; i < count; ++i) {
+    if (i == at) r.before = r.after;
+    r.after = apply_any(maps[i][threadIdx.x % 32], said[i], r.after);
+  }
+  return r;
+}
+// The maps of a block's warps behind one another.
+template <int V>
+__device__ __noinline__ Carried<V> wide_round(Affine<V> (*maps)[32], int* said, Affine<V> map, int of, Vec<V> carry) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  maps[warp][lane] = map;
+  if (lane == 0) said[warp] = of;
+  __syncthreads();
+  return wide_walk(maps, said, kWarps, warp, carry);
+}
+template <int V>
+__device__ __noinline__ Said<V> wide_block(Affine<V> (*maps)[32], int* said, Affine<V> map, int of) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  maps[warp][lane] = map;
+  if (lane == 0) said[warp] = of;
+  __syncthreads();
+  Said<V> r{maps[0][lane], said[0]};
+  for (int w = 1; w < kWarps; ++w) r = joined(r, {maps[w][lane], said[w]});
+  return r;
+}
 
 // How a call is cut: `ranks` blocks of a cluster take consecutive spans of kWarps * L steps, over
 // and over, and `parts` such clusters the consecutive parts of the time axis.  With several parts
@@ -230,7 +345,7 @@ struct Cut {
   int ranks, tiles, parts;
   int64_t part_steps;
   float2* maps;  // (A, H), [batch][parts][channels], parts > 1
-  int* begins;   // [batch][parts]
+  int* said;     // [batch][parts][tiles]
 };
 
 // A launch's part: a block walks its columns alone, or the blocks of a cluster together; or one of
@@ -290,6 +405,26 @@ __device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
   }
 }
 
+// As wide_round, by the warps of a cluster's blocks.  Each warp sends its map to all blocks by itself, so that
+// none waits for another but at the barrier, where waits are bounded.
+template <int V>
+__device__ __noinline__ Carried<V> wide_exchange(Affine<V> (*maps)[32], int* said, uint64_t* counted, Affine<V> map,
+                                                 int of, int ranks, int rank, int phase, Vec<V> carry) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, mine = rank * kWarps + warp;
+  const unsigned barrier = shared_address(counted);
+  if (threadIdx.x == 0)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier),
+                 "r"(ranks * kWarps * (32 * (int)sizeof(Affine<V>) + 4))
+                 : "memory");
+  for (int r = 0; r < ranks; ++r) {
+    const unsigned there = of_rank(barrier, r);
+    send(of_rank(shared_address(&maps[mine][lane]), r), there, map);
+    if (lane == 0) send(of_rank(shared_address(&said[mine]), r), there, of);
+  }
+  if (!arrived(barrier, phase)) return {splat<V>(NAN), splat<V>(NAN)};
+  return wide_walk(maps, said, ranks * kWarps, mine, carry);
+}
+
 // The recurrence, or with BACK the gradients, walked backwards: there the carried value is
 // c_t = a_t (dh_t + c_{t+1}), g_t = dh_t + c_{t+1}.
 //
@@ -303,6 +438,7 @@ struct Scan {
   typedef Raw<T, V> R;
   typedef typename R::type Row;
   static constexpr bool kReadsX = FORM == TB_SCAN_SIGMOID;
+  static constexpr bool kGrows = FORM == TB_SCAN_DIRECT;  // products of gates may leave the range
   const tb_scan_desc& d;
   const int64_t b, c;
   const bool in;  // this lane's channels exist
@@ -402,6 +538,17 @@ struct Scan {
     return map;
   }
 
+  // The map of a run of which no row is written yet, with A in 64 bits where 32 do not hold it.
+  __device__ __forceinline__ Said<V> said_of(Affine<V> map, const Marks& m, int first) const {
+    if (m.enters) return {map, kBegins};
+    if (!__any_sync(~0u, !finite(map.A))) return {map, 0};
+    const int t0 = BACK ? (int)d.length - 1 - first : first;
+    // steps and channels that do not exist have a gate of 0
+    map.A = in && first + L <= d.length ? wide_run<T, V>(at(d.gate, d.gate_strides, t0), step(d.gate_strides), L)
+                                        : splat<V>(0.0f);
+    return {map, kWide};
+  }
+
   // ALL as in load(); MARKED: some step enters or leaves a sequence or lies outside all of them.
   template <bool ALL, bool MARKED>
   __device__ __forceinline__ void write(const Rows& r, const Marks& m, int first, Vec<V> value) {
@@ -449,11 +596,15 @@ template <typename T, int V, int L, int FORM, bool BACK, int PASS>
 __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut) {
   pdl_entry();
   __shared__ alignas(16) Affine<V> maps[2][kWarps][32];
-  __shared__ int begins[2][kWarps];
+  __shared__ int said[2][kWarps];
   constexpr int kHeld = PASS == kCluster ? kMaxRanks : 1;
   __shared__ alignas(16) Affine<V> rank_maps[2][kHeld][32];
-  __shared__ int rank_begins[2][kHeld];
-  __shared__ alignas(8) uint64_t counted[2];  // barriers of the exchange, one a parity
+  __shared__ int rank_said[2][kHeld];
+  __shared__ alignas(8) uint64_t counted[3];  // barriers of the exchange, one a parity, and of wide maps
+  constexpr bool kGrows = Scan<T, V, L, FORM, BACK, PASS>::kGrows;
+  __shared__ alignas(16) Affine<V> wide_maps[kGrows ? kHeld * kWarps : 1][32];
+  __shared__ alignas(8) Vec<V> carries[2][32];  // what a round began with
+  __shared__ int wide_said[kGrows ? kHeld * kWarps : 1];
   const int lane = threadIdx.x % 32, warp = __shfl_sync(~0u, threadIdx.x / 32, 0);
   const int ranks = PASS == kCluster ? cut.ranks : 1;
   const int rank = blockIdx.x % ranks, tile = blockIdx.x / ranks % cut.tiles;
@@ -464,7 +615,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   if constexpr (PASS == kCluster) {
     if (threadIdx.x == 0)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 3; ++i)
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&counted[i])) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     cg::this_cluster().sync();
@@ -483,22 +634,34 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
   }
 
   Vec<V> carry = splat<V>(0.0f);
-  if (PASS == kFromMaps && s.in)
-#pragma unroll 8
-    for (int p = 0; p < part; ++p) {
-      const float2* from = cut.maps + (b * cut.parts + p) * d.channels + s.c;
+  if (PASS == kFromMaps && s.in) {
+    const float2* from = cut.maps + b * cut.parts * d.channels + s.c;
+    const int* of = cut.said + b * cut.parts * cut.tiles + tile;
+    const auto map = [&](int p) {
       Affine<V> f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        f.A.set(v, from[v].x);
-        f.H.set(v, from[v].y);
+        f.A.set(v, from[p * d.channels + v].x);
+        f.H.set(v, from[p * d.channels + v].y);
       }
-      carry = apply(f, cut.begins[b * cut.parts + p], carry);
+      return f;
+    };
+    int seen = 0;
+#pragma unroll 8
+    for (int p = 0; p < part; ++p) {
+      seen |= of[p * cut.tiles];
+      carry = apply(map(p), of[p * cut.tiles] & kBegins, carry);
     }
+    if (kGrows && seen & kWide) {
+      carry = splat<V>(0.0f);
+      for (int p = 0; p < part; ++p) carry = applied(map(p), of[p * cut.tiles], carry);
+    }
+  }
   Affine<V> whole{splat<V>(1.0f), splat<V>(0.0f)};  // the part's map so far
-  bool whole_begins = false;
+  int whole_said = 0;
 
   int parity = 0, phase = 0;  // of the exchange's buffers, and of their barriers
+  [[maybe_unused]] int wide_phase = 0;
   const int from = (int)(part * cut.part_steps), to = (int)min(from + cut.part_steps, d.length);
   const int span = ranks * kWarps * L;
   // a part is a whole number of spans, so that no step belongs to two
@@ -522,7 +685,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       next_m = marks_of<L, BACK>(d, (int)b, next_first, known);
     }
     maps[parity][warp][lane] = map;
-    if (lane == 0) begins[parity][warp] = m.enters != 0;
+    // whether a product is not finite is said of the run's map (16 x 512 x 4096 bf16 35.8 us, 37.9 by the
+    // product of all), or seen in the product of all maps that are walked: an infinity or NaN stays one
+    constexpr bool kMarked = kGrows && PASS == kWhole;
+    int mark = m.enters ? kBegins : 0;
+    if (kMarked && !mark && __any_sync(~0u, !finite(map.A))) mark = kWide;
+    if (lane == 0) said[parity][warp] = mark;
+    if (kGrows && PASS != kMaps && warp == 0) carries[parity][lane] = carry;
     __syncthreads();
     if constexpr (PASS == kCluster || PASS == kMaps) {
       // this block's map
@@ -530,14 +699,23 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       bool any = false;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const bool begun = begins[parity][w];
+        const bool begun = said[parity][w];
         const Affine<V> f = maps[parity][w][lane];
         any |= begun;
         block = {block.A * f.A, apply(f, begun, block.H)};
       }
       if constexpr (PASS == kMaps) {
-        whole = {whole.A * block.A, apply(block, any, whole.H)};
-        whole_begins |= any;
+        const Vec<V> A = whole.A * block.A;
+        if (kGrows && (whole_said & kWide ||
+                       __any_sync(~0u, !finite(block.A) || (!whole_said && !any && !finite(A))))) {
+          const Said<V> mine = s.said_of(maps[parity][warp][lane], m, first);
+          const Said<V> both = joined({whole, whole_said}, wide_block(wide_maps, wide_said, mine.map, mine.said));
+          whole = both.map;
+          whole_said = both.said;
+        } else {
+          whole = {A, apply(block, any, whole.H)};
+          if (any) whole_said = kBegins;
+        }
         m = next_m, first = next_first, all = next_all, base += span, parity ^= 1;
         return;
       }
@@ -549,26 +727,65 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       for (int r = warp; r < ranks; r += kWarps) {  // to every block of the cluster
         const unsigned there = of_rank(barrier, r);
         send(of_rank(shared_address(&rank_maps[parity][rank][lane]), r), there, block);
-        if (lane == 0) send(of_rank(shared_address(&rank_begins[parity][rank]), r), there, (int)any);
+        if (lane == 0) send(of_rank(shared_address(&rank_said[parity][rank]), r), there, (int)any);
       }
       if (!arrived(barrier, phase)) carry = splat<V>(NAN);
       phase ^= parity;
     }
     // the value carried into this warp's steps, and past all blocks' steps
     Vec<V> value = carry;
+    [[maybe_unused]] Vec<V> A = splat<V>(1.0f);  // finite where all are
+    [[maybe_unused]] int seen = 0;
     if constexpr (PASS == kCluster) {
       for (int r = 0; r < ranks; ++r) {
+        const Affine<V> f = rank_maps[parity][r][lane];
         if (r == rank) value = carry;
-        carry = apply(rank_maps[parity][r][lane], rank_begins[parity][r], carry);
+        carry = apply(f, rank_said[parity][r], carry);
+        if (kGrows) A = A * f.A;
       }
 #pragma unroll
       for (int w = 0; w < kWarps - 1; ++w)
-        if (w < warp) value = apply(maps[parity][w][lane], begins[parity][w], value);
+        if (w < warp) value = apply(maps[parity][w][lane], said[parity][w], value);
     } else {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w == warp) value = carry;
-        carry = apply(maps[parity][w][lane], begins[parity][w], carry);
+        const Affine<V> f = maps[parity][w][lane];
+        const int of = said[parity][w];
+        if (kMarked) seen |= of;
+        else if (kGrows) A = A * f.A;
+        carry = apply(f, of & kBegins, carry);
+      }
+    }
+    // the same for all warps of the block, or the cluster
+    if (kMarked ? (seen & kWide) != 0 : kGrows && __any_sync(~0u, !finite(A))) {
+      // Where two rows of registers for each step are all there are, what the calls would have to keep is
+      // read and reduced again (32 x 4096 x 512 bf16 73 us, 102 with it kept) -- but for entry states, for
+      // another warp may be about to write them.
+      constexpr bool kAgain = L * V >= 32;
+      [[maybe_unused]] volatile float kept[kAgain ? L * V : 1];
+      if (kAgain && m.enters)
+#pragma unroll
+        for (int i = 0; i < L * V; ++i) kept[i] = s.add[i / V].get(i % V);
+      const Said<V> mine = s.said_of(maps[parity][warp][lane], m, first);
+      Carried<V> c;
+      if constexpr (PASS == kCluster) {
+        c = wide_exchange(wide_maps, wide_said, &counted[2], mine.map, mine.said, ranks, rank, wide_phase,
+                          carries[parity][lane]);
+        wide_phase ^= 1;
+      } else {
+        c = wide_round(wide_maps, wide_said, mine.map, mine.said, carries[parity][lane]);
+      }
+      carry = c.after, value = c.before;
+      if constexpr (kAgain) {
+        s.template load<false>(rows, first);
+        s.template reduce<false>(rows, m);
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+          if (m.enters >> i & 1)
+#pragma unroll
+            for (int v = 0; v < V; ++v) s.add[i].set(v, kept[i * V + v]);
+        if (base + span < to) s.template load<false>(next, next_first);
       }
     }
     if (all && !marked) s.template write<true, false>(rows, m, first, value);
@@ -591,7 +808,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
 #pragma unroll
       for (int v = 0; v < V; ++v)
         cut.maps[(b * cut.parts + part) * d.channels + s.c + v] = {whole.A.get(v), whole.H.get(v)};
-    if (lane == 0 && tile == 0) cut.begins[b * cut.parts + part] = whole_begins;
+    if (lane == 0) cut.said[(b * cut.parts + part) * cut.tiles + tile] = whole_said;
   }
 }
 
@@ -791,7 +1008,7 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
     cut.part_steps = (spans + cut.parts - 1) / cut.parts * span;
     cut.parts = (int)((d.length + cut.part_steps - 1) / cut.part_steps);
     cut.maps = (float2*)d.workspace;
-    cut.begins = (int*)(cut.maps + d.batch * cut.parts * d.channels);
+    cut.said = (int*)(cut.maps + d.batch * cut.parts * d.channels);
     const cudaError_t e = launch<T, V, L, FORM, BACK, kMaps>(d, cut, stream);
     return e != cudaSuccess ? e : launch<T, V, L, FORM, BACK, kFromMaps>(d, cut, stream);
   }
@@ -851,7 +1068,8 @@ int64_t scan_workspace(int64_t batch, int64_t length, int64_t channels) {
     for (int64_t steps : {4, 8, 16})
       parts = std::max<int64_t>(parts, parts_of(batch * ((channels + width - 1) / width),
                                                 (length + kWarps * steps - 1) / (kWarps * steps)));
-  return parts > 1 ? (batch * parts * (channels * (int64_t)sizeof(float2) + 4) + 15) / 16 * 16 : 0;
+  const int64_t tiles = (channels + 31) / 32, words = 2 * channels + tiles;  // of a part: its maps, what is said
+  return parts > 1 ? (batch * parts * words * 4 + 15) / 16 * 16 : 0;
 }
 }  // namespace tb
 
