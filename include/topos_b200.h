@@ -325,13 +325,16 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
  *  - Outputs do not overlap inputs or each other, except where an operator allows it.
  *  - Packed batches: `offsets` holds sequences + 1 ascending row numbers; rows
  *    [offsets[s], offsets[s + 1]) are sequence s, which may be empty.  Rows before the first or
- *    behind the last offset belong to none and their outputs are left as they were. */
+ *    behind the last offset belong to none; their outputs are left as they were, or set to 0 where
+ *    `clear` names the array. */
 
 /* How the gate array of the gated scan is read. */
 enum {
   TB_SCAN_DIRECT = 0,   /* h_t = gate_t h_{t-1} + x_t */
   TB_SCAN_SIGMOID = 1   /* a = sigmoid(gate_t): h_t = a h_{t-1} + (1 - a) x_t */
 };
+/* tb_scan_desc.clear: outputs that are 0 at rows of no sequence. */
+enum { TB_SCAN_CLEAR_H = 1, TB_SCAN_CLEAR_DGATE = 2, TB_SCAN_CLEAR_DX = 4 };
 typedef struct tb_scan_desc {
   int64_t element, form;
   int64_t batch, length, channels;  /* arrays [batch][length][channels] */
@@ -352,6 +355,7 @@ typedef struct tb_scan_desc {
   float* dstate;                    /* gradient of state; NULL = not wanted */
   void* workspace;                  /* tb_gated_scan_workspace bytes, or NULL */
   int64_t workspace_bytes;
+  int64_t clear;                    /* TB_SCAN_CLEAR_* together, or 0 */
 } tb_scan_desc;
 /* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
  * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
@@ -434,6 +438,8 @@ typedef struct tb_policy_desc {
  * gradient of 0.  `gradient` may be `logits` with its stride. */
 int tb_policy_loss(const tb_policy_desc* desc, void* stream);
 
+/* tb_preference_desc.clear: outputs that are 0 at rows of no answer. */
+enum { TB_PREFERENCE_CLEAR_LOGP = 1, TB_PREFERENCE_CLEAR_GRADIENT = 2 };
 typedef struct tb_preference_desc {
   int64_t element, rows, vocab, pairs;
   int64_t logits_stride, gradient_stride;
@@ -451,6 +457,7 @@ typedef struct tb_preference_desc {
   void* gradient;                   /* rows x vocab; NULL = not wanted */
   void* workspace;                  /* tb_preference_workspace bytes */
   int64_t workspace_bytes;
+  int64_t clear;                    /* TB_PREFERENCE_CLEAR_* together, or 0 */
 } tb_preference_desc;
 /* Paired log-ratio loss with its gradient: m_i = beta (ratio_i - ratio_{pairs + i}),
  * loss = sum_i weight_i (-(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)).

@@ -70,7 +70,7 @@ TbScanDesc = _request(
     longs="element form batch length channels sequences gate_strides:2 x_strides:2 h_strides:2 "
           "dh_strides:2 dgate_strides:2 dx_strides:2",
     pointers="gate x h offsets state final_state dh dfinal dgate dx dstate workspace",
-    longs_last="workspace_bytes")
+    longs_last="workspace_bytes clear")
 TbRotateDesc = _request(
     "TbRotateDesc",
     longs="element style batch length q_heads k_heads dim turned table_rows q_strides:3 "
@@ -89,7 +89,7 @@ TbPreferenceDesc = _request(
     longs="element rows vocab pairs logits_stride gradient_stride",
     doubles="scale beta smoothing",
     pointers="logits targets offsets ref_logp weights loss ratios logp gradient workspace",
-    longs_last="workspace_bytes")
+    longs_last="workspace_bytes clear")
 
 
 def request_format(desc) -> str:

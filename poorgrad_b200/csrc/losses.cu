@@ -619,7 +619,10 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_preference_rows(tb_preference_desc d) {
   pdl_entry();
   const int64_t n = blockIdx.x;
-  if (!scored(d, n)) return;
+  if (!scored(d, n)) {
+    if (threadIdx.x == 0 && d.clear & TB_PREFERENCE_CLEAR_LOGP) d.logp[n] = 0.0f;
+    return;
+  }
   const int64_t t = d.targets[n];
   const float scale = (float)d.scale;
   RowStats s{0.0f, 0.0f};
@@ -640,7 +643,11 @@ template <typename T, int ITEMS>
 __global__ void __launch_bounds__(256) k_preference_rows_warps(tb_preference_desc d) {
   pdl_entry();
   const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (n >= d.rows || !scored(d, n)) return;
+  if (n >= d.rows) return;
+  if (!scored(d, n)) {
+    if (threadIdx.x % 32 == 0 && d.clear & TB_PREFERENCE_CLEAR_LOGP) d.logp[n] = 0.0f;
+    return;
+  }
   const int64_t t = d.targets[n];
   const float scale = (float)d.scale;
   RowStats s{0.0f, 0.0f};
@@ -724,14 +731,17 @@ __global__ void __launch_bounds__(THREADS) k_preference_gradient(tb_preference_d
   if (blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(d);
   // from the last row back: the rows that were read last are still in the L2 cache
   const int64_t n = d.rows - 1 - blockIdx.x;
-  if (!scored(d, n)) return;
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
+  if (!scored(d, n)) {
+    if (d.clear & TB_PREFERENCE_CLEAR_GRADIENT) zero_row<T, THREADS>(out, z, row);
+    return;
+  }
   const PreferenceScratch scratch(d);
   const RowStats s = scratch.stats[n];
   const int64_t t = d.targets[n];
   const float slope = t < d.vocab ? scratch.slopes[n] : NAN;
-  const T* z = (const T*)d.logits + n * d.logits_stride;
-  T* out = (T*)d.gradient + n * d.gradient_stride;
-  const RowShare<T> row(z, d.vocab, 0, 1, INT64_MAX / 2);
   if (s.sum == 0.0f) zero_row<T, THREADS>(out, z, row);
   else stream_gradient<T, THREADS>(z, row, RowGradient<T>(out, z, s, (float)d.scale, slope, t));
 }
@@ -740,12 +750,16 @@ __global__ void __launch_bounds__(256) k_preference_gradient_warps(tb_preference
   pdl_entry();
   if (blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(d);
   const int64_t n = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (n >= d.rows || !scored(d, n)) return;
+  if (n >= d.rows) return;
+  const T* z = (const T*)d.logits + n * d.logits_stride;
+  T* out = (T*)d.gradient + n * d.gradient_stride;
+  if (!scored(d, n)) {
+    if (d.clear & TB_PREFERENCE_CLEAR_GRADIENT) zero_warp_row(out, d.vocab);
+    return;
+  }
   const PreferenceScratch scratch(d);
   const RowStats s = scratch.stats[n];
   const int64_t t = d.targets[n];
-  const T* z = (const T*)d.logits + n * d.logits_stride;
-  T* out = (T*)d.gradient + n * d.gradient_stride;
   if (s.sum == 0.0f) {
     zero_warp_row(out, d.vocab);
     return;
@@ -924,6 +938,8 @@ int preference_loss(const tb_preference_desc* desc, void* stream) {
   if (d.pairs < 1 || d.pairs > INT32_MAX / 2) return call.invalid("pairs out of range");
   if (!(d.beta > 0) || d.beta > 3e38) return call.invalid("beta is positive and finite");
   if (!(d.smoothing >= 0 && d.smoothing < 1)) return call.invalid("smoothing lies in [0, 1)");
+  if (d.clear & ~(TB_PREFERENCE_CLEAR_LOGP | TB_PREFERENCE_CLEAR_GRADIENT))
+    return call.invalid("unknown array to clear");
   if (!words_ok({d.loss, d.ratios, d.offsets}) || !aligned_to(d.weights, 4) ||
       (d.rows > 0 && !words_ok({d.targets, d.ref_logp, d.logp})))
     return call.invalid("a row array is NULL or unaligned");

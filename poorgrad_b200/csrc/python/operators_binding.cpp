@@ -191,6 +191,7 @@ PyObject* gated_scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   e.strides(gate, d.gate_strides);
   e.strides(x, d.x_strides);
   e.strides(out, d.h_strides);
+  d.clear = given(v[5]) ? 0 : TB_SCAN_CLEAR_H;  // new arrays hold nothing to leave as it was
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan(&d, a.stream()), "tb_gated_scan");
   return tuple_of(out, final_state);
@@ -229,6 +230,7 @@ PyObject* gated_scan_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   e.strides(dh, d.dh_strides);
   e.strides(dgate, d.dgate_strides);
   e.strides(dx, d.dx_strides);
+  d.clear = (given(v[8]) ? 0 : TB_SCAN_CLEAR_DGATE) | (given(v[9]) ? 0 : TB_SCAN_CLEAR_DX);
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan_backward(&d, a.stream()), "tb_gated_scan_backward");
   return tuple_of(dgate, dx, dstate);
@@ -432,6 +434,7 @@ PyObject* preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.ratios = (float*)ratios.data_ptr();
   d.logp = (float*)logp.data_ptr();
   d.workspace = scratch.data_ptr();
+  d.clear = TB_PREFERENCE_CLEAR_LOGP | (v[8] == Py_True ? TB_PREFERENCE_CLEAR_GRADIENT : 0);
   checked(tb_preference_loss(&d, a.stream()), "tb_preference_loss");
   return tuple_of(loss, ratios, logp, gradient);
   END_HANDLE_TH_ERRORS

@@ -549,6 +549,20 @@ struct Scan {
     return {map, kWide};
   }
 
+  // Zeros to the rows before the first and behind the last sequence, for worker `mine` of `all`.
+  __device__ __forceinline__ void clear_outside(int mine, int all) const {
+    const int length = (int)d.length, begin = (int)clamped_offset(d, 0), end = (int)clamped_offset(d, d.sequences);
+    for (int t = mine; t < length; t += all) {
+      if (t >= begin && t < end) {
+        t += (end - 1 - t) / all * all;  // to the last of these rows that is this worker's
+        continue;
+      }
+      if (!BACK && d.clear & TB_SCAN_CLEAR_H) *(Row*)at(d.h, d.h_strides, t) = Row{};
+      if (BACK && d.clear & TB_SCAN_CLEAR_DGATE) *(Row*)at(d.dgate, d.dgate_strides, t) = Row{};
+      if (BACK && d.clear & TB_SCAN_CLEAR_DX) *(Row*)at(d.dx, d.dx_strides, t) = Row{};
+    }
+  }
+
   // ALL as in load(); MARKED: some step enters or leaves a sequence or lies outside all of them.
   template <bool ALL, bool MARKED>
   __device__ __forceinline__ void write(const Rows& r, const Marks& m, int first, Vec<V> value) {
@@ -803,6 +817,9 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       run(rows, rows);
     }
   }
+  // at the end, where no register is held (among the outputs it took a tenth of a backward pass)
+  if (PASS != kMaps && d.clear && d.sequences && s.in)
+    s.clear_outside((part * ranks + rank) * kWarps + warp, cut.parts * ranks * kWarps);
   if (PASS == kMaps && warp == 0) {
     if (s.in)
 #pragma unroll
@@ -924,6 +941,7 @@ const char* check(const tb_scan_desc& d, bool backward) {
     return "extents out of range";
   if (d.sequences ? !d.offsets || d.batch != 1 : d.offsets != nullptr)
     return "packed sequences come with offsets and a batch of 1";
+  if (d.clear & ~(TB_SCAN_CLEAR_H | TB_SCAN_CLEAR_DGATE | TB_SCAN_CLEAR_DX)) return "unknown array to clear";
   const bool reads_x = !backward || d.form == TB_SCAN_SIGMOID;
   if (!strides_ok(d, d.gate_strides, false) || (reads_x && !strides_ok(d, d.x_strides, false)) ||
       !strides_ok(d, d.h_strides, !backward) ||

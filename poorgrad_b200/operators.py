@@ -49,7 +49,8 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
     ``form="direct"``: a is ``gate`` and b is ``x``.  ``form="sigmoid"``: a is the sigmoid of
     ``gate`` and b is ``(1 - a) x``.  ``gate`` and ``x`` are ``[batch, length, channels]``, or a
     packed ``[rows, channels]`` whose sequences ``offsets`` (int32, sequences + 1 rising row
-    numbers) delimits; rows outside every sequence are left as they were.  ``state`` (float32,
+    numbers) delimits; rows outside every sequence are 0, or left as they were in a given array.
+    ``state`` (float32,
     ``[batch or sequences, channels]``, zeros when None) comes before the first step; the returned
     final state may be written into ``state`` itself (``final_state=state``), as a decode loop
     does.  ``out`` may be ``gate`` or ``x``."""
@@ -62,7 +63,7 @@ def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, of
     """Gradients ``(dgate, dx, dstate)`` of :func:`gated_scan` from the gradient ``dh`` of its
     outputs ``h`` and ``dfinal`` of its final state (zeros when None).  ``x`` is read by the
     sigmoid form only, and may be None in the direct one.  One of ``dgate`` and ``dx`` may be
-    ``dh``."""
+    ``dh``.  Rows outside every sequence are as in :func:`gated_scan`."""
     return _native.gated_scan_backward(dh, gate, x, h, _one_of(_FORM, "form", form), state, offsets,
                                        dfinal, dgate, dx)
 
@@ -152,6 +153,7 @@ def preference_loss(logits, targets, offsets, ref_logp, *, beta: float = 0.1,
     ``ref_logp`` holds the reference model's log probability of each row.  With
     ``m = beta (ratio_chosen - ratio_rejected)`` the loss is the weighted sum (``weights`` float32
     per pair, 1 / pairs when None) of ``-(1 - smoothing) log sigmoid(m) - smoothing log sigmoid(-m)``.
-    Rows outside every answer are left as they were.  ``gradient`` as in :func:`policy_loss`."""
+    Rows outside every answer have a log probability and a gradient of 0; a given gradient array is left
+    as it was there (the logits, where it is theirs).  ``gradient`` as in :func:`policy_loss`."""
     return PreferenceLoss(*_native.preference_loss(logits, targets, offsets, ref_logp, beta,
                                                    smoothing, weights, scale, gradient))
