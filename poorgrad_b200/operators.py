@@ -61,7 +61,8 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
 def gated_scan_backward(dh, gate, x, h, *, form: str = "sigmoid", state=None, offsets=None,
                         dfinal=None, dgate=None, dx=None):
     """Gradients ``(dgate, dx, dstate)`` of :func:`gated_scan` from the gradient ``dh`` of its
-    outputs ``h`` and ``dfinal`` of its final state (zeros when None).  ``x`` is read by the
+    outputs ``h`` and ``dfinal`` of its final state (zeros when None).  ``state`` is what the scan
+    began with: a carry that was written in place (``final_state=state``) no longer is.  ``x`` is read by the
     sigmoid form only, and may be None in the direct one.  One of ``dgate`` and ``dx`` may be
     ``dh``.  Rows outside every sequence are as in :func:`gated_scan`."""
     return _native.gated_scan_backward(dh, gate, x, h, _one_of(_FORM, "form", form), state, offsets,
