@@ -105,6 +105,14 @@ struct Arrays {
   void* stream() const { return (void*)c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 };
 
+// ------------------------------------------------- arrays that a call writes
+// What autograd has to know of an array that the caller gave and a call has written.
+void written(PyObject* o) {
+  if (!o || !THPVariable_Check(o)) return;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* wrapped(const Tensor& t) { return THPVariable_Wrap(t); }
 PyObject* wrapped_or_none(const Tensor& t) {
   if (t.defined()) return wrapped(t);
@@ -194,6 +202,8 @@ PyObject* gated_scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.clear = given(v[5]) ? 0 : TB_SCAN_CLEAR_H;  // new arrays hold nothing to leave as it was
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan(&d, a.stream()), "tb_gated_scan");
+  written(v[5]);
+  written(v[6]);
   return tuple_of(out, final_state);
   END_HANDLE_TH_ERRORS
 }
@@ -233,6 +243,8 @@ PyObject* gated_scan_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.clear = (given(v[8]) ? 0 : TB_SCAN_CLEAR_DGATE) | (given(v[9]) ? 0 : TB_SCAN_CLEAR_DX);
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan_backward(&d, a.stream()), "tb_gated_scan_backward");
+  written(v[8]);
+  written(v[9]);
   return tuple_of(dgate, dx, dstate);
   END_HANDLE_TH_ERRORS
 }
@@ -296,6 +308,8 @@ PyObject* head_rotate(PyObject*, PyObject* const* v, Py_ssize_t n) {
   arguments(n, 10);
   const RotateCall call(v);
   checked(tb_head_rotate(&call.d, call.a.stream()), "tb_head_rotate");
+  written(v[8]);
+  written(v[9]);
   return tuple_of(call.q_out, call.k_out);
   END_HANDLE_TH_ERRORS
 }
@@ -321,6 +335,8 @@ PyObject* head_rotate_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
     d.workspace = scratch.data_ptr();
   }
   checked(tb_head_rotate_backward(&d, call.a.stream()), "tb_head_rotate_backward");
+  written(v[8]);
+  written(v[9]);
   return tuple_of(call.q_out, call.k_out, dq_weight, dk_weight);
   END_HANDLE_TH_ERRORS
 }
@@ -392,6 +408,7 @@ PyObject* policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.token_loss = (float*)token_loss.data_ptr();
   d.logp = (float*)logp.data_ptr();
   checked(tb_policy_loss(&d, a.stream()), "tb_policy_loss");
+  written(v[10]);
   return tuple_of(loss, token_loss, logp, gradient);
   END_HANDLE_TH_ERRORS
 }
@@ -436,6 +453,7 @@ PyObject* preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.workspace = scratch.data_ptr();
   d.clear = TB_PREFERENCE_CLEAR_LOGP | (v[8] == Py_True ? TB_PREFERENCE_CLEAR_GRADIENT : 0);
   checked(tb_preference_loss(&d, a.stream()), "tb_preference_loss");
+  written(v[8]);
   return tuple_of(loss, ratios, logp, gradient);
   END_HANDLE_TH_ERRORS
 }
