@@ -106,6 +106,63 @@ struct Arrays {
 };
 
 // ------------------------------------------------- arrays that a call writes
+// The bytes of an array, from the first to behind the last.
+struct Place {
+  const Tensor& t;
+  const char *begin, *end;
+  explicit Place(const Tensor& t) : t(t), begin((const char*)t.const_data_ptr()), end(begin) {
+    if (t.numel() == 0) return;
+    int64_t reach = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
+    end += reach * (int64_t)t.element_size();
+  }
+};
+// Whether an element of the one, `apart` elements behind the other's first, is one of the other: strides
+// `s`, `n` steps forwards of the one and `m` of the other, from axis i on.
+bool step_onto(int64_t apart, int i, const int64_t* s, const int64_t* n, const int64_t* m, int axes) {
+  if (i == axes) return apart == 0;
+  int64_t back = 0, forth = 0;  // what the axes behind this one reach
+  for (int j = i + 1; j < axes; ++j) back += m[j] * s[j], forth += n[j] * s[j];
+  // steps k of this axis that leave the rest within reach: -back <= apart - k s <= forth
+  const auto down = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+  const int64_t from = std::max(-m[i], -down(forth - apart, s[i])), to = std::min(n[i], down(apart + back, s[i]));
+  for (int64_t k = from; k <= to; ++k)
+    if (step_onto(apart - k * s[i], i + 1, s, n, m, axes)) return true;
+  return false;
+}
+// Whether two arrays of the same axes share an element.  Arrays that lie in one another's gaps with
+// strides of their own are taken to share none.
+bool meet(const Place& a, const Place& b) {
+  if (a.begin >= b.end || b.begin >= a.end) return false;
+  constexpr int kAxes = 4;
+  const int64_t size = a.t.element_size();
+  if (a.t.dim() != b.t.dim() || a.t.dim() > kAxes || b.t.element_size() != size || (b.begin - a.begin) % size)
+    return true;
+  int64_t s[kAxes], n[kAxes], m[kAxes];
+  int axes = 0;
+  for (int64_t i = 0; i < a.t.dim(); ++i) {
+    const int64_t steps = a.t.size(i) - 1, others = b.t.size(i) - 1;
+    if (steps == 0 && others == 0) continue;
+    const int64_t stride = steps ? a.t.stride(i) : b.t.stride(i);
+    if ((steps && others && a.t.stride(i) != b.t.stride(i)) || stride <= 0) return a.begin == b.begin;
+    int at = axes++;
+    for (; at > 0 && s[at - 1] < stride; --at) s[at] = s[at - 1], n[at] = n[at - 1], m[at] = m[at - 1];
+    s[at] = stride, n[at] = steps, m[at] = others;
+  }
+  return step_onto((b.begin - a.begin) / size, 0, s, n, m, axes);
+}
+bool same(const Place& a, const Place& b) {
+  if (a.begin != b.begin || a.t.sizes() != b.t.sizes()) return false;
+  for (int64_t i = 0; i < a.t.dim(); ++i)
+    if (a.t.size(i) > 1 && a.t.stride(i) != b.t.stride(i)) return false;
+  return true;
+}
+// An output may not share memory with another one or with an input; with an input that it may take
+// the place of, it shares all of it.
+void apart(const Place& a, const char* name, const Place& b, const char* other, bool in_place = false) {
+  if (meet(a, b) && !(in_place && same(a, b)))
+    refuse(std::string(name) + " shares memory with " + other + (in_place ? ", but is not the same array" : ""));
+}
 // What autograd has to know of an array that the caller gave and a call has written.
 void written(PyObject* o) {
   if (!o || !THPVariable_Check(o)) return;
@@ -199,6 +256,19 @@ PyObject* gated_scan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   e.strides(gate, d.gate_strides);
   e.strides(x, d.x_strides);
   e.strides(out, d.h_strides);
+  if (given(v[5]) || given(v[6])) {
+    const Place to(out), last(final_state), from_gate(gate), from_x(x);
+    apart(to, "out", from_gate, "gate", true);
+    apart(to, "out", from_x, "x", true);
+    apart(to, "out", last, "final_state");
+    apart(last, "final_state", from_gate, "gate");
+    apart(last, "final_state", from_x, "x");
+    if (given(v[3])) {
+      const Place state(tensor(v[3], "state"));
+      apart(last, "final_state", state, "state", true);
+      apart(to, "out", state, "state");
+    }
+  }
   d.clear = given(v[5]) ? 0 : TB_SCAN_CLEAR_H;  // new arrays hold nothing to leave as it was
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan(&d, a.stream()), "tb_gated_scan");
@@ -240,6 +310,28 @@ PyObject* gated_scan_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   e.strides(dh, d.dh_strides);
   e.strides(dgate, d.dgate_strides);
   e.strides(dx, d.dx_strides);
+  if (given(v[8]) || given(v[9])) {
+    const Place to_gate(dgate), to_x(dx), from_dh(dh), from_gate(gate), from_h(h);
+    apart(to_gate, "dgate", to_x, "dx");
+    // a row of h is read for the next step's gradient too
+    apart(to_gate, "dgate", from_h, "h");
+    apart(to_x, "dx", from_h, "h");
+    apart(to_gate, "dgate", from_dh, "dh", true);
+    apart(to_x, "dx", from_dh, "dh", true);
+    apart(to_gate, "dgate", from_gate, "gate", true);
+    apart(to_x, "dx", from_gate, "gate", true);
+    if (d.form != TB_SCAN_DIRECT) {
+      const Place from_x(tensor(v[2], "x"));
+      apart(to_gate, "dgate", from_x, "x", true);
+      apart(to_x, "dx", from_x, "x", true);
+    }
+    for (int i : {5, 7})
+      if (given(v[i])) {
+        const Place from(tensor(v[i], "state"));
+        apart(to_gate, "dgate", from, i == 5 ? "state" : "dfinal");
+        apart(to_x, "dx", from, i == 5 ? "state" : "dfinal");
+      }
+  }
   d.clear = (given(v[8]) ? 0 : TB_SCAN_CLEAR_DGATE) | (given(v[9]) ? 0 : TB_SCAN_CLEAR_DX);
   const Tensor scratch = scan_scratch(d, a);
   checked(tb_gated_scan_backward(&d, a.stream()), "tb_gated_scan_backward");
@@ -302,11 +394,29 @@ struct RotateCall {
     head_strides(k_out, d.k_out_strides);
   }
   std::vector<int64_t> k_sizes;
+  // No output in the place of anything but its own inputs.
+  void outputs_apart(PyObject* const* v, const Tensor* dq = nullptr, const Tensor* dk = nullptr) const {
+    if (!given(v[8]) && !given(v[9])) return;
+    const Place to_q(q_out), to_k(k_out), from_q(q), from_k(k);
+    apart(to_q, "q_out", to_k, "k_out");
+    apart(to_q, "q_out", from_q, "q", true);
+    apart(to_q, "q_out", from_k, "k");
+    apart(to_k, "k_out", from_k, "k", true);
+    apart(to_k, "k_out", from_q, "q");
+    if (dq) {
+      const Place grad_q(*dq), grad_k(*dk);
+      apart(to_q, "q_out", grad_q, "dq", true);
+      apart(to_q, "q_out", grad_k, "dk");
+      apart(to_k, "k_out", grad_k, "dk", true);
+      apart(to_k, "k_out", grad_q, "dq");
+    }
+  }
 };
 PyObject* head_rotate(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 10);
   const RotateCall call(v);
+  call.outputs_apart(v);
   checked(tb_head_rotate(&call.d, call.a.stream()), "tb_head_rotate");
   written(v[8]);
   written(v[9]);
@@ -324,6 +434,7 @@ PyObject* head_rotate_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
   d.dk = call.a.rows(dk, "dk", call.k_sizes);
   head_strides(dq, d.dq_strides);
   head_strides(dk, d.dk_strides);
+  call.outputs_apart(v, &dq, &dk);
   Tensor dq_weight, dk_weight, scratch;
   if (v[12] == Py_True) {
     dq_weight = call.a.made({d.dim}, at::kFloat);
@@ -352,6 +463,7 @@ Tensor gradient_of(PyObject* o, const Tensor& logits, const Arrays& a) {
   if (o == Py_False || o == Py_None) return {};
   const Tensor t = o == Py_True ? a.like(logits) : tensor(o, "gradient");
   a.rows(t, "gradient", logits.sizes());
+  if (o != Py_True) apart(Place(t), "gradient", Place(logits), "logits", true);
   return t;
 }
 

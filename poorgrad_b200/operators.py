@@ -9,7 +9,8 @@ products of a decoder's training and decode steps, on device arrays that the cal
 
 Device arrays are torch tensors (float32 or bfloat16), used as memory only: nothing here records
 gradients.  An array that is given to be written counts as changed in place, so that a backward pass
-that still needs what it held raises.  Arguments of one call live on one device; the work is enqueued on that device's current
+that still needs what it held raises; no two arrays of a call share memory unless one is written over the
+other as a function says.  Arguments of one call live on one device; the work is enqueued on that device's current
 torch stream, and outputs that are not given are allocated by torch on that stream.  A malformed
 request raises ``ValueError`` or :class:`~poorgrad_b200.backend.BackendError`; there is no CPU
 fallback.
