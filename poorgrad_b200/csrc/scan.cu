@@ -563,6 +563,22 @@ struct Scan {
     }
   }
 
+  // Sequences without a step hand their entry state on, for worker `mine` of `all`, whose lanes look at one
+  // sequence each.
+  __device__ __forceinline__ void hand_on(int mine, int all) const {
+    for (int64_t base = (int64_t)mine * 32; base < d.sequences; base += (int64_t)all * 32) {
+      const int64_t i = base + threadIdx.x % 32;
+      unsigned empty = __ballot_sync(~0u, i < d.sequences && clamped_offset(d, i + 1) <= clamped_offset(d, i));
+      for (; empty; empty &= empty - 1) {
+        const int64_t at = (base + __ffs(empty) - 1) * d.channels + c;
+        const Vec<V> e = state_at(entry_state, at);
+        if (in)
+#pragma unroll
+          for (int v = 0; v < V; ++v) exit_state[at + v] = e.get(v);
+      }
+    }
+  }
+
   // ALL as in load(); MARKED: some step enters or leaves a sequence or lies outside all of them.
   template <bool ALL, bool MARKED>
   __device__ __forceinline__ void write(const Rows& r, const Marks& m, int first, Vec<V> value) {
@@ -633,18 +649,6 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&counted[i])) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     cg::this_cluster().sync();
-  }
-
-  // sequences without a step hand their entry state on
-  if (PASS != kMaps && s.exit_state && rank == 0 && part == 0 && (d.sequences || d.length == 0)) {
-    const int64_t count = d.sequences ? d.sequences : 1;
-    for (int64_t i = warp; i < count; i += kWarps) {
-      if (d.sequences && clamped_offset(d, i + 1) > clamped_offset(d, i)) continue;
-      const int64_t at = (d.sequences ? i : b) * d.channels + s.c;
-      const Vec<V> e = s.state_at(s.entry_state, at);
-      if (s.in)
-        for (int v = 0; v < V; ++v) s.exit_state[at + v] = e.get(v);
-    }
   }
 
   Vec<V> carry = splat<V>(0.0f);
@@ -817,9 +821,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       run(rows, rows);
     }
   }
-  // at the end, where no register is held (among the outputs it took a tenth of a backward pass)
-  if (PASS != kMaps && d.clear && d.sequences && s.in)
-    s.clear_outside((part * ranks + rank) * kWarps + warp, cut.parts * ranks * kWarps);
+  // at the end, where no register is held (zeros among the outputs took a tenth of a backward pass) and no
+  // block waits for this one
+  if (PASS != kMaps && d.sequences) {
+    const int worker = (part * ranks + rank) * kWarps + warp, workers = cut.parts * ranks * kWarps;
+    if (s.exit_state) s.hand_on(worker, workers);
+    if (d.clear && s.in) s.clear_outside(worker, workers);
+  }
   if (PASS == kMaps && warp == 0) {
     if (s.in)
 #pragma unroll
