@@ -319,7 +319,8 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
  *    element size; strides count elements and are not negative; the last axis has stride 1.
  *  - Results do not depend on scheduling: the same call gives the same bits.
  *  - A malformed request answers TB_INVALID before anything is enqueued, a launch failure
- *    TB_RUNTIME (and poisons the library).  Index values on the device (offsets, positions,
+ *    TB_RUNTIME (and poisons the library), and what goes wrong on the device later is told by
+ *    tb_operators_synchronize.  Index values on the device (offsets, positions,
  *    targets) are not seen by the host: the kernels keep every access in bounds whatever they
  *    hold, and each operator says what a bad one gives.
  *  - Outputs do not overlap inputs or each other, except where an operator allows it.
@@ -327,6 +328,10 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
  *    [offsets[s], offsets[s + 1]) are sequence s, which may be empty.  Rows before the first or
  *    behind the last offset belong to none; their outputs are left as they were, or set to 0 where
  *    `clear` names the array. */
+
+/* Waits for the stream's work.  TB_RUNTIME (and a poisoned library) where it failed, or where a wait
+ * between blocks of an operator ever ran out on the current device.  Not for a stream under capture. */
+int tb_operators_synchronize(void* stream);
 
 /* How the gate array of the gated scan is read. */
 enum {
@@ -361,8 +366,9 @@ typedef struct tb_scan_desc {
  * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
  * final state is its state.  Gates of the direct form may be larger than 1: steps are taken together, but
  * outputs are finite wherever the recurrence is.  Steps that together shrink what they are handed by
- * more than 2^126 may hand on nothing of it.  A wait between blocks that runs out (4 s, a fault) makes the outputs
- * behind it NaN. */
+ * more than 2^126 may hand on nothing of it.  Where a wait between the
+ * blocks of one sequence runs out (4 s; nothing but a fault explains it), the values carried over from
+ * there on are NaN, and tb_operators_synchronize tells of it. */
 int tb_gated_scan(const tb_scan_desc* desc, void* stream);
 /* Its gradients from dh and dfinal: with g_t = dh_t + a_{t+1} g_{t+1}, d a_t = g_t h_{t-1},
  * d b_t = g_t, chained through the form.  Reads the saved outputs h.  `dstate` may be `dfinal`;

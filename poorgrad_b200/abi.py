@@ -274,6 +274,7 @@ def load_library() -> C.CDLL:
         "tb_gemm_f32_noalloc": (C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.c_void_p,
                                           C.POINTER(C.c_int64), C.c_int64, C.c_int64, C.c_int64,
                                           C.c_void_p, C.c_void_p]),
+        "tb_operators_synchronize": (C.c_int, [P]),
         # the operators' requests are passed as packed bytes
         "tb_gated_scan": (C.c_int, [C.c_char_p, P]),
         "tb_gated_scan_backward": (C.c_int, [C.c_char_p, P]),

@@ -306,6 +306,7 @@ __device__ __noinline__ Vec<V> wide_run(const char* gate, int64_t bytes, int cou
 template <int V>
 struct Carried {
   Vec<V> after, before;
+  bool arrived = true;
 };
 template <int V>
 __device__ __forceinline__ Carried<V> wide_walk(const Affine<V> (*maps)[32], const int* said, int count, int at,
@@ -346,6 +347,7 @@ struct Cut {
   int64_t part_steps;
   float2* maps;  // (A, H), [batch][parts][channels], parts > 1
   int* said;     // [batch][parts][tiles]
+  unsigned wait_ns;  // what a wait between blocks may take; 0 lets each run out at once
 };
 
 // A launch's part: a block walks its columns alone, or the blocks of a cluster together; or one of
@@ -382,11 +384,12 @@ __device__ __forceinline__ void send(unsigned to, unsigned barrier, int v) {
 // Set where a wait of the exchange ran out.
 __device__ int g_wait_expired;
 
-// Whether all that was expected has arrived; false after 4 seconds, which nothing but a fault
-// explains (the caller then makes its outputs NaN and goes on).
-__device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
+// Whether all that was expected has arrived; false after `limit` (4 seconds), which nothing but a fault
+// explains.  The value carried into the block is NaN for the lane from there on, and it neither waits nor
+// sends again, so that the waits for its maps run out too, and none takes a later round's for them.
+__device__ __forceinline__ bool arrived(unsigned barrier, int phase, unsigned limit) {
   unsigned long long since = 0;
-  while (true) {
+  while (limit != 0) {
     int done;
     asm volatile(
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
@@ -398,18 +401,28 @@ __device__ __forceinline__ bool arrived(unsigned barrier, int phase) {
     unsigned long long now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (since == 0) since = now;
-    if (now - since > 4000000000ull) {
-      g_wait_expired = 1;
-      return false;
-    }
+    if (now - since > limit) break;
   }
+  g_wait_expired = 1;
+  return false;
+}
+// The end of a block of which a wait ran out: its shared memory stays until nothing can be on its way to it.
+// The barrier waits for no block that has left, and the others come to it or leave within their own limits;
+// what they sent before has landed long before a millisecond is over.
+__device__ __noinline__ void leave_late() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  unsigned long long now, since;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(since));
+  do {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+  } while (now - since < 1000000);
 }
 
 // As wide_round, by the warps of a cluster's blocks.  Each warp sends its map to all blocks by itself, so that
 // none waits for another but at the barrier, where waits are bounded.
 template <int V>
 __device__ __noinline__ Carried<V> wide_exchange(Affine<V> (*maps)[32], int* said, uint64_t* counted, Affine<V> map,
-                                                 int of, int ranks, int rank, int phase, Vec<V> carry) {
+                                                 int of, int ranks, int rank, int phase, unsigned limit, Vec<V> carry) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, mine = rank * kWarps + warp;
   const unsigned barrier = shared_address(counted);
   if (threadIdx.x == 0)
@@ -421,7 +434,7 @@ __device__ __noinline__ Carried<V> wide_exchange(Affine<V> (*maps)[32], int* sai
     send(of_rank(shared_address(&maps[mine][lane]), r), there, map);
     if (lane == 0) send(of_rank(shared_address(&said[mine]), r), there, of);
   }
-  if (!arrived(barrier, phase)) return {splat<V>(NAN), splat<V>(NAN)};
+  if (__any_sync(~0u, !arrived(barrier, phase, limit))) return {carry, carry, false};
   return wide_walk(maps, said, ranks * kWarps, mine, carry);
 }
 
@@ -680,6 +693,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
 
   int parity = 0, phase = 0;  // of the exchange's buffers, and of their barriers
   [[maybe_unused]] int wide_phase = 0;
+  [[maybe_unused]] int reached = ranks;  // blocks that this one exchanges maps with: 0 once a wait has run out
+  [[maybe_unused]] unsigned wait_ns = cut.wait_ns;
   const int from = (int)(part * cut.part_steps), to = (int)min(from + cut.part_steps, d.length);
   const int span = ranks * kWarps * L;
   // a part is a whole number of spans, so that no step belongs to two
@@ -714,13 +729,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
     if constexpr (PASS == kCluster || PASS == kMaps) {
       // this block's map
       Affine<V> block{splat<V>(1.0f), splat<V>(0.0f)};
-      bool any = false;
+      int any = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const bool begun = said[parity][w];
+        const int of = said[parity][w];
         const Affine<V> f = maps[parity][w][lane];
-        any |= begun;
-        block = {block.A * f.A, apply(f, begun, block.H)};
+        any |= of;
+        block = {block.A * f.A, apply(f, of & kBegins, block.H)};
       }
       if constexpr (PASS == kMaps) {
         const Vec<V> A = whole.A * block.A;
@@ -731,23 +746,26 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
           whole = both.map;
           whole_said = both.said;
         } else {
-          whole = {A, apply(block, any, whole.H)};
+          whole = {A, apply(block, any & kBegins, whole.H)};
           if (any) whole_said = kBegins;
         }
         m = next_m, first = next_first, all = next_all, base += span, parity ^= 1;
         return;
       }
       const unsigned barrier = shared_address(&counted[parity]);
-      if (threadIdx.x == 0)
+      if (threadIdx.x == 0 && reached)
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier),
                      "r"(ranks * (32 * (int)sizeof(Affine<V>) + 4))
                      : "memory");
-      for (int r = warp; r < ranks; r += kWarps) {  // to every block of the cluster
+      for (int r = warp; r < reached; r += kWarps) {  // to every block of the cluster
         const unsigned there = of_rank(barrier, r);
         send(of_rank(shared_address(&rank_maps[parity][rank][lane]), r), there, block);
-        if (lane == 0) send(of_rank(shared_address(&rank_said[parity][rank]), r), there, (int)any);
+        if (lane == 0) send(of_rank(shared_address(&rank_said[parity][rank]), r), there, any & kBegins);
       }
-      if (!arrived(barrier, phase)) carry = splat<V>(NAN);
+      if (!arrived(barrier, phase, wait_ns)) {
+        carry = splat<V>(NAN);
+        reached = wait_ns = 0;
+      }
       phase ^= parity;
     }
     // the value carried into this warp's steps, and past all blocks' steps
@@ -755,15 +773,15 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
     [[maybe_unused]] Vec<V> A = splat<V>(1.0f);  // finite where all are
     [[maybe_unused]] int seen = 0;
     if constexpr (PASS == kCluster) {
-      for (int r = 0; r < ranks; ++r) {
+      for (int r = 0; r < reached; ++r) {
         const Affine<V> f = rank_maps[parity][r][lane];
         if (r == rank) value = carry;
-        carry = apply(f, rank_said[parity][r], carry);
+        carry = apply(f, rank_said[parity][r] & kBegins, carry);
         if (kGrows) A = A * f.A;
       }
 #pragma unroll
       for (int w = 0; w < kWarps - 1; ++w)
-        if (w < warp) value = apply(maps[parity][w][lane], said[parity][w], value);
+        if (w < warp) value = apply(maps[parity][w][lane], said[parity][w] & kBegins, value);
     } else {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
@@ -775,7 +793,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
         carry = apply(f, of & kBegins, carry);
       }
     }
-    // the same for all warps of the block, or the cluster
+    // the same for all warps of the block, or the cluster; never for what a lane found whose wait ran out, as
+    // the other blocks may have left
     if (kMarked ? (seen & kWide) != 0 : kGrows && __any_sync(~0u, !finite(A))) {
       // Where two rows of registers for each step are all there are, what the calls would have to keep is
       // read and reduced again (32 x 4096 x 512 bf16 73 us, 102 with it kept) -- but for entry states, for
@@ -789,8 +808,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
       Carried<V> c;
       if constexpr (PASS == kCluster) {
         c = wide_exchange(wide_maps, wide_said, &counted[2], mine.map, mine.said, ranks, rank, wide_phase,
-                          carries[parity][lane]);
+                          wait_ns, carries[parity][lane]);
         wide_phase ^= 1;
+        if (!c.arrived) {
+          c = {splat<V>(NAN), splat<V>(NAN)};
+          reached = wait_ns = 0;
+        }
       } else {
         c = wide_round(wide_maps, wide_said, mine.map, mine.said, carries[parity][lane]);
       }
@@ -828,6 +851,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) k_scan(tb_scan_desc d, Cut cut
     if (s.exit_state) s.hand_on(worker, workers);
     if (d.clear && s.in) s.clear_outside(worker, workers);
   }
+  if (PASS == kCluster && __syncthreads_or(reached == 0)) leave_late();
   if (PASS == kMaps && warp == 0) {
     if (s.in)
 #pragma unroll
@@ -993,6 +1017,8 @@ bool lanes_fit(const tb_scan_desc& d, bool backward, int64_t size, int64_t bytes
   return true;
 }
 
+std::atomic<unsigned> g_wait_ns{4000000000u};
+
 template <typename T, int V, int L, int FORM, bool BACK, int PASS>
 cudaError_t launch(const tb_scan_desc& d, const Cut& cut, cudaStream_t stream) {
   const int64_t blocks = d.batch * cut.parts * cut.tiles * cut.ranks;
@@ -1023,6 +1049,7 @@ template <typename T, int V, int L, int FORM, bool BACK>
 cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
   const int64_t span = kWarps * L;
   Cut cut = {};
+  cut.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   cut.tiles = (int)((d.channels + 32 * V - 1) / (32 * V));
   cut.ranks = cut.parts = 1;
   cut.part_steps = std::max<int64_t>(d.length, 1);
@@ -1097,6 +1124,16 @@ int64_t scan_workspace(int64_t batch, int64_t length, int64_t channels) {
   const int64_t tiles = (channels + 31) / 32, words = 2 * channels + tiles;  // of a part: its maps, what is said
   return parts > 1 ? (batch * parts * words * 4 + 15) / 16 * 16 : 0;
 }
+
+int operators_synchronize(void* stream) {
+  OperatorCall call("tb_operators_synchronize", stream);
+  if (const int code = call.ready()) return code;
+  int expired = 0;
+  cudaError_t e = cudaStreamSynchronize(call.stream());
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&expired, g_wait_expired, sizeof expired);
+  if (e == cudaSuccess && expired) e = cudaErrorLaunchTimeout;
+  return call.finish(e);
+}
 }  // namespace tb
 
 extern "C" int tb_gated_scan(const tb_scan_desc* desc, void* stream) {
@@ -1109,8 +1146,13 @@ extern "C" int64_t tb_gated_scan_workspace(int64_t batch, int64_t length, int64_
   return tb::scan_workspace(batch, length, channels);
 }
 
-// ---- internal hook for tests (not part of the public ABI): whether a wait between the blocks of a
+extern "C" int tb_operators_synchronize(void* stream) {
+  return tb::guarded([&] { return tb::operators_synchronize(stream); });
+}
+
+// ---- internal hooks for tests (not part of the public ABI): the limit of a scan's waits, and whether a wait between the blocks of a
 // cluster ever ran out on the current device (1), or the flag cannot be read (-1).
+extern "C" void tbx_scan_wait_limit(int64_t ns) { tb::g_wait_ns = (unsigned)ns; }
 extern "C" int tbx_scan_error(void) {
   int expired = 0;
   return cudaMemcpyFromSymbol(&expired, tb::g_wait_expired, sizeof expired) == cudaSuccess ? expired : -1;

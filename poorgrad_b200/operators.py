@@ -6,6 +6,7 @@ products of a decoder's training and decode steps, on device arrays that the cal
   position rotation; :func:`rotation_table` makes its cosines and sines
 - :func:`token_logp`, :func:`policy_loss`, :func:`preference_loss` -- losses over a vocabulary
   with their gradients by the logits
+- :func:`synchronize` -- waits for the work, and raises what went wrong in it
 
 Device arrays are torch tensors (float32 or bfloat16), used as memory only: nothing here records
 gradients.  An array that is given to be written counts as changed in place, so that a backward pass
@@ -22,7 +23,7 @@ from typing import NamedTuple, Optional
 import numpy as np
 import torch
 
-from .abi import library_path
+from .abi import library_path, load_library
 from .backend import BackendError
 
 try:
@@ -41,6 +42,16 @@ def _one_of(names: dict, name: str, value):
     if code is None:
         raise ValueError(f"{name}: one of {sorted(names)} is expected, got {value!r}")
     return code
+
+
+def synchronize(device=None) -> None:
+    """Waits for the current stream of ``device`` (the current one when None), and raises
+    :class:`~poorgrad_b200.backend.BackendError` where its work failed or a wait between the blocks of an
+    operator ever ran out there."""
+    with torch.cuda.device(device):
+        code = load_library().tb_operators_synchronize(torch.cuda.current_stream().cuda_stream)
+    if code != 0:
+        raise BackendError(code, "tb_operators_synchronize")
 
 
 # ------------------------------------------------------------------ gated scan
