@@ -236,7 +236,12 @@ bool poisoned() {
 }
 void poison_library(const char* why) {
   g_error = why;
-  poison(why);
+  // a process without a plan may not have asked for the state before its first failure
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (g_state < 0 || g_state == TB_OK) {
+    g_state = TB_POISONED;
+    g_status_message = why;
+  }
 }
 }  // namespace tb
 
