@@ -318,11 +318,11 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
  *    or batch f64), rounded once to the storage type.  Base addresses are multiples of the
  *    element size; strides count elements and are not negative; the last axis has stride 1.
  *  - Results do not depend on scheduling: the same call gives the same bits.
- *  - A malformed request answers TB_INVALID before anything is enqueued, a launch failure
- *    TB_RUNTIME (and poisons the library), and what goes wrong on the device later is told by
- *    tb_operators_synchronize.  Index values on the device (offsets, positions,
- *    targets) are not seen by the host: the kernels keep every access in bounds whatever they
- *    hold, and each operator says what a bad one gives.
+ *  - A malformed request, or one that a stream's capture does not take, answers TB_INVALID before
+ *    anything is enqueued, a launch failure TB_RUNTIME (and poisons the library), and what goes wrong
+ *    on the device later is told by tb_operators_synchronize.  Index values on the device (offsets,
+ *    positions, targets) are not seen by the host: the kernels keep every access in bounds whatever
+ *    they hold, and each operator says what a bad one gives.
  *  - Outputs do not overlap inputs or each other, except where an operator allows it.
  *  - Packed batches: `offsets` holds sequences + 1 ascending row numbers; rows
  *    [offsets[s], offsets[s + 1]) are sequence s, which may be empty.  Rows before the first or

@@ -102,6 +102,8 @@ class OperatorCall {
     // refused before anything ran, and the device is well
     if (e == cudaErrorInvalidResourceHandle)
       return invalid("the stream is not one of the current device");
+    if (e >= cudaErrorStreamCaptureUnsupported && e <= cudaErrorStreamCaptureWrongThread)
+      return invalid("not taken by the capture of a stream");  // that is lost, or would be
     if (e == cudaErrorInvalidConfiguration) return invalid("more work than one launch takes");
     char text[256];
     snprintf(text, sizeof text, "%s: %s", name_, cudaGetErrorString(e));
