@@ -417,7 +417,7 @@ int64_t tb_head_rotate_workspace(int64_t dim);
 
 /* log softmax(scale * logits[n])[targets[n]] of every row.  A row counts as hidden where its
  * target is negative or its logits are all -inf: its log probability is 0.  A target of vocab or
- * more gives NaN.  scale > 0 is the inverse temperature. */
+ * more gives NaN.  scale, above 0 and at most 2e38, is the inverse temperature. */
 int tb_token_logp(int64_t element, const void* logits, int64_t row_stride, const int32_t* targets,
                   int64_t rows, int64_t vocab, double scale, float* logp, void* stream);
 

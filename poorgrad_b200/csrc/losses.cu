@@ -775,7 +775,9 @@ const char* check_logits(int64_t element, int64_t rows, int64_t vocab, int64_t s
   if (!extents_fit({rows, vocab}) || !extents_fit({rows, stride}) || rows > INT32_MAX)
     return "extents out of range";
   if (rows > 0 && vocab < 1) return "an empty vocabulary";
-  if (!(scale > 0) || scale > 3e38 || (float)scale == 0.0f) return "scale is positive and finite";
+  // scale log2(e) has to be finite too
+  if (!(scale > 0) || scale > 2e38 || (float)scale == 0.0f)
+    return "scale is positive and at most 2e38";
   if (rows > 0 && !logits) return "a required array is NULL";
   if (!aligned_to(logits, element == TB_ELEMENT_F32 ? 4 : 2))
     return "an array is not aligned to its elements";
