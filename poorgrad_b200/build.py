@@ -9,11 +9,13 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
 import sys
 import sysconfig
+from typing import Optional
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 OUT = os.path.join(HERE, "libtopos_b200.so")
 BINDING = os.path.join(HERE, "_operators.so")
+BINDING_STAMP = os.path.join(HERE, "_operators.stamp")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-contract=off",
@@ -43,14 +46,20 @@ def _compile(src: str) -> str:
     return obj
 
 
-def build_binding(force: bool = False) -> str:
-    """Compiles ``csrc/python/operators_binding.cpp`` against torch and the library."""
+def build_binding(force: bool = False) -> Optional[str]:
+    """Compiles ``csrc/python/operators_binding.cpp`` against torch and the library; where there is no
+    torch, nothing, for then nobody has a tensor to pass."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    torch = os.path.dirname(spec.origin)
+    # another torch or Python has another layout, whatever the files' times say
+    stamp = f"torch {importlib.metadata.version('torch')} in {torch}, Python {sys.version}\n"
     src = os.path.join(CSRC, "python", "operators_binding.cpp")
     deps = [src, os.path.join(ROOT, "include", "topos_b200.h")]
-    if (not force and os.path.exists(BINDING)
+    if (not force and os.path.exists(BINDING) and _text(BINDING_STAMP) == stamp
             and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps)):
         return BINDING
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", src, "-o", BINDING,
            f"-I{os.path.join(torch, 'include')}", f"-I{sysconfig.get_paths()['include']}",
            "-I/usr/local/cuda/include", f"-L{os.path.join(torch, 'lib')}", "-ltorch_python", "-ltorch",
@@ -60,7 +69,17 @@ def build_binding(force: bool = False) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {src}:\n{res.stdout}\n{res.stderr}")
+    with open(BINDING_STAMP, "w") as f:
+        f.write(stamp)
     return BINDING
+
+
+def _text(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
 
 
 def build(force: bool = False) -> str:
