@@ -327,7 +327,7 @@ int tb_gemm_f32_noalloc(const float* a, const int64_t a_strides[2], const float*
  *  - Packed batches: `offsets` holds sequences + 1 ascending row numbers; rows
  *    [offsets[s], offsets[s + 1]) are sequence s, which may be empty.  Rows before the first or
  *    behind the last offset belong to none; their outputs are left as they were, or set to 0 where
- *    `clear` names the array. */
+ *    `clear` names the array.  Offsets that do not ascend give unspecified values within the arrays. */
 
 /* Waits for the stream's work.  TB_RUNTIME (and a poisoned library) where it failed, or where a wait
  * between blocks of an operator ever ran out on the current device.  Not for a stream under capture. */
@@ -363,7 +363,8 @@ typedef struct tb_scan_desc {
   int64_t clear;                    /* TB_SCAN_CLEAR_* together, or 0 */
 } tb_scan_desc;
 /* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
- * (a decode loop's carry), `h` may be `gate` or `x` with the same strides.  An empty sequence's
+ * (a decode loop's carry; a long sequence of few channels is then not cut along time, and takes up to
+ * four times as long as with an array of its own), `h` may be `gate` or `x` with the same strides.  An empty sequence's
  * final state is its state.  Gates of the direct form may be larger than 1: steps are taken together, but
  * outputs are finite wherever the recurrence is.  Steps that together shrink what they are handed by
  * more than 2^126 may hand on nothing of it.  Where a wait between the
@@ -407,10 +408,12 @@ typedef struct tb_rotate_desc {
   int64_t workspace_bytes;
 } tb_rotate_desc;
 /* Root-mean-square norm of every query and key head, x / sqrt(mean(x^2) + epsilon) * weight, then
- * the rotation by the token's position, in one pass.  A position outside the table turns its
+ * the rotation by the token's position, in one pass.  Squares are summed in f32: elements past 1e19
+ * in magnitude overflow them.  A position outside the table turns its
  * token's heads into NaN.  q_out may be q (k_out k) with the same strides. */
 int tb_head_rotate(const tb_rotate_desc* desc, void* stream);
-/* Gradients of q, k and the weights.  q_out may be dq (k_out dk), or q (k), with the same strides. */
+/* Gradients of q, k and the weights; a token whose position is outside the table makes the weights' NaN
+ * too.  q_out may be dq (k_out dk), or q (k), with the same strides. */
 int tb_head_rotate_backward(const tb_rotate_desc* desc, void* stream);
 /* Bytes of 16-byte aligned workspace for the weight gradients of heads of `dim` elements. */
 int64_t tb_head_rotate_workspace(int64_t dim);

@@ -9,11 +9,13 @@
 // Measured on B200 (against a copy's 6.55 TB/s): the policy loss with its gradient over 8192 x 50257
 // logits, a quarter of the rows hidden, f32 485 us, 5.9 TB/s, bf16 280 us, 5.1 TB/s; the loss
 // alone f32 182 us, bf16 103 us, 6.0 TB/s.  Memory bounds the f32 forms (under load the power cap too:
-// up to 540 us in a long run), issue slots and the two exponentials a logit the bf16 ones.  Sums that
-// are carried over exactly cost rows that leave a thread two or three vectors most: 8192 x 4099 bf16
-// took 36 us before, 43 now, 3000 x 130000 f32 477 and 522; the longer bf16 rows that are only read
-// gained (123 -> 103).  The preference loss cannot know a row's slope before its pair's last row, and rows of a pair
-// do not fit the chip: it reads the logits twice, 4099 x 50257 bf16 in 181 us, 988 MB at 5.5 TB/s.
+// up to 540 us in a long run), issue slots and the two exponentials a logit the bf16 ones.  Rows that
+// leave a thread two or three vectors are furthest from that (8192 x 4099 bf16 43 us, 3.1 TB/s): sums that
+// are carried over exactly cost them most (36 us before; 3000 x 130000 f32 477 and 522), and where a
+// group of a thread's vectors is odd its last one goes with one that is not there, at a whole vector's
+// exponentials.  The longer bf16 rows that are only read gained (123 -> 103).  The preference loss cannot
+// know a row's slope before its pair's last row.  It takes all rows' statistics before any gradient, so the
+// logits are read twice: 4099 x 50257 bf16 in 184 us, 988 MB at 5.4 TB/s.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -41,6 +43,10 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^-f, which is as low: it is what the sum is divided by in the end, and a row of one likely token comes
 // out right to the last bit.  Where k top is past 2^21, f is 0 and the factors are rounded.
 // A sum of 0: no logit above -inf.
+// An exponential's argument is one rounded sum, so a term d below the top has a relative error of about
+// 2^-25 d besides the instruction's own (7e-7 at 24 below, where expf would leave 5e-8), and below 2^-126
+// it is 0.  Such terms weigh that little in the sums; in the gradient of an f32 row they stand alone, and
+// two more instructions a logit would be needed there.
 struct RowStats {
   float top, sum;
 };
@@ -729,7 +735,8 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_preference_gradient(tb_preference_desc d) {
   pdl_entry();
   if (blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(d);
-  // from the last row back: the rows that were read last are still in the L2 cache
+  // from the last row back, for the rows that were read last may still be in the L2 cache (32 of 288 MB
+  // are: 4099 x 50257 bf16 reads 256 from memory here)
   const int64_t n = d.rows - 1 - blockIdx.x;
   const T* z = (const T*)d.logits + n * d.logits_stride;
   T* out = (T*)d.gradient + n * d.gradient_stride;

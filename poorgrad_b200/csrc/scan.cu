@@ -8,12 +8,13 @@
 // parts are reduced by a launch of their own first.
 //
 // Measured on B200 (bytes moved over time, against a copy's 6.55 TB/s): 16 x 512 x 4096 bf16 direct
-// forward 36 us, 5.6 TB/s; 32 x 4096 x 512 bf16 sigmoid forward 82 us, 4.9 TB/s, backward 160 us,
-// 5.0 TB/s; a packed 131072 x 768 bf16 forward in two launches 169 us, which read 403 MB at 5.7 and
-// read and write 604 MB at 6.0 TB/s.  What bounds it: 31 (direct forward) to 94 (sigmoid backward)
-// instructions a pair of elements, issued by the sixteen warps a SM that 128 registers each leave (issue slots half busy, the rest
-// waiting for rows and for the exchange of maps).  Copies through shared memory several runs ahead
-// were slower (16 x 512 x 4096: 44 us), and so were lanes of four bf16 (8 x 1024 x 768: 25 us for 15).
+// forward 36 us, 5.6 TB/s; 32 x 4096 x 512 bf16 direct forward 74 us, 5.4 TB/s, sigmoid forward 82 us,
+// 4.9 TB/s, backward 157 us, 5.1 TB/s; a packed 131072 x 768 bf16 direct forward in two launches 170 us,
+// which read 403 MB and read and write 604 MB, both inputs from memory each time.  What bounds it: 31
+// (direct forward) to 94 (sigmoid backward) instructions a pair of elements, issued by the sixteen warps a
+// SM that 128 registers each leave (issue slots half busy, the rest waiting for rows and for the exchange
+// of maps).  Copies through shared memory several runs ahead were slower (16 x 512 x 4096: 44 us), and so
+// were lanes of four bf16 (8 x 1024 x 768: 25 us for 15).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -96,7 +97,10 @@ struct Raw<bf16, 2> {
 };
 
 // The bare instructions: the intrinsics around them also serve denormals, which do not matter here
-// and cost half of the instructions of a sigmoid.
+// and cost half of the instructions of a sigmoid.  The argument of the power of two is one rounded
+// product, so that 1 - a, where it is small, has a relative error of up to 2^-24 |g| besides the
+// instructions' own, as of a gate that is off by one rounding (6e-7 at gates of 10, where expf would leave
+// 1e-7).
 __device__ __forceinline__ float ex2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -1055,6 +1059,7 @@ cudaError_t enqueue(const tb_scan_desc& d, cudaStream_t stream) {
   cut.part_steps = std::max<int64_t>(d.length, 1);
   const int64_t columns = d.batch * cut.tiles, spans = (d.length + span - 1) / span;
   // a state that is read and written in one call is read before it is written only within a launch
+  // (12 columns of 2048 spans take 728 us so, and 172 with a final state of its own)
   const bool carries = BACK ? d.dstate && d.dstate == d.dfinal : d.final_state && d.final_state == d.state;
   if (d.workspace && columns * spans > 0 && !carries) cut.parts = parts_of(columns, spans);
   if (cut.parts > 1) {

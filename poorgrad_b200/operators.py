@@ -66,7 +66,7 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
     ``state`` (float32,
     ``[batch or sequences, channels]``, zeros when None) comes before the first step; the returned
     final state may be written into ``state`` itself (``final_state=state``), as a decode loop
-    does.  ``out`` may be ``gate`` or ``x``."""
+    does; over a long sequence of few channels an array of its own is up to four times as fast.  ``out`` may be ``gate`` or ``x``."""
     return _native.gated_scan(gate, x, _one_of(_FORM, "form", form), state, offsets, out,
                               final_state)
 
@@ -115,7 +115,7 @@ def head_rotate_backward(dq, dk, q, k, table, positions=None, *, q_weight=None, 
                          weights: bool = True):
     """Gradients ``(q_grad, k_grad, q_weight_grad, k_weight_grad)`` of :func:`head_rotate` from the
     gradients ``dq`` and ``dk`` of its outputs; the last two are float32 ``[dim]``, or None with
-    ``weights=False``.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
+    ``weights=False``, and NaN where a token's position is outside the table.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
     return _native.head_rotate_backward(q, k, table, positions, q_weight, k_weight, epsilon,
                                         _one_of(_STYLE, "style", style), q_out, k_out, dq, dk,
                                         bool(weights))
