@@ -364,16 +364,16 @@ typedef struct tb_scan_desc {
 } tb_scan_desc;
 /* Gated linear recurrence over time, per channel and sequence.  `final_state` may be `state`
  * (a decode loop's carry; a long sequence of few channels is then not cut along time, and takes up to
- * four times as long as with an array of its own), `h` may be `gate` or `x` with the same strides.  An empty sequence's
- * final state is its state.  Gates of the direct form may be larger than 1: steps are taken together, but
- * outputs are finite wherever the recurrence is.  Steps that together shrink what they are handed by
- * more than 2^126 may hand on nothing of it.  Where a wait between the
- * blocks of one sequence runs out (4 s; nothing but a fault explains it), the values carried over from
- * there on are NaN, and tb_operators_synchronize tells of it. */
+ * four times as long as with an array of its own), `h` may be `gate` or `x` with the same strides.
+ * An empty sequence's final state is its state.  Gates of the direct form may be larger than 1: steps
+ * are taken together, but outputs are finite wherever the recurrence is.  Steps that together shrink
+ * what they are handed by more than 2^126 may hand on nothing of it.  Where a wait between the blocks of
+ * one sequence runs out (4 s; nothing but a fault explains it), the values carried over from there on
+ * are NaN, and tb_operators_synchronize tells of it. */
 int tb_gated_scan(const tb_scan_desc* desc, void* stream);
 /* Its gradients from dh and dfinal: with g_t = dh_t + a_{t+1} g_{t+1}, d a_t = g_t h_{t-1},
- * d b_t = g_t, chained through the form.  Reads the saved outputs h.  `dstate` may be `dfinal`;
- * `dgate` and `dx` may be `dh` with its strides (one of them). */
+ * d b_t = g_t, chained through the form.  Reads the saved outputs h.  `state` is what the scan
+ * began with.  `dstate` may be `dfinal`; `dgate` and `dx` may be `dh` with its strides (one of them). */
 int tb_gated_scan_backward(const tb_scan_desc* desc, void* stream);
 /* Bytes of 16-byte aligned workspace with which long sequences of few channels are cut along time
  * (0: such a call needs none).  Without it the call is served all the same, more slowly. */
@@ -409,8 +409,8 @@ typedef struct tb_rotate_desc {
 } tb_rotate_desc;
 /* Root-mean-square norm of every query and key head, x / sqrt(mean(x^2) + epsilon) * weight, then
  * the rotation by the token's position, in one pass.  Squares are summed in f32: elements past 1e19
- * in magnitude overflow them.  A position outside the table turns its
- * token's heads into NaN.  q_out may be q (k_out k) with the same strides. */
+ * in magnitude overflow them.  A position outside the table turns its token's heads into NaN.  q_out
+ * may be q (k_out k) with the same strides. */
 int tb_head_rotate(const tb_rotate_desc* desc, void* stream);
 /* Gradients of q, k and the weights; a token whose position is outside the table makes the weights' NaN
  * too.  q_out may be dq (k_out dk), or q (k), with the same strides. */

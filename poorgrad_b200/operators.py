@@ -10,11 +10,11 @@ products of a decoder's training and decode steps, on device arrays that the cal
 
 Device arrays are torch tensors (float32 or bfloat16), used as memory only: nothing here records
 gradients.  An array that is given to be written counts as changed in place, so that a backward pass
-that still needs what it held raises; no two arrays of a call share memory unless one is written over the
-other as a function says.  Arguments of one call live on one device; the work is enqueued on that device's current
-torch stream, and outputs that are not given are allocated by torch on that stream.  A malformed
-request raises ``ValueError`` or :class:`~poorgrad_b200.backend.BackendError`; there is no CPU
-fallback.
+that still needs what it held raises; no two arrays of a call share memory unless one is written over
+the other as a function says.  Arguments of one call live on one device; the work is enqueued on that
+device's current torch stream, and outputs that are not given are allocated by torch on that stream.  A
+malformed request raises ``ValueError`` or :class:`~poorgrad_b200.backend.BackendError`; there is no
+CPU fallback.
 """
 from __future__ import annotations
 
@@ -63,10 +63,10 @@ def gated_scan(gate, x, *, form: str = "sigmoid", state=None, offsets=None, out=
     ``gate`` and b is ``(1 - a) x``.  ``gate`` and ``x`` are ``[batch, length, channels]``, or a
     packed ``[rows, channels]`` whose sequences ``offsets`` (int32, sequences + 1 rising row
     numbers) delimits; rows outside every sequence are 0, or left as they were in a given array.
-    ``state`` (float32,
-    ``[batch or sequences, channels]``, zeros when None) comes before the first step; the returned
-    final state may be written into ``state`` itself (``final_state=state``), as a decode loop
-    does; over a long sequence of few channels an array of its own is up to four times as fast.  ``out`` may be ``gate`` or ``x``."""
+    ``state`` (float32, ``[batch or sequences, channels]``, zeros when None) comes before the first
+    step; the returned final state may be written into ``state`` itself (``final_state=state``), as a
+    decode loop does; over a long sequence of few channels an array of its own is up to four times as
+    fast.  ``out`` may be ``gate`` or ``x``."""
     return _native.gated_scan(gate, x, _one_of(_FORM, "form", form), state, offsets, out,
                               final_state)
 
@@ -115,7 +115,8 @@ def head_rotate_backward(dq, dk, q, k, table, positions=None, *, q_weight=None, 
                          weights: bool = True):
     """Gradients ``(q_grad, k_grad, q_weight_grad, k_weight_grad)`` of :func:`head_rotate` from the
     gradients ``dq`` and ``dk`` of its outputs; the last two are float32 ``[dim]``, or None with
-    ``weights=False``, and NaN where a token's position is outside the table.  ``q_out`` and ``k_out`` receive the first two and may be ``dq`` and ``dk``."""
+    ``weights=False``, and NaN where a token's position is outside the table.  ``q_out`` and ``k_out``
+    receive the first two and may be ``dq`` and ``dk``."""
     return _native.head_rotate_backward(q, k, table, positions, q_weight, k_weight, epsilon,
                                         _one_of(_STYLE, "style", style), q_out, k_out, dq, dk,
                                         bool(weights))
